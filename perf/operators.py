@@ -295,13 +295,13 @@ def _run_own(s, c):
     t = s["table"]
     if op == "append":
         E = c["heads"] * c["dim"]
-        g2.kv8_append(s["cache"], s["qkv"][:, E:], s["qkv"][:, 2 * E:], c["seqs"], t, t.shape[1], s["pos"],
-                      q_start=s["q_start"], max_q=c["max_q"], row_stride=3 * E, dtype=dt)
-        g2.kv8_gather(s["cache"], s["k_out"], s["v_out"], c["seqs"], t, t.shape[1], s["first"], q_start=s["b_start"],
-                      max_q=s["max_back"], dtype=F32)
+        g2.kv8_append(s["cache"], s["qkv"][:, E:], s["qkv"][:, 2 * E:], s["rows"], c["seqs"], t, t.shape[1],
+                      s["pos"], q_start=s["q_start"], max_q=c["max_q"], row_stride=3 * E, dtype=dt)
+        g2.kv8_gather(s["cache"], s["k_out"], s["v_out"], s["back"], c["seqs"], t, t.shape[1], s["first"],
+                      q_start=s["b_start"], max_q=s["max_back"], dtype=F32)
         return {"k": s["k_out"], "v": s["v_out"], "k_scale": s["k_scale"], "v_scale": s["v_scale"]}
-    g2.kv8_attention(s["cache"], s["q"], s["out"], c["kv_heads"] * c["group"], c["seqs"], t, t.shape[1], s["len"], s["ws"],
-                     s["ws"].numel(), q_start=s["q_start"], max_q=c["max_q"], dtype=dt)
+    g2.kv8_attention(s["cache"], s["q"], s["out"], c["kv_heads"] * c["group"], s["q"].shape[0], c["seqs"], t, t.shape[1],
+                     s["len"], s["ws"], s["ws"].numel(), q_start=s["q_start"], max_q=c["max_q"], dtype=dt)
     return s["out"]
 
 
