@@ -176,6 +176,7 @@ struct g2_engine {
     int *sample_ctx = nullptr;      // [n_ctx] context ids
     int *topk_out = nullptr;        // g2_topk: [G2_MAX_TOPK] values (as float) then [G2_MAX_TOPK] ids
     int *h_ctx = nullptr;           // pinned staging of the context ids
+    int *rules_buf = nullptr;       // g2_process_logits' arrays on the device (allocated by its first call)
     std::vector<TcWeights> tc_maps;           // [L][4]: qkv, proj, fc, fc2
     TcWeights tc_lm{};                        // the tied LM head: wte [V][E] as a K-major operand
     // LM head over one range of vocabulary rows (g2_lm_head_rows): its operand map and logits
@@ -212,7 +213,7 @@ static void free_engine(g2_engine *e) {
     if (e->batch_graph) cudaGraphExecDestroy(e->batch_graph);
     for (auto &kv : e->prefill_graphs)
         if (kv.second.exec) cudaGraphExecDestroy(kv.second.exec);
-    void *dev_ptrs[] = {e->shard_logits, e->sample_work, e->sample_ctx, e->topk_out, e->tc_w, e->tc_lm_w, e->tc_img, e->tc_idx, e->tc_perm, e->tc_xhi, e->tc_xlo, e->tc_x2hi, e->tc_x2lo, e->tc_ctr, e->tc_part, e->tc_err, e->d_trace, e->packed, e->d_layer_off, e->d_layers, e->t_qkv, e->mega_acc,
+    void *dev_ptrs[] = {e->rules_buf, e->shard_logits, e->sample_work, e->sample_ctx, e->topk_out, e->tc_w, e->tc_lm_w, e->tc_img, e->tc_idx, e->tc_perm, e->tc_xhi, e->tc_xlo, e->tc_x2hi, e->tc_x2lo, e->tc_ctr, e->tc_part, e->tc_err, e->d_trace, e->packed, e->d_layer_off, e->d_layers, e->t_qkv, e->mega_acc,
                         e->t_best, e->t_att, e->d_err, e->wbuf, e->kbuf, e->vbuf, e->h, e->xln, e->qkv, e->attn, e->ffn, e->logits,
                         e->logits_rows, e->gemv_partial, e->attn_partial, e->lm_partial, e->gemv_ctr,
                         e->attn_ctr, e->lm_ctr, e->rows_tok, e->rows_pos, e->rows_slot, e->result,
@@ -1568,6 +1569,55 @@ extern "C" int g2_topk(g2_engine *e, int slot, int k, float *values, int *ids) {
     CK(cudaMemcpyAsync(values, dv, sizeof(float) * k, cudaMemcpyDeviceToHost, e->st));
     CK(cudaMemcpyAsync(ids, di, sizeof(int) * k, cudaMemcpyDeviceToHost, e->st));
     return sync_and_check(e);
+}
+
+extern "C" int g2_process_logits(g2_engine *e, int slot, const g2_logit_rules *rules) {
+    NvtxRange nvtx_range("g2_process_logits");
+    const char *who = "g2_process_logits";
+    if (!e) return set_err(G2_ERR_ARG, "%s: null argument", who);
+    int rc;
+    if ((rc = check_slot(e, slot))) return rc;
+    const int V = e->c.vocab_size, words = (V + 31) / 32;
+    if ((rc = check_rules(who, rules, 1, V, false))) return rc;
+    if (rules->n_ctx > e->c.n_ctx) return set_err(G2_ERR_RANGE, "%s: %d context ids > n_ctx %d", who, rules->n_ctx, e->c.n_ctx);
+    if (rules->n_bias > V) return set_err(G2_ERR_RANGE, "%s: %d biases > vocab_size %d", who, rules->n_bias, V);
+    if (e->filled[slot] == 0) return set_err(G2_ERR_STATE, "%s: slot %d has no logits yet", who, slot);
+    CK(cudaSetDevice(e->device));
+    // [n_ctx] ids, [V] bias ids, [V] biases, [words] mask, then n_prompt and the three penalties
+    if (!e->rules_buf && (rc = dalloc(e, &e->rules_buf, (size_t)e->c.n_ctx + 2 * (size_t)V + words + 4))) return rc;
+    int *ctx = e->rules_buf, *ids = ctx + e->c.n_ctx, *bias = ids + V, *mask = bias + V, *rest = mask + words;
+    auto put = [&](int *dst, const void *src, size_t n) {
+        return n ? cudaMemcpyAsync(dst, src, 4 * n, cudaMemcpyHostToDevice, e->st) : cudaSuccess;
+    };
+    g2_logit_rules d = *rules;
+    d.ctx_start = d.bias_start = nullptr;
+    CK(put(ctx, rules->ctx, rules->n_ctx));
+    CK(put(ids, rules->bias_ids, rules->n_bias));
+    CK(put(bias, rules->bias, rules->n_bias));
+    d.ctx = ctx;
+    d.bias_ids = ids;
+    d.bias = reinterpret_cast<float *>(bias);
+    if (rules->mask) {
+        CK(put(mask, rules->mask, words));
+        d.mask = reinterpret_cast<unsigned *>(mask);
+    }
+    if (rules->n_prompt) {
+        CK(put(rest, rules->n_prompt, 1));
+        d.n_prompt = rest;
+    }
+    const float *one[3] = {rules->rep_penalty, rules->presence, rules->frequency};
+    const float **to[3] = {&d.rep_penalty, &d.presence, &d.frequency};
+    for (int i = 0; i < 3; ++i)
+        if (one[i]) {
+            CK(put(rest + 1 + i, one[i], 1));
+            *to[i] = reinterpret_cast<float *>(rest + 1 + i);
+        }
+    float *lg = e->logits + (size_t)slot * e->c.padded_vocab;
+    launch_rules(lg, e->c.padded_vocab, lg, e->c.padded_vocab, 1, V, d, e->st);
+    e->launches += 1;
+    if (e->result_slot == slot) e->result_slot = -1;   // the LM head's argmax no longer holds
+    CKL();
+    return sync_and_check(e);   // the caller's arrays are free again
 }
 
 extern "C" int g2_synchronize(g2_engine *e) {

@@ -7,6 +7,8 @@
 #include <cstddef>
 #include <cstdint>
 
+struct g2_logit_rules;
+
 namespace g2 {
 
 // Launch a kernel with programmatic dependent launch (it may start while the
@@ -111,6 +113,11 @@ void launch_sample(const float *logits, float *work, int V, const int *ctx, int 
 // The k (<= G2_MAX_TOPK) largest of logits[0..V) on the device (g2_sample_dev.cu):
 // vals / idx [k], the larger value first, equal values by the smaller index.
 void launch_topk(const float *logits, int V, int k, float *vals, int *idx, cudaStream_t st);
+
+// Rules on rows of logits (g2_logits.cu): the host checks, and the kernel with `rules` in device memory.
+int check_rules(const char *who, const g2_logit_rules *r, int rows, int vocab, bool device);
+void launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
+                  const g2_logit_rules &rules, cudaStream_t st);
 
 template <typename WT>
 void launch_embed(const WT *wte, const WT *wpe, Rows rows, float *h, int E, int V, int n_pos, int nrows,

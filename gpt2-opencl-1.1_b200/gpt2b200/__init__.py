@@ -20,6 +20,8 @@ PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("G2_LIB") or os.path.join(PKG_DIR, "libgpt2b200.so")
 
 G2_F32, G2_F16 = 0, 1
+G2_KV_I8, G2_KV_E4M3 = 0, 1
+MASKED = -1e30   # G2_MASKED
 EOS = 50256
 ERRORS = {-1: "ARG", -2: "IO", -3: "FORMAT", -4: "CUDA", -5: "OOM", -6: "RANGE", -7: "STATE", -8: "TIMEOUT"}
 
@@ -35,6 +37,21 @@ class Config(C.Structure):
                 ("vocab_size", C.c_int), ("ffn_dim", C.c_int), ("padded_vocab", C.c_int), ("dtype", C.c_int),
                 ("max_batch", C.c_int), ("device", C.c_int), ("weight_bytes", C.c_size_t),
                 ("device_bytes", C.c_size_t), ("persistent", C.c_int)]
+
+
+class KV8(C.Structure):
+    """g2_kv8: a paged cache of 8-bit codes (make one with kv8_cache)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int), ("n_kv_head", C.c_int), ("page_size", C.c_int), ("head_dim", C.c_int),
+                ("format", C.c_int)]
+
+
+class LogitRules(C.Structure):
+    """g2_logit_rules (make one with logit_rules)."""
+    _fields_ = [("ctx", C.c_void_p), ("ctx_start", C.c_void_p), ("n_prompt", C.c_void_p), ("n_ctx", C.c_int),
+                ("rep_penalty", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_start", C.c_void_p), ("n_bias", C.c_int),
+                ("mask", C.c_void_p), ("mask_stride", C.c_int)]
 
 
 def _load():
@@ -82,6 +99,19 @@ def _load():
     L.g2k_attention_workspace.restype = C.c_size_t
     L.g2k_attention.argtypes = [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_size_t, vp]
     L.g2k_topk.argtypes = [vp, C.c_int, C.c_int, vp, vp, vp]
+    i, ll, sz = C.c_int, C.c_longlong, C.c_size_t
+    L.g2k_q4_bytes.argtypes = [i, i, i]
+    L.g2k_q4_bytes.restype = sz
+    L.g2k_q4_pack.argtypes = [vp, i, i, vp, i, i, i, vp]
+    L.g2k_q4_unpack.argtypes = [vp, vp, i, i, i, vp]
+    L.g2k_matvec_q4.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, vp, vp]
+    L.g2k_kv8_append.argtypes = [vp, vp, vp, i, ll, i, i, vp, vp, i, vp, i, vp, vp]
+    L.g2k_kv8_gather.argtypes = [vp, vp, vp, i, ll, i, i, vp, vp, i, vp, i, vp, vp]
+    L.g2k_kv8_attention_workspace.argtypes = [vp, i, i, i]
+    L.g2k_kv8_attention_workspace.restype = sz
+    L.g2k_kv8_attention.argtypes = [vp, vp, ll, vp, ll, i, i, C.c_float, i, i, vp, vp, i, vp, i, vp, sz, vp, vp]
+    L.g2k_process_logits.argtypes = [vp, ll, vp, ll, i, i, vp, vp]
+    L.g2_process_logits.argtypes = [vp, i, vp]
     return L
 
 
@@ -183,6 +213,33 @@ class Engine:
         check(lib.g2_sample_device(self.h, slot, p, len(a), int(forbid_eos), temperature, top_k, rep_penalty, u,
                                    C.byref(t)))
         return t.value
+
+    def process_logits(self, context=(), n_prompt: int = 0, rep_penalty: float = 1.0, presence: float = 0.0,
+                       frequency: float = 0.0, bias=None, allowed=None, slot: int = 0):
+        """The rules of g2_process_logits on the logits of `slot`, in place: penalties over the ids of
+        `context` (`presence` and `frequency` over those after the first `n_prompt`), `bias` as a dict
+        of id -> value, and `allowed` as the ids or a truth value per id that stay possible."""
+        V = self.cfg.vocab_size
+        ctx = np.ascontiguousarray(context, np.int32)
+        ids = np.ascontiguousarray(list(bias or ()), np.int32)
+        val = np.ascontiguousarray(list((bias or {}).values()), np.float32)
+        one = np.array([rep_penalty, presence, frequency], np.float32)
+        n = np.array([n_prompt], np.int32)
+        r = LogitRules(ctx=ctx.ctypes.data, n_ctx=ctx.size, n_prompt=n.ctypes.data, rep_penalty=one[0:].ctypes.data,
+                       presence=one[1:].ctypes.data, frequency=one[2:].ctypes.data, bias_ids=ids.ctypes.data,
+                       bias=val.ctypes.data, n_bias=ids.size)
+        if allowed is not None:
+            a = np.asarray(allowed)
+            ok = np.zeros(-(-V // 32) * 32, bool)
+            if a.dtype == bool:
+                if a.shape != (V,):
+                    raise G2Error(-1, f"allowed has {a.shape} truth values, not one for each of {V} ids")
+                ok[:V] = a
+            else:
+                ok[a.astype(np.int64)[(a >= 0) & (a < V)]] = True
+            words = np.packbits(ok, bitorder="little").view("<u4")
+            r.mask = words.ctypes.data
+        check(lib.g2_process_logits(self.h, slot, C.byref(r)))
 
     def generate(self, prompt, n_new: int, min_new: int = None, slot: int = 0) -> np.ndarray:
         a, p = _i32(prompt)
@@ -329,3 +386,94 @@ def attention_workspace(n_head: int, max_seq: int) -> int:
 def attention(q, K, V, out, n_head, max_seq, T_kv, workspace, workspace_bytes, stream=0):
     check(lib.g2k_attention(_ptr(q), _ptr(K), _ptr(V), _ptr(out), n_head, max_seq, T_kv, _ptr(workspace),
                             workspace_bytes, C.c_void_p(stream)))
+
+
+# ---- 4-bit weights, the 8-bit paged cache, rules on logits: kernels on device pointers ----
+def _addr(t):
+    """The device address of a tensor (or an int); other memory is refused here, before a kernel sees it."""
+    if t is None or isinstance(t, int):
+        return t
+    if not t.is_cuda:
+        raise G2Error(-1, "a tensor is not in device memory")
+    return t.data_ptr()
+
+
+def q4_bytes(N: int, K: int, group: int) -> int:
+    """Bytes of a [K, N] weight matrix packed in 4 bits (0 for a bad shape or group)."""
+    return lib.g2k_q4_bytes(N, K, group)
+
+
+def q4_pack(W, packed, N, K, group, transposed=False, dtype=G2_F32, stream=0):
+    """Quantise W ([K, N], or [N, K] if transposed) to 4 bits with a scale for each `group` rows of a column."""
+    check(lib.g2k_q4_pack(_addr(W), dtype, int(transposed), _addr(packed), N, K, group, stream))
+
+
+def q4_unpack(packed, W, N, K, group, stream=0):
+    """The values of a packed matrix, fp32 [K, N]."""
+    check(lib.g2k_q4_unpack(_addr(packed), _addr(W), N, K, group, stream))
+
+
+def matvec_q4(x, packed, y, M, N, K, group, bias=None, residual=None, gelu=False, ln_gamma=None, ln_beta=None,
+              dtype=G2_F32, stream=0):
+    """y [M, N] = x' [M, K] times a packed [K, N] matrix; M up to 16 rows; x, residual and y of `dtype`."""
+    check(lib.g2k_matvec_q4(_addr(x), _addr(packed), _addr(bias), _addr(residual), _addr(y), dtype, M, N, K, group,
+                            int(gelu), _addr(ln_gamma), _addr(ln_beta), stream))
+
+
+def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
+    """A paged 8-bit cache over the caller's tensors: k, v [n_pages, n_kv_head, page_size, head_dim] of one
+    byte each, the scales fp32 [n_pages, n_kv_head].  The cache keeps the tensors alive."""
+    shape = tuple(k.shape)
+    if len(shape) != 4 or tuple(v.shape) != shape or k.element_size() != 1 or v.element_size() != 1:
+        raise G2Error(-1, "k and v are one-byte tensors [n_pages, n_kv_head, page_size, head_dim]")
+    if tuple(k_scale.shape) != shape[:2] or tuple(v_scale.shape) != shape[:2] or k_scale.element_size() != 4 \
+            or v_scale.element_size() != 4:
+        raise G2Error(-1, "the scales are fp32 tensors [n_pages, n_kv_head]")
+    if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+        raise G2Error(-1, "the cache's tensors are not contiguous")
+    c = KV8(_addr(k), _addr(v), _addr(k_scale), _addr(v_scale), *shape, fmt)
+    c.tensors = (k, v, k_scale, v_scale)
+    return c
+
+
+def kv8_append(cache, k, v, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0, dtype=G2_F32,
+               status=None, stream=0):
+    """Write K and V rows of new tokens into the pages of their sequences (g2k_kv8_append)."""
+    check(lib.g2k_kv8_append(C.byref(cache), _addr(k), _addr(v), dtype, row_stride, n_rows, n_seq, _addr(q_start),
+                             _addr(pos), max_q, _addr(table), table_stride, _addr(status), stream))
+
+
+def kv8_gather(cache, k_out, v_out, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0,
+               dtype=G2_F32, status=None, stream=0):
+    """Read rows of the cache back as values (g2k_kv8_gather)."""
+    check(lib.g2k_kv8_gather(C.byref(cache), _addr(k_out), _addr(v_out), dtype, row_stride, n_rows, n_seq, _addr(q_start),
+                             _addr(pos), max_q, _addr(table), table_stride, _addr(status), stream))
+
+
+def kv8_attention_workspace(cache, n_head: int, n_seq: int, max_q: int = 1) -> int:
+    return lib.g2k_kv8_attention_workspace(C.byref(cache), n_head, n_seq, max_q)
+
+
+def kv8_attention(cache, q, out, n_head, n_rows, n_seq, table, table_stride, seq_len, workspace, workspace_bytes,
+                  q_start=None, max_q=1, scale=None, q_stride=0, out_stride=0, dtype=G2_F32, status=None, stream=0):
+    """Softmax attention of query rows over the cache (g2k_kv8_attention); scale defaults to head_dim ** -0.5."""
+    check(lib.g2k_kv8_attention(C.byref(cache), _addr(q), q_stride, _addr(out), out_stride, dtype, n_head,
+                                cache.head_dim ** -0.5 if scale is None else scale, n_rows, n_seq, _addr(q_start),
+                                _addr(seq_len), max_q, _addr(table), table_stride, _addr(workspace), workspace_bytes,
+                                _addr(status), stream))
+
+
+def logit_rules(ctx=None, ctx_start=None, n_prompt=None, rep_penalty=None, presence=None, frequency=None, bias_ids=None,
+                bias=None, bias_start=None, mask=None, mask_stride=0) -> LogitRules:
+    """Rules on rows of logits over the caller's device tensors (g2_logit_rules), which it keeps alive."""
+    r = LogitRules(_addr(ctx), _addr(ctx_start), _addr(n_prompt), 0 if ctx is None else ctx.numel(), _addr(rep_penalty),
+                   _addr(presence), _addr(frequency), _addr(bias_ids), _addr(bias), _addr(bias_start),
+                   0 if bias is None else bias.numel(), _addr(mask), mask_stride)
+    r.tensors = (ctx, ctx_start, n_prompt, rep_penalty, presence, frequency, bias_ids, bias, bias_start, mask)
+    return r
+
+
+def process_logits(logits, out, rows, vocab_size, rules, ld=0, ld_out=0, stream=0):
+    """Apply `rules` to rows of logits (out may be logits); a row stride of 0 means vocab_size."""
+    check(lib.g2k_process_logits(_addr(logits), ld or vocab_size, _addr(out), ld_out or vocab_size, rows, vocab_size,
+                                 C.byref(rules), stream))

@@ -234,6 +234,142 @@ int g2k_attention(const float *q, const float *K, const float *V, float *out, in
  * Asynchronous on `stream`. */
 int g2k_topk(const float *logits, int n, int k, float *values, int *ids, void *stream);
 
+/* ---- 4-bit weights ----------------------------------------------------------
+ * A weight matrix W [K][N] as 4-bit codes in -7..7 with one scale for each
+ * `group` consecutive rows (32, 64 or 128; the last group may be shorter) of
+ * each column: scale = bf16(fp32(max |w| / 7)), code = w / scale rounded to
+ * nearest even and clamped (0 where the scale is 0), the value code * scale.
+ * An infinite or NaN weight makes its group's values NaN.  Any K and N >= 1.
+ * The packed layout is this library's own: move it as bytes.
+ *
+ * g2k_q4_bytes: bytes of a packed matrix (0 for a bad shape or group).
+ * g2k_q4_pack: from W on the device, dtype G2_F32 or G2_F16, Conv1D [K][N], or
+ * nn.Linear [N][K] if `transposed`.  packed: 256-byte aligned.
+ * g2k_q4_unpack: the values, fp32 [K][N]. */
+size_t g2k_q4_bytes(int N, int K, int group);
+int g2k_q4_pack(const void *W, int dtype, int transposed, void *packed, int N, int K, int group, void *stream);
+int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *stream);
+
+/* g2k_matvec on a packed matrix, for M = 1..G2_Q4_MAX_ROWS rows:
+ * y[m][n] = sum_k x'[m][k] * W[k][n] (+bias[n]) (then GELU) (+residual[m][n]),
+ * x' = LayerNorm(x; ln_gamma, ln_beta, eps 1e-5) when ln_gamma is not NULL.
+ * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
+ * ln_gamma and ln_beta are fp32.  Sums are fp32; with G2_F32 the operands
+ * carry 22 bits of each x', with G2_F16 too after a LayerNorm, else x exactly.
+ * residual may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls on
+ * different streams may overlap. */
+#define G2_Q4_MAX_ROWS 16
+#define G2_Q4_MAX_K 32768
+int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const void *residual, void *y, int dtype,
+                  int M, int N, int K, int group, int apply_gelu, const float *ln_gamma, const float *ln_beta,
+                  void *stream);
+
+/* ---- 8-bit paged KV cache -----------------------------------------------------
+ * K and V rows as 8-bit codes in pages of page_size tokens, one fp32 scale for
+ * each page and head: the value of a code c is c * scale.  Code j of token t of
+ * head h of page p is at ((p * n_kv_head + h) * page_size + t) * head_dim + j;
+ * its scale at p * n_kv_head + h.  The caller owns the memory and which pages
+ * a sequence has: `table` [n_seq][table_stride] (device) lists them in order.
+ * All arrays below are in device memory unless said otherwise.
+ *
+ * Rows: with q_start NULL sequence s has the one row s (n_rows == n_seq, max_q
+ * 1); else rows q_start[s] .. q_start[s+1]-1, at most max_q of them.  Rows that
+ * no sequence has are left as they were.  Row i of head h is at element
+ * i * stride + h * head_dim; a stride of 0 means heads * head_dim, others let
+ * rows be parts of wider ones (the thirds of a c_attn row).  Base pointers and
+ * strides in bytes are multiples of 16.
+ *
+ * A sequence with a count outside [0, max_q], rows outside [0, n_rows), or a
+ * position or length outside its table row is skipped, and so is a page whose
+ * id is outside [0, n_pages); *status (may be NULL) then becomes G2_ERR_RANGE.
+ * It is never cleared here. */
+#define G2_KV_I8 0      /* int8 codes in -127..127 */
+#define G2_KV_E4M3 1    /* fp8 e4m3 codes, finite, up to 448 */
+typedef struct g2_kv8 {
+    void *k, *v;                /* 16-byte aligned codes */
+    float *k_scale, *v_scale;
+    int n_pages, n_kv_head;
+    int page_size;              /* 16, 32, 64 or 128 tokens */
+    int head_dim;               /* 64 or 128 */
+    int format;                 /* G2_KV_I8 or G2_KV_E4M3 */
+} g2_kv8;
+
+/* Write the K and V rows (dtype G2_F32 or G2_F16) of new tokens: row j of
+ * sequence s goes to position pos[s] + j.  For each page and head that receives
+ * rows: scale = max(max |x| / 127 (or 448) over the new rows, 2^-64), and, where
+ * rows below pos[s] stay in the page, at least its old scale; if that grew, the
+ * rows that stay are rounded again to the new scale.  Codes are value / scale
+ * rounded to nearest even (the exact quotient).  A non-finite row makes the
+ * scale, and so every value, of its page and head NaN, until the page is
+ * written anew from its first token.  Pages that receive rows must belong to
+ * one sequence of the call only. */
+int g2k_kv8_append(const g2_kv8 *cache, const void *k, const void *v, int dtype, long long row_stride, int n_rows,
+                   int n_seq, const int *q_start, const int *pos, int max_q, const int *table, int table_stride,
+                   int *status, void *stream);
+
+/* Read rows back as values (G2_F32: code * scale exactly rounded; G2_F16): row
+ * j of sequence s is position pos[s] + j. */
+int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int dtype, long long row_stride, int n_rows,
+                   int n_seq, const int *q_start, const int *pos, int max_q, const int *table, int table_stride,
+                   int *status, void *stream);
+
+/* g2k_attention over the cache, for the query rows of several sequences: with
+ * n rows in sequence s and seq_len[s] tokens in its cache (the new ones
+ * included), row j attends to positions 0 .. seq_len[s] - n + j; a row with no
+ * position gives zeros.  Query head h reads K/V head h / (n_head / n_kv_head).
+ * q and out are of `dtype`; sums are fp32, and so is the accuracy of G2_F32.
+ * scale multiplies q . k (1 / sqrt(head_dim)).  Keys of a skipped page count
+ * as absent.  `workspace` holds g2k_kv8_attention_workspace() bytes,
+ * 256-byte aligned, zero-filled before its first use; each call leaves it ready
+ * for the next.  Calls (and captured graphs) that may overlap need one each. */
+size_t g2k_kv8_attention_workspace(const g2_kv8 *cache, int n_head, int n_seq, int max_q);
+int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q_stride, void *out, long long out_stride,
+                      int dtype, int n_head, float scale, int n_rows, int n_seq, const int *q_start,
+                      const int *seq_len, int max_q, const int *table, int table_stride, void *workspace,
+                      size_t workspace_bytes, int *status, void *stream);
+
+/* ---- rules on logits ------------------------------------------------------------
+ * What to do to each row of logits before a token is picked, in this order;
+ * NULL arrays are left out:
+ *  1. repetition penalty (main.c:1885-1895): each distinct id of the row's
+ *     context once, l > 0 ? l / rep_penalty[r] : l * rep_penalty[r]
+ *     (a value <= 0 counts as 1);
+ *  2. l -= frequency[r] * c + presence[r] for each id that occurs c > 0 times
+ *     after the first n_prompt[r] ids of the context (n_prompt NULL: 0);
+ *  3. l += bias of the row's (bias_ids, bias) pairs; of pairs with the same id
+ *     the last one counts;
+ *  4. a token whose bit is 0 in the row's grammar mask becomes G2_MASKED, the
+ *     value that the samplers treat as removed: bit v % 32 of word
+ *     mask[r * mask_stride + v / 32] (mask_stride 0: one mask for every row).
+ * Row r's context is ctx[ctx_start[r] .. ctx_start[r+1]), its pairs are
+ * bias_ids / bias[bias_start[r] .. bias_start[r+1]); ids outside the vocabulary
+ * are ignored, and so are entries outside [0, n_ctx) or [0, n_bias). */
+#define G2_MASKED (-1e30f)
+typedef struct g2_logit_rules {
+    const int *ctx, *ctx_start, *n_prompt;
+    int n_ctx;
+    const float *rep_penalty, *presence, *frequency;   /* [rows] */
+    const int *bias_ids;
+    const float *bias;
+    const int *bias_start;
+    int n_bias;
+    const unsigned *mask;
+    int mask_stride;            /* words */
+} g2_logit_rules;
+
+/* Apply the rules (arrays in device memory) to rows 0..rows-1 of logits
+ * [rows][ld] over columns 0..vocab_size-1; the result goes to out [rows][ld_out],
+ * whose other columns are left as they were.  out may be logits (same ld). */
+int g2k_process_logits(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab_size,
+                       const g2_logit_rules *rules, void *stream);
+
+/* The rules on the logits of `slot`, in place, so that g2_argmax, g2_topk,
+ * g2_sample_device and g2_logits see the result.  Arrays in `rules` are host
+ * arrays of one row; ctx_start and bias_start are not read (the row has all
+ * n_ctx ids and n_bias pairs).  n_ctx <= n_ctx of the model, n_bias <=
+ * vocab_size. */
+int g2_process_logits(g2_engine *e, int slot, const g2_logit_rules *rules);
+
 #ifdef __cplusplus
 }
 #endif
