@@ -213,74 +213,566 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- attention --------------------------------------------------------------------
-// One CTA for each query row and head, keys in tiles of 128: a key per thread
-// for the scores, a dimension per thread for the sums, with the running
-// maximum and sum of the softmax carried from tile to tile.
-constexpr int kAttnThreads = 128;
+// out_i = sum_j w_ij c_j / sum_j w_ij / vs_j,   w_ij = 2^(t_ij - m_i),
+// t_ij = (q_i . k_j) ks_j scale log2(e) + log2(vs_j),
+// with k_j, c_j the integer (or e4m3) codes of a key's K and V rows and ks_j,
+// vs_j the scales of its page: the V scale rides in the exponent, so a key
+// costs no multiplication for either scale.
+//
+// A *run* is the keys of one sequence under one K/V head for a group of up to
+// 4 NT query columns (column c of a sequence: row c / group, head c % group).
+// Runs are cut into units of `unit` keys; all units, in order, are shared
+// equally among the workers (WPR warps each), so the shares do not depend on
+// how ragged the sequences are.  A run that crosses shares leaves partial
+// results (m, sum, accumulators) in the workspace; the last worker to arrive
+// merges them in order, so results do not depend on timing.
+//
+// A warp takes tiles of 16 keys.  Each tile's codes and scales are copied by
+// cp.async into the warp's own ring of kStages slots, so that the copies of the
+// next tiles are always in flight and no barrier is needed beyond the warp.
+// Both products run on the tensor cores (m16n8k16, fp16 operands, fp32 sums):
+//   scores   keys on m, query columns on n;
+//   outputs  dimensions on m, query columns on n, keys on k.
+// 8-bit codes are exact in fp16.  Each query and each weight takes two columns,
+// its fp16 rounding and 2^11 times the rest (22 bits together), which fill
+// columns that a few queries leave idle.  Both lie in the same thread, so
+// neither product needs a shuffle, and `movmatrix` turns the weights into the
+// second product's operand.  Operand orders are permuted (dimensions of the
+// scores' k, of the outputs' m) so that every thread reads 8 or 16 consecutive
+// bytes; the ring's slots are swizzled so that those reads have no bank
+// conflicts.
+//
+// The running reference m is raised only when a score exceeds it by 2^8: one
+// vote a tile in place of a maximum over the warp.
+constexpr int kAttnWarps = 8;
+constexpr int kMaxWorkers = 4096;   // counters at the start of the workspace
+constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
+constexpr float kNoMax = -1e30f;    // reference of a column that has seen no key
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kAttnThreads)
-    kv8_attention_kernel(g2_kv8 c, const T *q, long long q_stride, T *out, long long out_stride, int group, float scale,
-                         const int *seq_len, Rows8 r) {
-    __shared__ float qs[128], ps[kAttnThreads], red[kAttnThreads / 32];
-    __shared__ int pages[kAttnThreads];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int s = blockIdx.x / r.max_q, j = blockIdx.x % r.max_q, h = blockIdx.y, kh = h / group;
-    const int P = c.page_size, D = c.head_dim;
-    const Span sp = seq_rows(r, s);
-    if (j >= sp.n) return;
-    const int len = seq_len[s];
-    if (len < 0 || len > (long long)r.table_stride * P) {
-        bad(r);
-        return;
+template <int D>
+struct AttnRing {
+    static constexpr int kStages = D == 64 ? 6 : 3;
+    static constexpr int kTileBytes = 32 * D;   // 16 keys' K and V codes
+    static constexpr int kSmem = kAttnWarps * kStages * (kTileBytes + 16);
+};
+
+struct AttnArgs {
+    g2_kv8 c;
+    const void *q;
+    void *out;
+    long long q_stride, out_stride;
+    int f16, group;
+    float scale_log2e;
+    const int *seq_len;
+    Rows8 r;
+    int unit, workers;       // most workers; fewer where there are fewer units
+    unsigned *counters;      // [kMaxWorkers], zero between calls
+    float *parts;            // [workers][2][columns * (D + 2)]
+};
+
+__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(unsigned dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(unsigned dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned transpose8x8(unsigned v) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Four codes to two fp16 pairs, exactly.  int8: code + 128 put below the exponent of 1024, minus 1152.
+template <int FMT>
+__device__ __forceinline__ void codes_to_half(unsigned w, unsigned &lo, unsigned &hi) {
+    if (FMT == G2_KV_I8) {
+        w ^= 0x80808080u;
+        const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+        unsigned a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off), y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+        lo = *reinterpret_cast<const unsigned *>(&x);
+        hi = *reinterpret_cast<const unsigned *>(&y);
+    } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     }
-    const int keys = len - sp.n + j + 1;
-    const long long row = sp.first + j;
-    if (t < D) qs[t] = tof(q[row * q_stride + (long long)h * D + t]) * scale;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int k0 = 0; k0 < keys; k0 += kAttnThreads) {
-        __syncthreads();
-        const int key = k0 + t;
-        float sc = -INFINITY;
-        pages[t] = -1;
-        if (key < keys) {
-            const int page = page_of(r, c, s, key / P);
-            pages[t] = page;
-            if (page >= 0) {
-                const long long at = (long long)page * c.n_kv_head + kh;
-                const unsigned char *p = static_cast<const unsigned char *>(c.k) + (at * P + key % P) * D;
-                float dot = 0.0f;
-                for (int d = 0; d < D; d += 4) {
-                    const unsigned w = *reinterpret_cast<const unsigned *>(p + d);
-                    dot += qs[d] * decode<FMT>(w & 0xffu) + qs[d + 1] * decode<FMT>((w >> 8) & 0xffu) +
-                           qs[d + 2] * decode<FMT>((w >> 16) & 0xffu) + qs[d + 3] * decode<FMT>(w >> 24);
+}
+
+// v = hi + lo / 2048 as a pair of fp16 (hi in the low half)
+__device__ __forceinline__ unsigned split_half(float v) {
+    const __half h = __float2half_rn(v);
+    const __half2 p = __halves2half2(h, __float2half_rn((v - __half2float(h)) * kLoScale));
+    return *reinterpret_cast<const unsigned *>(&p);
+}
+
+template <int WPR>
+__device__ __forceinline__ void group_sync(int group) {
+    if (WPR == 1)
+        __syncwarp();
+    else
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * WPR) : "memory");
+}
+
+// Units of sequence s (0 where it has no rows or is out of range).
+struct SeqWork {
+    int first, n, len, units, col_groups;
+    long long total;
+};
+template <int COLS>
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
+    SeqWork w{};
+    const Span sp = seq_rows(a.r, s);
+    w.first = sp.first;
+    w.n = sp.n;
+    if (!sp.n) return w;
+    w.len = a.seq_len[s];
+    if (w.len < 0 || w.len > (long long)a.r.table_stride * a.c.page_size) {
+        bad(a.r);
+        w.n = 0;
+        return w;
+    }
+    w.units = max(1, (w.len + a.unit - 1) / a.unit);   // a row that sees nothing is still written
+    w.col_groups = (w.n * a.group + COLS - 1) / COLS;
+    w.total = (long long)w.units * w.col_groups * a.c.n_kv_head;
+    return w;
+}
+
+template <int FMT, int D, int NT, int WPR>
+__global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnArgs a) {
+    constexpr int COLS = 4 * NT, KS = D / 16, S = AttnRing<D>::kStages, TILE = AttnRing<D>::kTileBytes, GROUPS = kAttnWarps / WPR;
+    constexpr int PART = COLS * (D + 2);
+    static_assert(WPR * PART * 4 <= WPR * S * TILE, "the merge buffer lies in the ring");
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ long long prefix[kAttnWarps * 32 + 1];
+    __shared__ long long warp_sum[kAttnWarps];
+    __shared__ int arrived[GROUPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int grp = warp / WPR, wr = warp % WPR, gt = tid - grp * 32 * WPR;
+    const int H = a.c.n_kv_head, P = a.c.page_size, n_seq = a.r.n_seq;
+
+    // ---- the units before every `per` sequences
+    const int per = (n_seq + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+    long long mine = 0;
+    for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) mine += seq_work<COLS>(a, s).total;
+    long long sum = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    long long before = 0;
+    for (int i = 0; i < warp; ++i) before += warp_sum[i];
+    prefix[tid] = before + sum - mine;
+    if (tid == kAttnWarps * 32 - 1) prefix[kAttnWarps * 32] = before + sum;
+    __syncthreads();
+    const long long total = prefix[kAttnWarps * 32];
+    const long long W = min((long long)a.workers, total);
+    const int worker = blockIdx.x * GROUPS + grp;
+    if (worker >= W) return;   // whole groups leave; later barriers are the groups' own
+    long long u = worker * total / W;
+    const long long u_end = (worker + 1) * total / W;
+    auto worker_of = [&](long long unit) { return (int)(((unit + 1) * W - 1) / total); };
+
+    // ---- the share's first sequence
+    int lo = 0, hi = kAttnWarps * 32 - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (prefix[mid] <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    int s = lo * per;
+    long long seq_begin = prefix[lo];
+    SeqWork sw = seq_work<COLS>(a, s);
+    bool first_piece = true;
+
+    unsigned char *slots = ring + warp * S * TILE;
+    float *meta = reinterpret_cast<float *>(ring + kAttnWarps * S * TILE) + warp * S * 4;   // K scale, V scale, valid
+    float *merge = reinterpret_cast<float *>(ring + grp * WPR * S * TILE);                  // [WPR][PART]
+    const unsigned slots_addr = smem_addr(slots), meta_addr = smem_addr(meta);
+
+    // this lane's places in a slot: where it copies to and reads from
+    const int crow = lane / (D / 16), ccol = lane % (D / 16);
+    const int pv = (crow & 8) | ((crow & 1) << 2) | ((crow >> 1) & 3);   // D = 64: even rows first
+    const unsigned k_put = D == 64 ? lane * 16 : crow * 128 + (ccol ^ ((crow & 1) << 2)) * 16;
+    const unsigned v_put = 16 * D + (D == 64 ? pv * 64 + (ccol ^ (((pv >> 1) & 1) << 1)) * 16
+                                             : crow * 128 + (ccol ^ (((crow >> 1) & 3) << 1)) * 16);
+
+    while (u < u_end) {
+        while (u >= seq_begin + sw.total) {   // only past sequences without units or the end of one
+            seq_begin += sw.total;
+            sw = seq_work<COLS>(a, ++s);
+        }
+        const long long rem = u - seq_begin;
+        const int run = (int)(rem / sw.units), unit0 = (int)(rem % sw.units);
+        const int h = run / sw.col_groups, col0 = run % sw.col_groups * COLS;
+        const int n_units = (int)min((long long)(sw.units - unit0), u_end - u);
+        const long long run_begin = u - unit0;
+        const int cols = min(COLS, sw.n * a.group - col0);
+        // key limits of the columns; `lim` of this thread's (column t of each n tile)
+        const int lim_first = sw.len - sw.n + col0 / a.group + 1, lim_last = sw.len - sw.n + (col0 + cols - 1) / a.group + 1;
+        int lim[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int col = col0 + n * 4 + t;
+            lim[n] = n * 4 + t < cols ? sw.len - sw.n + col / a.group + 1 : 0;
+        }
+        const int kbeg = unit0 * a.unit;
+        const int kend = (int)min((long long)min(sw.len, lim_last), (long long)(unit0 + n_units) * a.unit);
+        const int n_tiles = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
+        const int my_tiles = n_tiles > wr ? (n_tiles - wr + WPR - 1) / WPR : 0;
+        const int *table = a.r.table + (long long)s * a.r.table_stride;
+
+        // pages of this warp's tiles, 32 at a time, a window ahead of the copies
+        auto load_pages = [&](int base) -> int {
+            const int j = base + lane;
+            if (j >= my_tiles) return -1;
+            const int page = table[(kbeg + (j * WPR + wr) * 16) / P];
+            if (page >= 0 && page < a.c.n_pages) return page;
+            bad(a.r);
+            return -1;
+        };
+        int pages = load_pages(0), pages_next = load_pages(32);
+        auto issue = [&](int j) {
+            if (j < my_tiles) {
+                if (j && (j & 31) == 0) {
+                    pages = pages_next;
+                    pages_next = load_pages(j + 32);
                 }
-                sc = dot * c.k_scale[at];
+                const int key0 = kbeg + (j * WPR + wr) * 16;
+                const int page = __shfl_sync(0xffffffffu, pages, j & 31);
+                const long long at = (long long)max(page, 0) * H + h;
+                const long long off = (at * P + key0 % P) * D + lane * 16;
+                const unsigned char *ks = static_cast<const unsigned char *>(a.c.k) + off;
+                const unsigned char *vs = static_cast<const unsigned char *>(a.c.v) + off;
+                const unsigned slot = slots_addr + (j % S) * TILE;
+                const int rows = page >= 0 ? sw.len - key0 : 0;   // rows from here on are not the sequence's
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const int bytes = crow + i * (512 / D) < rows ? 16 : 0;
+                    cp_async16(slot + k_put + i * 512, ks + i * 512, bytes);
+                    cp_async16(slot + (D == 64 ? v_put : v_put ^ ((i & 1) << 6)) + i * 512, vs + i * 512, bytes);
+                }
+                const unsigned m = meta_addr + (j % S) * 16;
+                if (lane == 0) cp_async4(m, a.c.k_scale + at, 4);
+                if (lane == 1) cp_async4(m + 4, a.c.v_scale + at, 4);
+                if (lane == 2) meta[(j % S) * 4 + 2] = page >= 0 ? 1.0f : 0.0f;
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int j = 0; j < S - 1; ++j) issue(j);
+
+        // ---- queries: column n of an n tile is part n & 1 of query n >> 1
+        unsigned qf[NT][KS][2];
+        float qfac[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = n * 4 + (g >> 1);
+            float x[D / 4];
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            if (c < cols) {
+                const int col = col0 + c;
+                const long long o = (long long)(sw.first + col / a.group) * a.q_stride +
+                                    (long long)(h * a.group + col % a.group) * D + t * 16;
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 v = a.f16 ? load4<__half>(static_cast<const __half *>(a.q) + o + b * 64 + i * 4)
+                                               : load4<float>(static_cast<const float *>(a.q) + o + b * 64 + i * 4);
+                        x[b * 16 + i * 4] = v.x;
+                        x[b * 16 + i * 4 + 1] = v.y;
+                        x[b * 16 + i * 4 + 2] = v.z;
+                        x[b * 16 + i * 4 + 3] = v.w;
+                    }
+            }
+            unsigned peak = 0;
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) peak = max(peak, abs_bits(x[i]));
+            peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+            peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+            // a power of two that brings the largest below 2, so that fp16's range does not matter
+            const int e = max(-126, min(126, (int)(peak >> 23) - 127));
+            const float down = __uint_as_float((unsigned)(127 - e) << 23), up = __uint_as_float((unsigned)(127 + e) << 23);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const unsigned p0 = split_half(x[k * 4 + b * 2] * down), p1 = split_half(x[k * 4 + b * 2 + 1] * down);
+                    qf[n][k][b] = __byte_perm(p0, p1, (g & 1) ? 0x7632 : 0x5410);
+                }
+            qfac[n] = __shfl_sync(0xffffffffu, up, t * 8) * a.scale_log2e;   // of query t
+        }
+
+        float acc[NT][KS][4], mref[NT], l[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            mref[n] = kNoMax;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[n][i][x] = 0.0f;
+        }
+
+        for (int j = 0; j < my_tiles; ++j) {
+            cp_wait<S - 2>();
+            __syncwarp();
+            issue(j + S - 1);
+            const unsigned char *slot = slots + (j % S) * TILE;
+            const float *mt = meta + (j % S) * 4;
+            // ---- scores
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b) {
+                const int c = D == 64 ? t : (b * 4 + t) ^ ((g & 1) << 2);
+                const uint4 r0 = *reinterpret_cast<const uint4 *>(slot + g * D + c * 16);
+                const uint4 r1 = *reinterpret_cast<const uint4 *>(slot + (g + 8) * D + c * 16);
+                const unsigned w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned f[4];
+                    codes_to_half<FMT>(w0[i], f[0], f[2]);
+                    codes_to_half<FMT>(w1[i], f[1], f[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(sc[n], f, qf[n][b * 4 + i][0], qf[n][b * 4 + i][1]);
+                }
+            }
+            // ---- weights
+            const int key0 = kbeg + (j * WPR + wr) * 16;
+            const float ks = mt[0], vs = fmaxf(mt[1], kScaleFloor) + (mt[1] - mt[1]);   // NaN stays NaN
+            const bool there = mt[2] != 0.0f;
+            const float lvs = there ? log2_fast(vs) : -INFINITY, rvs = there ? __frcp_rn(vs) : 0.0f;
+            const bool all = key0 + 16 <= lim_first;
+            float w[NT][2];
+            bool raise = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float f = there ? ks * qfac[n] : 0.0f;
+                w[n][0] = fmaf(fmaf(sc[n][1], kLoUnscale, sc[n][0]), f, lvs);
+                w[n][1] = fmaf(fmaf(sc[n][3], kLoUnscale, sc[n][2]), f, lvs);
+                if (!all) {
+                    if (key0 + g >= lim[n]) w[n][0] = -INFINITY;
+                    if (key0 + g + 8 >= lim[n]) w[n][1] = -INFINITY;
+                }
+                raise |= fmaxf(w[n][0], w[n][1]) > mref[n] + 8.0f;
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float m = fmaxf(fmaxf(w[n][0], w[n][1]), mref[n]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    const float fix = exp2_fast(mref[n] - m);
+                    mref[n] = m;
+                    l[n] *= fix;
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[n][i][x] *= fix;
+                }
+            }
+            unsigned pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float p0 = exp2_fast(w[n][0] - mref[n]), p1 = exp2_fast(w[n][1] - mref[n]);
+                if (p0 + p1 != 0.0f) l[n] = fmaf(p0 + p1, rvs, l[n]);   // a NaN scale reaches only columns that see it
+                pb[n][0] = transpose8x8(split_half(p0));
+                pb[n][1] = transpose8x8(split_half(p1));
+            }
+            // ---- outputs: keys 2t, 2t + 1, 2t + 8, 2t + 9 of this thread's D / 8 dimensions
+            const unsigned char *vslot = slot + 16 * D;
+            unsigned v[4][D / 32];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int row = 2 * t + (x & 1) + (x >> 1) * 8;
+                if (D == 64) {
+                    const int pr = (row & 8) | ((row & 1) << 2) | ((row >> 1) & 3);
+                    const uint2 r = *reinterpret_cast<const uint2 *>(vslot + pr * 64 + ((g >> 1) ^ (((pr >> 1) & 1) << 1)) * 16 + (g & 1) * 8);
+                    v[x][0] = r.x;
+                    v[x][1] = r.y;
+                } else {
+                    const uint4 r = *reinterpret_cast<const uint4 *>(vslot + row * 128 + (g ^ (((row >> 1) & 3) << 1)) * 16);
+                    const unsigned all4[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                    for (int y = 0; y < D / 32; ++y) v[x][y] = all4[y];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {   // dimensions 2i and 2i + 1 of the thread's
+                const unsigned sel = (i & 1) ? 0x7362 : 0x5140;
+                unsigned f[4];
+                codes_to_half<FMT>(__byte_perm(v[0][i / 2], v[1][i / 2], sel), f[0], f[1]);
+                codes_to_half<FMT>(__byte_perm(v[2][i / 2], v[3][i / 2], sel), f[2], f[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816(acc[n][i], f, pb[n][0], pb[n][1]);
             }
         }
-        float mx = sc;
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (lane == 0) red[warp] = mx;
-        __syncthreads();
-        mx = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        const float p = expf(sc - base), fix = expf(m - base);
-        ps[t] = p;
-        __syncthreads();
-        float sum = 0.0f;
-        acc *= fix;
-        const int n = min(kAttnThreads, keys - k0);
-        for (int i = 0; i < n; ++i) {
-            sum += ps[i];
-            if (t < D && pages[i] >= 0) {
-                const long long at = (long long)pages[i] * c.n_kv_head + kh;
-                acc += ps[i] * decode<FMT>(static_cast<const unsigned char *>(c.v)[(at * P + (k0 + i) % P) * D + t]) * c.v_scale[at];
+        cp_wait<0>();
+
+        // ---- the warps' results of this piece, into the ring's memory
+        group_sync<WPR>(grp);
+        float *mw = merge + wr * PART;   // [COLS][D] sums, [COLS] references, [COLS] weights
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+            const int c = n * 4 + t;
+            if (g == 0) {
+                mw[COLS * D + c] = mref[n];
+                mw[COLS * (D + 1) + c] = l[n];
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                float2 o;
+                o.x = fmaf(acc[n][i][1], kLoUnscale, acc[n][i][0]);
+                o.y = fmaf(acc[n][i][3], kLoUnscale, acc[n][i][2]);
+                *reinterpret_cast<float2 *>(mw + c * D + g * (D / 8) + 2 * i) = o;
             }
         }
-        l = l * fix + sum;
-        m = mx;
+        group_sync<WPR>(grp);
+
+        const bool whole = n_units == sw.units;
+        const int w0 = worker_of(run_begin), w1 = worker_of(run_begin + sw.units - 1);
+        float *part = a.parts + ((long long)worker * 2 + (first_piece ? 0 : 1)) * PART;
+        auto store = [&](int c, int d, float v) {
+            const int col = col0 + c;
+            const long long o = (long long)(sw.first + col / a.group) * a.out_stride +
+                                (long long)(h * a.group + col % a.group) * D + d;
+            if (a.f16) static_cast<__half *>(a.out)[o] = __float2half_rn(v);
+            else static_cast<float *>(a.out)[o] = v;
+        };
+        for (int i = gt; i < cols * D; i += 32 * WPR) {
+            const int c = i / D, d = i % D;
+            float m = kNoMax, sum_w = 0.0f, sum_o = 0.0f;
+#pragma unroll
+            for (int x = 0; x < WPR; ++x) m = fmaxf(m, merge[x * PART + COLS * D + c]);
+#pragma unroll
+            for (int x = 0; x < WPR; ++x) {
+                const float fix = exp2_fast(merge[x * PART + COLS * D + c] - m);
+                sum_w = fmaf(merge[x * PART + COLS * (D + 1) + c], fix, sum_w);
+                sum_o = fmaf(merge[x * PART + c * D + d], fix, sum_o);
+            }
+            if (whole) {
+                store(c, d, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
+            } else {
+                part[i] = sum_o;
+                if (d == 0) {
+                    part[COLS * D + c] = m;
+                    part[COLS * (D + 1) + c] = sum_w;
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            group_sync<WPR>(grp);
+            if (gt == 0) arrived[grp] = (int)atomicAdd(&a.counters[w0], 1u);
+            group_sync<WPR>(grp);
+            if (arrived[grp] == w1 - w0) {   // every other piece is there
+                __threadfence();
+                if (gt == 0) a.counters[w0] = 0;
+                // piece of worker x: its first one, or, where the run begins inside the share, its last
+                auto piece = [&](int x) {
+                    const bool later = x == w0 && run_begin > x * total / W;
+                    return a.parts + ((long long)x * 2 + (later ? 1 : 0)) * PART;
+                };
+                for (int i = gt; i < cols * D; i += 32 * WPR) {
+                    const int c = i / D, d = i % D;
+                    float m = kNoMax, sum_w = 0.0f, sum_o = 0.0f;
+                    for (int x = w0; x <= w1; ++x) {
+                        const float *p = piece(x);
+                        const float pm = __ldcg(p + COLS * D + c), nm = fmaxf(m, pm);
+                        const float f0 = exp2_fast(m - nm), f1 = exp2_fast(pm - nm);
+                        sum_w = sum_w * f0 + __ldcg(p + COLS * (D + 1) + c) * f1;
+                        sum_o = sum_o * f0 + __ldcg(p + i) * f1;
+                        m = nm;
+                    }
+                    store(c, d, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
+                }
+            }
+        }
+        group_sync<WPR>(grp);   // the merge buffer is the next piece's ring
+        first_piece = false;
+        u += n_units;
     }
-    if (t < D) out[row * out_stride + (long long)h * D + t] = fromf<T>(l > 0.0f || l != l ? acc / l : 0.0f);
+}
+
+// Query columns a warp works on together, and how the work is cut.
+struct AttnPlan {
+    int nt, wpr, unit, workers;
+    size_t part_floats;
+};
+AttnPlan attn_plan(const g2_kv8 &c, int n_head, int n_seq, int max_q, int sms) {
+    AttnPlan p;
+    const long long cols = (long long)max_q * (n_head / c.n_kv_head);
+    p.nt = cols <= 4 ? 1 : cols <= 8 || c.head_dim == 128 ? 2 : 4;
+    const long long runs = (long long)n_seq * c.n_kv_head * ((cols + 4 * p.nt - 1) / (4 * p.nt));
+    p.wpr = runs >= 2LL * sms * kAttnWarps ? 1 : 8;
+    p.unit = p.wpr == 1 ? 64 : 128;
+    p.workers = sms * 2 * (kAttnWarps / p.wpr);
+    if (p.workers > kMaxWorkers) p.workers = kMaxWorkers;
+    p.part_floats = (size_t)p.workers * 2 * 4 * p.nt * (c.head_dim + 2);
+    return p;
+}
+
+int attn_sms() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    return n > 0 ? n : 148;
+}
+
+template <int FMT, int D, int NT, int WPR>
+int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
+    auto kernel = kv8_attention_kernel<FMT, D, NT, WPR>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnRing<D>::kSmem) != cudaSuccess)
+        return arg_error(G2_ERR_CUDA, "g2k_kv8_attention", cudaGetErrorString(cudaGetLastError()));
+    const int per_cta = kAttnWarps / WPR;
+    kernel<<<(a.workers + per_cta - 1) / per_cta, kAttnWarps * 32, AttnRing<D>::kSmem, st>>>(a);
+    return launch_status("g2k_kv8_attention");
+}
+
+template <int FMT, int D, int NT>
+int launch_attn(const AttnArgs &a, int wpr, int sms, cudaStream_t st) {
+    return wpr == 1 ? launch_attn<FMT, D, NT, 1>(a, sms, st) : launch_attn<FMT, D, NT, 8>(a, sms, st);
+}
+
+template <int FMT>
+int launch_attn(const AttnArgs &a, const AttnPlan &p, int sms, cudaStream_t st) {
+    if (a.c.head_dim == 64)
+        return p.nt == 1 ? launch_attn<FMT, 64, 1>(a, p.wpr, sms, st)
+             : p.nt == 2 ? launch_attn<FMT, 64, 2>(a, p.wpr, sms, st) : launch_attn<FMT, 64, 4>(a, p.wpr, sms, st);
+    return p.nt == 1 ? launch_attn<FMT, 128, 1>(a, p.wpr, sms, st) : launch_attn<FMT, 128, 2>(a, p.wpr, sms, st);
 }
 
 // ---- argument checks ----------------------------------------------------------------
@@ -343,13 +835,6 @@ void launch_gather(const g2_kv8 &c, void *k, void *v, long long stride, const in
         c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
 }
 
-template <typename T, int FMT>
-void launch_attention8(const g2_kv8 &c, const void *q, long long q_stride, void *out, long long out_stride, int n_head,
-                       float scale, const int *seq_len, const Rows8 &r, cudaStream_t st) {
-    kv8_attention_kernel<T, FMT><<<dim3((unsigned)r.max_q * r.n_seq, n_head), kAttnThreads, 0, st>>>(
-        c, static_cast<const T *>(q), q_stride, static_cast<T *>(out), out_stride, n_head / c.n_kv_head, scale, seq_len, r);
-}
-
 // dtype and format to template arguments
 #define G2_KV8_DISPATCH(fn, ...)                                     \
     do {                                                             \
@@ -401,9 +886,10 @@ extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int
     return launch_status(who);
 }
 
+// [counters | partial results], each 256-byte aligned; the counters' place does not depend on the call's sizes
 extern "C" size_t g2k_kv8_attention_workspace(const g2_kv8 *cache, int n_head, int n_seq, int max_q) {
-    if (!cache || n_head < 1 || n_seq < 0 || max_q < 1) return 0;
-    return 256;
+    if (!cache || n_head < 1 || n_seq < 0 || max_q < 1 || cache->n_kv_head < 1 || n_head % cache->n_kv_head) return 0;
+    return kMaxWorkers * 4 + attn_plan(*cache, n_head, n_seq, max_q, attn_sms()).part_floats * 4;
 }
 
 extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q_stride, void *out, long long out_stride,
@@ -426,6 +912,11 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, q, out, q_start, seq_len, table,
                                       workspace, status})))
         return rc;
-    G2_KV8_DISPATCH(launch_attention8, *cache, q, q_stride, out, out_stride, n_head, scale, seq_len, r, (cudaStream_t)stream);
-    return launch_status(who);
+    const int sms = attn_sms();
+    const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, sms);
+    const AttnArgs a{*cache, q, out, q_stride, out_stride, dtype == G2_F16, n_head / cache->n_kv_head,
+                     scale * 1.4426950408889634f, seq_len, r, p.unit, p.workers, static_cast<unsigned *>(workspace),
+                     static_cast<float *>(workspace) + kMaxWorkers};
+    return cache->format == G2_KV_I8 ? launch_attn<G2_KV_I8>(a, p, sms, (cudaStream_t)stream)
+                                     : launch_attn<G2_KV_E4M3>(a, p, sms, (cudaStream_t)stream);
 }
