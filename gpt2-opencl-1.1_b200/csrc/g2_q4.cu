@@ -9,13 +9,16 @@
 //   codes  [tile][chunk][lane 0..31][4 words]   512 bytes a chunk
 //   scales [tile][group][8][2] bf16             features g and g + 8 of a tile together
 // Word s of lane (g = lane / 4, t = lane % 4) holds features g and g + 8 at rows
-// 64 chunk + 16 s + 4 t + {0, 1, 2, 3}, as code + 8 in nibbles
+// 64 chunk + 32 (s / 2) + 8 t + 4 (s % 2) + {0, 1, 2, 3}, as code + 8 in nibbles
 //   0, 4: feature g,     rows +0, +1      1, 5: feature g + 8, rows +0, +1
 //   2, 6: feature g,     rows +2, +3      3, 7: feature g + 8, rows +2, +3
 // so that nibbles j and j + 4 are register j of the A operand of a 16 x 8 x 16
-// tensor-core product whose k index is a permutation of the rows.  Rows past K
-// and columns past N hold code 0.
+// tensor-core product whose k index is a permutation of the rows, and the x of
+// a lane's words s and s + 1 are eight consecutive ones.  Rows past K and columns
+// past N hold code 0.
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "g2_args.h"
 #include "g2_device.cuh"
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
         const int lane = i & 31, step16 = i >> 5, kk = k0 + step16 * 16;
         const int chunk = kk / kChunk, s = (kk % kChunk) / 16;
         if (chunk >= sh.chunks) continue;
-        const int g = lane >> 2, r = step16 * 16 + (lane & 3) * 4;
+        const int g = lane >> 2, r = chunk * kChunk + 32 * (s >> 1) + 8 * (lane & 3) + 4 * (s & 1) - k0;
         unsigned w = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -117,8 +120,8 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
 
 __device__ __forceinline__ int q4_code(const unsigned *codes, const Q4Shape &sh, int k, int n) {
     const int f = n % kTile, kc = k % kChunk, r = kc & 3;
-    const int lane = (f & 7) * 4 + ((kc >> 2) & 3);
-    const unsigned w = codes[(((size_t)(n / kTile) * sh.chunks + k / kChunk) * 32 + lane) * 4 + kc / 16];
+    const int lane = (f & 7) * 4 + ((kc >> 3) & 3), s = (kc >> 5) * 2 + ((kc >> 2) & 1);
+    const unsigned w = codes[(((size_t)(n / kTile) * sh.chunks + k / kChunk) * 32 + lane) * 4 + s];
     const int nib = (f >> 3) + (r >> 1) * 2 + (r & 1) * 4;
     return (int)((w >> (4 * nib)) & 15u) - 8;
 }
@@ -136,68 +139,317 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned *codes, c
     W[i] = q4_code(codes, sh, k, n) * q4_scale(scales, sh, k, n);
 }
 
-// The product, one warp per feature: each lane takes every 32nd row.
+// ---- the product ----------------------------------------------------------------
+// One CTA of 16 warps per SM takes an equal share of the tiles.  Its x is staged
+// in shared memory once, as columns of fp16 operands of m16n8k16 products
+// (features on m, rows of x on n): an fp16 x as it is, an fp32 one (or a
+// LayerNorm's result) as two columns, the fp16 rounding and 2^11 times the rest,
+// after a power of two has brought the row's largest below 2 (22 bits in all; the
+// columns of a few rows would be idle otherwise).
+//
+// The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
+// that each warp streams one contiguous piece of the codes, kDepth 512-byte loads
+// ahead, whatever the shape: the weights are read once, and nothing else is
+// large.  Codes become fp16 exactly (0x6400 | code is 1024 + code); a group's
+// sum is taken in fp32 and scaled once.  A tile that crosses warps is summed in
+// warp order, so the bits do not depend on timing.
+constexpr int kQ4Warps = 16, kQ4Threads = 32 * kQ4Warps;
+constexpr int kMaxTiles = 32;              // tiles of a CTA summed at a time
+constexpr int kXBytes = 128 * 1024;        // x staged at a time; longer rows go in slices
+constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
+
 struct Q4Args {
     const void *x;
-    const unsigned *codes;
-    const __nv_bfloat16 *scales;
+    const uint4 *codes;
+    const unsigned *scales;                // pairs of bf16
     const float *bias, *gamma, *beta;
     const void *residual;
     void *y;
-    int M, gelu;
+    int M, gelu, f16;
+    int slice;                             // chunks of x staged at a time
+    int most;                              // tiles (of TP feature tiles) summed at a time
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
-    __shared__ float mean_s[G2_Q4_MAX_ROWS], rstd_s[G2_Q4_MAX_ROWS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = sh.K;
-    const T *x = static_cast<const T *>(a.x);
-    if (a.gamma) {
-        for (int m = warp; m < a.M; m += 8) {
-            float s = 0.0f;
-            for (int k = lane; k < K; k += 32) s += tof(x[(size_t)m * K + k]);
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            const float mu = s / K;
-            float v = 0.0f;
-            for (int k = lane; k < K; k += 32) {
-                const float d = tof(x[(size_t)m * K + k]) - mu;
-                v += d * d;
-            }
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) {
-                mean_s[m] = mu;
-                rstd_s[m] = rsqrtf(v / K + 1e-5f);
-            }
-        }
-        __syncthreads();
+__device__ __forceinline__ float load_x(const Q4Args &a, size_t i) {
+    return a.f16 ? __half2float(static_cast<const __half *>(a.x)[i]) : static_cast<const float *>(a.x)[i];
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
+}
+
+// (w & mask) | 0x64006400: two fp16 of 1024 + (16 times, for the upper nibbles) a code
+__device__ __forceinline__ __half2 nibbles(unsigned w, unsigned mask) {
+    unsigned r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
+    return *reinterpret_cast<__half2 *>(&r);
+}
+__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned *>(&v); }
+__device__ __forceinline__ void codes_to_half(unsigned w, unsigned (&f)[4]) {
+    const __half2 even = __half2half2(__ushort_as_half((unsigned short)0x6408));   // 1032
+    const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2c00)), odd = __half2half2(__ushort_as_half((unsigned short)0xd480));   // -72
+    f[0] = bits(__hsub2(nibbles(w, 0x000f000fu), even));
+    f[1] = bits(__hfma2(nibbles(w, 0x00f000f0u), sixteenth, odd));
+    w >>= 8;
+    f[2] = bits(__hsub2(nibbles(w, 0x000f000fu), even));
+    f[3] = bits(__hfma2(nibbles(w, 0x00f000f0u), sixteenth, odd));
+}
+
+// Sum (or largest) over the `n` warps of a row, which begin at warp `w0`: every lane gets it.
+template <bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float *scratch, int w0, int n) {
+    for (int o = 16; o; o >>= 1) {
+        const float x = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MAX ? fmaxf(v, x) : v + x;
     }
-    const int n = blockIdx.x * 8 + warp;
-    if (n >= sh.N) return;
-    float acc[G2_Q4_MAX_ROWS] = {};
-    for (int k = lane; k < K; k += 32) {
-        const float w = q4_code(a.codes, sh, k, n) * q4_scale(a.scales, sh, k, n);
-        const float ga = a.gamma ? a.gamma[k] : 0.0f, be = a.gamma ? a.beta[k] : 0.0f;
+    if (n == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = scratch[w0];
+    for (int i = 1; i < n; ++i) v = MAX ? fmaxf(v, scratch[w0 + i]) : v + scratch[w0 + i];
+    return v;
+}
+
+// NT n tiles of 8 columns, TP feature tiles that share an operand of x, NP columns a row.
+template <int NT, int TP, int NP>
+__global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
+    constexpr int kDepth = TP == 1 ? 8 : 4;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float scratch[kQ4Warps], mean_s[G2_Q4_MAX_ROWS], rstd_s[G2_Q4_MAX_ROWS], up_s[G2_Q4_MAX_ROWS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int M = a.M, K = sh.K;
+    const int stride = a.slice * kChunk + 32;                     // halves of a column; 64 bytes past a multiple of 128
+    __half *xs = reinterpret_cast<__half *>(smem);                // [8 NT][stride]
+    float *pieces = reinterpret_cast<float *>(smem + (size_t)8 * NT * stride * 2);   // [tiles + warps][M][16 TP]
+    float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;               // [M][tiles][16 TP], only with slices
+    const int ntiles = (sh.tiles + TP - 1) / TP;                  // of TP feature tiles
+    const int tile0 = (int)((long long)blockIdx.x * ntiles / gridDim.x), tile1 = (int)((long long)(blockIdx.x + 1) * ntiles / gridDim.x);
+    // warps of a row of x in the passes over it
+    int wpr = kQ4Warps;
+    while (wpr * M > kQ4Warps && wpr > 1) wpr >>= 1;
+    const int rows_at_once = kQ4Warps / wpr, w0 = warp / wpr * wpr;
+    const int first = (warp - w0) * 32 + lane, step = wpr * 32;
+
+    for (int tile = tile0; tile < tile1; tile += a.most) {
+        const int R = min(a.most, tile1 - tile);
+        for (int c0 = 0; c0 < sh.chunks; c0 += a.slice) {
+            const int nc = min(a.slice, sh.chunks - c0);          // chunks of this slice
+            const int U = R * nc, W = min(kQ4Warps, U);
+            const int u0 = warp < W ? warp * U / W : 0, u1 = warp < W ? (warp + 1) * U / W : 0;
+
+            // ---- the first loads of the codes
+            uint4 w[kDepth][TP];
+            unsigned sc[kDepth][TP][2];
+            int lr = nc ? u0 / nc : 0, lc = nc ? u0 % nc : 0, lu = u0;
+            auto load = [&](int p) {
+                if (lu < u1) {
 #pragma unroll
-        for (int m = 0; m < G2_Q4_MAX_ROWS; ++m) {
-            if (m >= a.M) break;
-            float v = tof(x[(size_t)m * K + k]);
-            if (a.gamma) v = (v - mean_s[m]) * rstd_s[m] * ga + be;
-            acc[m] += v * w;
-        }
-    }
+                    for (int x = 0; x < TP; ++x) {
+                        const int ft = min((tile + lr) * TP + x, sh.tiles - 1);   // a last odd tile is read twice
+                        w[p][x] = __ldcs(a.codes + ((size_t)ft * sh.chunks + c0 + lc) * 32 + lane);
+                        const unsigned *s = a.scales + ((size_t)ft * sh.groups + (c0 + lc) * kChunk / sh.group) * 8 + g;
+                        sc[p][x][0] = __ldg(s);
+                        if (sh.group == 32) sc[p][x][1] = __ldg(s + 8);
+                    }
+                    if (++lc == nc) {
+                        lc = 0;
+                        ++lr;
+                    }
+                    ++lu;
+                }
+            };
 #pragma unroll
-    for (int m = 0; m < G2_Q4_MAX_ROWS; ++m) {
-        if (m >= a.M) break;
-        float v = acc[m];
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) {
-            if (a.bias) v += a.bias[n];
-            if (a.gelu) v = gelu_f(v);
-            const size_t i = (size_t)m * sh.N + n;
-            if (a.residual) v += tof(static_cast<const T *>(a.residual)[i]);
-            static_cast<T *>(a.y)[i] = fromf<T>(v);
+            for (int p = 0; p < kDepth; ++p) load(p);
+
+            // ---- x of this slice, once
+            if (sh.chunks > a.slice || tile == tile0) {
+                const int k0 = c0 * kChunk, kn = nc * kChunk;
+                for (int r0 = 0; r0 < M; r0 += rows_at_once) {   // columns past M rows keep what they hold
+                    const int m = r0 + warp / wpr;
+                    const bool live = m < M;
+                    const size_t row = (size_t)(live ? m : 0) * K;
+                    float mu = 0.0f, rstd = 1.0f;
+                    if (a.gamma) {
+                        if (c0 == 0 && tile == tile0) {
+                            float s = 0.0f;
+                            for (int k = first; k < K; k += step) s += load_x(a, row + k);
+                            mu = row_reduce<false>(s, scratch, w0, wpr) / K;
+                            float v = 0.0f;
+                            for (int k = first; k < K; k += step) {
+                                const float d = load_x(a, row + k) - mu;
+                                v = fmaf(d, d, v);
+                            }
+                            rstd = rsqrtf(row_reduce<false>(v, scratch, w0, wpr) / K + 1e-5f);
+                            if (live && first == 0) {
+                                mean_s[m] = mu;
+                                rstd_s[m] = rstd;
+                            }
+                        } else {
+                            mu = mean_s[live ? m : 0];
+                            rstd = rstd_s[live ? m : 0];
+                        }
+                    }
+                    auto value = [&](int k) -> float {
+                        if (k >= K) return 0.0f;
+                        float v = load_x(a, row + k);
+                        if (a.gamma) v = fmaf((v - mu) * rstd, a.gamma[k], a.beta[k]);
+                        return v;
+                    };
+                    if (NP == 1) {
+                        for (int k = live ? first : kn; k < kn; k += step) xs[m * stride + k] = __float2half_rn(value(k0 + k));
+                    } else {
+                        float peak = 0.0f;
+                        for (int k = live ? first : kn; k < kn; k += step) peak = fmaxf(peak, fabsf(value(k0 + k)));
+                        peak = row_reduce<true>(peak, scratch, w0, wpr);
+                        const int e = max(-126, min(126, (int)(__float_as_uint(peak) >> 23) - 127));
+                        const float down = __uint_as_float((unsigned)(127 - e) << 23);
+                        if (live && first == 0) up_s[m] = __uint_as_float((unsigned)(127 + e) << 23);
+                        for (int k = live ? first : kn; k < kn; k += step) {
+                            const float v = value(k0 + k) * down;
+                            const __half h = __float2half_rn(v);
+                            xs[2 * m * stride + k] = h;
+                            xs[(2 * m + 1) * stride + k] = __float2half_rn((v - __half2float(h)) * kLoScale);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+
+            // ---- the warp's units
+            float tot[TP][NT][4];
+#pragma unroll
+            for (int x = 0; x < TP; ++x)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) tot[x][n][0] = tot[x][n][1] = tot[x][n][2] = tot[x][n][3] = 0.0f;
+            int r = nc ? u0 / nc : 0, c = nc ? u0 % nc : 0;
+            auto flush = [&]() {   // a tile's (part of a) sum to its piece
+                float *o = pieces + (size_t)(r + warp) * M * 16 * TP;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < TP; ++x) {
+                        float (&v)[4] = tot[x][n];
+                        if (NP == 2) {
+                            const int m = n * 4 + t;
+                            if (m < M) {
+                                o[m * 16 * TP + x * 16 + g] = fmaf(v[1], kLoUnscale, v[0]);
+                                o[m * 16 * TP + x * 16 + g + 8] = fmaf(v[3], kLoUnscale, v[2]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int m = n * 8 + 2 * t + (i & 1);
+                                if (m < M) o[m * 16 * TP + x * 16 + g + (i >> 1) * 8] = v[i];
+                            }
+                        }
+                        v[0] = v[1] = v[2] = v[3] = 0.0f;
+                    }
+            };
+            for (int u = u0; u < u1; u += kDepth) {
+#pragma unroll
+                for (int p = 0; p < kDepth; ++p) {
+                    if (u + p < u1) {
+                        uint4 b[NT][2];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                b[n][half] = *reinterpret_cast<const uint4 *>(xs + (n * 8 + g) * stride + c * kChunk + half * 32 + t * 8);
+#pragma unroll
+                        for (int x = 0; x < TP; ++x) {
+                            const unsigned words[4] = {w[p][x].x, w[p][x].y, w[p][x].z, w[p][x].w};
+                            float acc[NT][4];
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+                            auto scaled = [&](unsigned s) {
+                                const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    tot[x][n][0] = fmaf(acc[n][0], lo, tot[x][n][0]);
+                                    tot[x][n][1] = fmaf(acc[n][1], lo, tot[x][n][1]);
+                                    tot[x][n][2] = fmaf(acc[n][2], hi, tot[x][n][2]);
+                                    tot[x][n][3] = fmaf(acc[n][3], hi, tot[x][n][3]);
+                                    acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+                                }
+                            };
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                unsigned f[4];
+                                codes_to_half(words[i], f);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const uint4 &v = b[n][i >> 1];
+                                    mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
+                                }
+                                if (i == 1 && sh.group == 32) scaled(sc[p][x][0]);
+                            }
+                            scaled(sh.group == 32 ? sc[p][x][1] : sc[p][x][0]);
+                        }
+                        if (++c == nc || u + p == u1 - 1) flush();
+                        if (c == nc) {
+                            c = 0;
+                            ++r;
+                        }
+                        load(p);
+                    }
+                }
+            }
+            __syncthreads();
+
+            // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
+            for (int o = tid; o < R * M * 16 * TP; o += kQ4Threads) {
+                const int f = o % (16 * TP), rr = o / (16 * TP) % R, m = o / (16 * TP * R);
+                const int wa = ((rr * nc + 1) * W - 1) / U, wb = ((rr * nc + nc) * W - 1) / U;   // the warps of its units
+                float v = 0.0f;
+                for (int x = wa; x <= wb; ++x) v += pieces[((size_t)(rr + x) * M + m) * 16 * TP + f];
+                if (NP == 2) v *= up_s[m];
+                if (c0 > 0) v += total[o];
+                if (c0 + nc < sh.chunks) {
+                    total[o] = v;
+                    continue;
+                }
+                const int n = (tile + rr) * 16 * TP + f;
+                if (n >= sh.N) continue;
+                if (a.bias) v += a.bias[n];
+                if (a.gelu) v = gelu_f(v);
+                const size_t at = (size_t)m * sh.N + n;
+                if (a.f16) {
+                    if (a.residual) v += __half2float(static_cast<const __half *>(a.residual)[at]);
+                    static_cast<__half *>(a.y)[at] = __float2half_rn(v);
+                } else {
+                    if (a.residual) v += static_cast<const float *>(a.residual)[at];
+                    static_cast<float *>(a.y)[at] = v;
+                }
+            }
+            __syncthreads();
         }
     }
+}
+
+int q4_sms() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return n;
+}
+
+template <int NT, int TP, int NP>
+int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
+    auto kernel = q4_matvec_kernel<NT, TP, NP>;
+    const int ntiles = (sh.tiles + TP - 1) / TP, grid = std::min(q4_sms(), ntiles);
+    a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
+    // equal slices of at most kXBytes of staged columns
+    const int fit = (kXBytes / (8 * NT * 2) - 32) / kChunk, slices = (sh.chunks + fit - 1) / fit;
+    a.slice = (sh.chunks + slices - 1) / slices;
+    const size_t smem = (size_t)8 * NT * (a.slice * kChunk + 32) * 2 +
+                        (size_t)(a.most + kQ4Warps + (slices > 1 ? a.most : 0)) * a.M * 16 * TP * 4;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
+    kernel<<<grid, kQ4Threads, smem, st>>>(a, sh);
+    return launch_status("g2k_matvec_q4");
 }
 
 bool bad_shape(int N, int K, int group) {
@@ -273,13 +525,11 @@ extern "C" int g2k_matvec_q4(const void *x, const void *packed, const float *bia
         return arg_error(G2_ERR_ARG, who, "an array is not aligned to its elements");
     if ((rc = check_device_ptrs(who, {x, packed, bias, residual, y, ln_gamma, ln_beta}))) return rc;
     const Q4Shape sh(N, K, group);
-    Q4Args a{x, static_cast<const unsigned *>(packed),
-             reinterpret_cast<const __nv_bfloat16 *>(static_cast<const char *>(packed) + sh.scale_off), bias, ln_gamma,
-             ln_beta, residual, y, M, apply_gelu};
+    const Q4Args a{x, static_cast<const uint4 *>(packed),
+                   reinterpret_cast<const unsigned *>(static_cast<const char *>(packed) + sh.scale_off), bias, ln_gamma,
+                   ln_beta, residual, y, M, apply_gelu, dtype == G2_F16, 0};
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == G2_F32)
-        q4_matvec_kernel<float><<<(N + 7) / 8, 256, 0, st>>>(a, sh);
-    else
-        q4_matvec_kernel<__half><<<(N + 7) / 8, 256, 0, st>>>(a, sh);
-    return launch_status(who);
+    // more rows than one n tile holds: two feature tiles share each operand of x, which halves its reads
+    if (dtype == G2_F16 && !ln_gamma) return M <= 8 ? launch_q4<1, 1, 1>(a, sh, st) : launch_q4<2, 2, 1>(a, sh, st);
+    return M <= 4 ? launch_q4<1, 1, 2>(a, sh, st) : M <= 8 ? launch_q4<2, 2, 2>(a, sh, st) : launch_q4<4, 2, 2>(a, sh, st);
 }
