@@ -5,9 +5,11 @@
 // s = bf16(max|w| / 7) and its codes c = w / s rounded, in -7..7, so that
 //   y[m][n] = sum_groups s[g][n] * sum_{k in g} x'[m][k] c[k][n].
 //
-// Packed layout, for tiles of 16 columns (features) and chunks of 64 rows:
-//   codes  [tile][chunk][lane 0..31][4 words]   512 bytes a chunk
-//   scales [tile][group][8][2] bf16             features g and g + 8 of a tile together
+// Packed layout, for tiles of 16 columns (features) and chunks of 64 rows, in the
+// order in which the product reads them:
+//   [tile][chunk] { codes [lane 0..31][4 words], scales [1, or 2 for groups of 32][8][2] bf16 }
+// A scale pair is that of features g and g + 8; a group of 128 rows has its scale
+// in both of its chunks (3% more bytes, and a chunk needs nothing but itself).
 // Word s of lane (g = lane / 4, t = lane % 4) holds features g and g + 8 at rows
 // 64 chunk + 32 (s / 2) + 8 t + 4 (s % 2) + {0, 1, 2, 3}, as code + 8 in nibbles
 //   0, 4: feature g,     rows +0, +1      1, 5: feature g + 8, rows +0, +1
@@ -31,15 +33,17 @@ constexpr int kTile = 16, kChunk = 64;
 
 struct Q4Shape {
     int N, K, group;
-    int tiles, chunks, groups;   // groups cover the chunks (zero scales past K)
-    long long scale_off;         // bytes from the codes to the scales
+    int tiles, chunks;
+    int per_chunk;       // scale groups of a chunk
+    int chunk_bytes;
     __host__ __device__ Q4Shape(int N_, int K_, int group_) : N(N_), K(K_), group(group_) {
         tiles = (N + kTile - 1) / kTile;
         chunks = (K + kChunk - 1) / kChunk;
-        groups = (chunks * kChunk + group - 1) / group;
-        scale_off = ((long long)tiles * chunks * 512 + 255) / 256 * 256;
+        per_chunk = group == 32 ? 2 : 1;
+        chunk_bytes = 512 + 32 * per_chunk;
     }
-    size_t bytes() const { return (size_t)scale_off + (size_t)tiles * groups * kTile * 2; }
+    size_t bytes() const { return (size_t)tiles * chunks * chunk_bytes; }
+    __device__ size_t at(int tile, int chunk) const { return ((size_t)tile * chunks + chunk) * chunk_bytes; }
 };
 
 // w / s rounded to the nearest integer, ties to even, from the exact quotient:
@@ -56,8 +60,8 @@ __device__ __forceinline__ int round_quotient(float w, float s) {
 constexpr int kPackThreads = 128;
 
 template <typename T>
-__global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int transposed, unsigned *codes,
-                                                               __nv_bfloat16 *scales, Q4Shape sh) {
+__global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int transposed, unsigned char *packed,
+                                                               Q4Shape sh) {
     __shared__ unsigned peak[kTile];
     __shared__ float step[kTile];
     __shared__ unsigned char code[128][kTile];
@@ -88,8 +92,11 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
     if (t < kTile) {
         const __nv_bfloat16 s = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(peak[t]), 7.0f));
         step[t] = __bfloat162float(s);
-        const size_t o = ((size_t)tile * sh.groups + grp) * kTile + (t & 7) * 2 + (t >> 3);
-        scales[o] = peak[t] >= 0x7f800000u ? __ushort_as_bfloat16(0x7fc0) : s;
+        const __nv_bfloat16 v = peak[t] >= 0x7f800000u ? __ushort_as_bfloat16(0x7fc0) : s;
+        for (int c = k0 / kChunk; c * kChunk < k0 + sh.group && c < sh.chunks; ++c) {
+            auto *o = reinterpret_cast<__nv_bfloat16 *>(packed + sh.at(tile, c) + 512 + (k0 % kChunk) / 32 * 32);
+            o[(t & 7) * 2 + (t >> 3)] = v;
+        }
     }
     __syncthreads();
     for (int i = t; i < sh.group * kTile; i += kPackThreads) {
@@ -114,29 +121,21 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
             w |= (unsigned)code[k][f] << (4 * j);
             w |= (unsigned)code[k + 1][f] << (4 * j + 16);
         }
-        codes[(((size_t)tile * sh.chunks + chunk) * 32 + lane) * 4 + s] = w;
+        reinterpret_cast<unsigned *>(packed + sh.at(tile, chunk))[lane * 4 + s] = w;
     }
 }
 
-__device__ __forceinline__ int q4_code(const unsigned *codes, const Q4Shape &sh, int k, int n) {
-    const int f = n % kTile, kc = k % kChunk, r = kc & 3;
-    const int lane = (f & 7) * 4 + ((kc >> 3) & 3), s = (kc >> 5) * 2 + ((kc >> 2) & 1);
-    const unsigned w = codes[(((size_t)(n / kTile) * sh.chunks + k / kChunk) * 32 + lane) * 4 + s];
-    const int nib = (f >> 3) + (r >> 1) * 2 + (r & 1) * 4;
-    return (int)((w >> (4 * nib)) & 15u) - 8;
-}
-
-__device__ __forceinline__ float q4_scale(const __nv_bfloat16 *scales, const Q4Shape &sh, int k, int n) {
-    const int f = n % kTile;
-    return __bfloat162float(scales[((size_t)(n / kTile) * sh.groups + k / sh.group) * kTile + (f & 7) * 2 + (f >> 3)]);
-}
-
-__global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned *codes, const __nv_bfloat16 *scales, float *W,
-                                                        Q4Shape sh) {
+__global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *packed, float *W, Q4Shape sh) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long long)sh.K * sh.N) return;
     const int k = (int)(i / sh.N), n = (int)(i % sh.N);
-    W[i] = q4_code(codes, sh, k, n) * q4_scale(scales, sh, k, n);
+    const int f = n % kTile, kc = k % kChunk, r = kc & 3;
+    const int lane = (f & 7) * 4 + ((kc >> 3) & 3), s = (kc >> 5) * 2 + ((kc >> 2) & 1);
+    const unsigned char *chunk = packed + sh.at(n / kTile, k / kChunk);
+    const unsigned w = reinterpret_cast<const unsigned *>(chunk)[lane * 4 + s];
+    const int nib = (f >> 3) + (r >> 1) * 2 + (r & 1) * 4;
+    const auto *scale = reinterpret_cast<const __nv_bfloat16 *>(chunk + 512 + (sh.per_chunk == 2 ? kc / 32 * 32 : 0));
+    W[i] = (float)((int)((w >> (4 * nib)) & 15u) - 8) * __bfloat162float(scale[(f & 7) * 2 + (f >> 3)]);
 }
 
 // ---- the product ----------------------------------------------------------------
@@ -148,30 +147,71 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned *codes, c
 // columns of a few rows would be idle otherwise).
 //
 // The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
-// that each warp streams one contiguous piece of the codes, kDepth 512-byte loads
-// ahead, whatever the shape: the weights are read once, and nothing else is
-// large.  Codes become fp16 exactly (0x6400 | code is 1024 + code); a group's
-// sum is taken in fp32 and scaled once.  A tile that crosses warps is summed in
-// warp order, so the bits do not depend on timing.
+// that each warp streams one contiguous piece of the packed matrix whatever the
+// shape, through a ring of its own in shared memory (cp.async; registers as the
+// ring left at most a few loads in flight).  The weights are read once, and
+// nothing else is large.  Codes become fp16 exactly (0x6400 | code is 1024 +
+// code); a group's sum is taken in fp32 and scaled once.  A tile that crosses
+// warps is summed in warp order, so the bits do not depend on timing.
 constexpr int kQ4Warps = 16, kQ4Threads = 32 * kQ4Warps;
 constexpr int kMaxTiles = 32;              // tiles of a CTA summed at a time
-constexpr int kXBytes = 128 * 1024;        // x staged at a time; longer rows go in slices
+constexpr int kQ4Smem = 220 * 1024;
 constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
+
+// One stage: a chunk of each of TP feature tiles.
+template <int TP>
+struct Q4Ring {
+    static constexpr int kStages = TP == 1 ? 8 : 5;
+};
 
 struct Q4Args {
     const void *x;
-    const uint4 *codes;
-    const unsigned *scales;                // pairs of bf16
+    const unsigned char *packed;
     const float *bias, *gamma, *beta;
     const void *residual;
     void *y;
     int M, gelu, f16;
+    int vec;                               // rows of x, gamma and beta can be read four elements at a time
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
 };
 
-__device__ __forceinline__ float load_x(const Q4Args &a, size_t i) {
-    return a.f16 ? __half2float(static_cast<const __half *>(a.x)[i]) : static_cast<const float *>(a.x)[i];
+// x[m][k .. k + 3] (0 past K) and the same of gamma or beta
+__device__ __forceinline__ float4 load_x4(const Q4Args &a, size_t row, int k, int K) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.vec) {
+        if (k < K) {
+            if (a.f16) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.x) + row + k);
+                const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
+                const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+                v = make_float4(p.x, p.y, q.x, q.y);
+            } else {
+                v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.x) + row + k);
+            }
+        }
+        return v;
+    }
+    float *e = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (k + i < K)
+            e[i] = a.f16 ? __half2float(static_cast<const __half *>(a.x)[row + k + i]) : static_cast<const float *>(a.x)[row + k + i];
+    return v;
+}
+__device__ __forceinline__ float4 load_f4(const Q4Args &a, const float *p, int k, int K) {
+    if (a.vec) return k < K ? *reinterpret_cast<const float4 *>(p + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(k < K ? p[k] : 0.0f, k + 1 < K ? p[k + 1] : 0.0f, k + 2 < K ? p[k + 2] : 0.0f, k + 3 < K ? p[k + 3] : 0.0f);
+}
+
+__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(unsigned dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
@@ -213,25 +253,28 @@ __device__ __forceinline__ float row_reduce(float v, float *scratch, int w0, int
     return v;
 }
 
-// NT n tiles of 8 columns, TP feature tiles that share an operand of x, NP columns a row.
-template <int NT, int TP, int NP>
+// NT n tiles of 8 columns, TP feature tiles that share an operand of x, NP columns a row, PC scale groups a chunk.
+template <int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
-    constexpr int kDepth = TP == 1 ? 8 : 4;
-    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int S = Q4Ring<TP>::kStages, CB = 512 + 32 * PC;
+    constexpr int kHeld = 2;                                      // groups of four x that a thread keeps between passes
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float scratch[kQ4Warps], mean_s[G2_Q4_MAX_ROWS], rstd_s[G2_Q4_MAX_ROWS], up_s[G2_Q4_MAX_ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int M = a.M, K = sh.K;
     const int stride = a.slice * kChunk + 32;                     // halves of a column; 64 bytes past a multiple of 128
-    __half *xs = reinterpret_cast<__half *>(smem);                // [8 NT][stride]
-    float *pieces = reinterpret_cast<float *>(smem + (size_t)8 * NT * stride * 2);   // [tiles + warps][M][16 TP]
-    float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;               // [M][tiles][16 TP], only with slices
+    unsigned char *ring = smem + (size_t)warp * S * TP * CB;      // [stage][TP] chunks
+    __half *xs = reinterpret_cast<__half *>(smem + (size_t)kQ4Warps * S * TP * CB);   // [8 NT][stride]
+    float *pieces = reinterpret_cast<float *>(xs + (size_t)8 * NT * stride);          // [tiles + warps][M][16 TP]
+    float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;                // [M][tiles][16 TP], only with slices
+    const unsigned ring_addr = smem_addr(ring);
     const int ntiles = (sh.tiles + TP - 1) / TP;                  // of TP feature tiles
     const int tile0 = (int)((long long)blockIdx.x * ntiles / gridDim.x), tile1 = (int)((long long)(blockIdx.x + 1) * ntiles / gridDim.x);
     // warps of a row of x in the passes over it
     int wpr = kQ4Warps;
     while (wpr * M > kQ4Warps && wpr > 1) wpr >>= 1;
     const int rows_at_once = kQ4Warps / wpr, w0 = warp / wpr * wpr;
-    const int first = (warp - w0) * 32 + lane, step = wpr * 32;
+    const int first = ((warp - w0) * 32 + lane) * 4, step = wpr * 128;
 
     for (int tile = tile0; tile < tile1; tile += a.most) {
         const int R = min(a.most, tile1 - tile);
@@ -240,19 +283,17 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             const int U = R * nc, W = min(kQ4Warps, U);
             const int u0 = warp < W ? warp * U / W : 0, u1 = warp < W ? (warp + 1) * U / W : 0;
 
-            // ---- the first loads of the codes
-            uint4 w[kDepth][TP];
-            unsigned sc[kDepth][TP][2];
-            int lr = nc ? u0 / nc : 0, lc = nc ? u0 % nc : 0, lu = u0;
-            auto load = [&](int p) {
+            // ---- the first copies of the codes
+            int lr = u0 / nc, lc = u0 % nc, lu = u0;
+            auto issue = [&]() {
                 if (lu < u1) {
+                    const unsigned slot = ring_addr + (unsigned)((lu - u0) % S) * TP * CB;
 #pragma unroll
                     for (int x = 0; x < TP; ++x) {
                         const int ft = min((tile + lr) * TP + x, sh.tiles - 1);   // a last odd tile is read twice
-                        w[p][x] = __ldcs(a.codes + ((size_t)ft * sh.chunks + c0 + lc) * 32 + lane);
-                        const unsigned *s = a.scales + ((size_t)ft * sh.groups + (c0 + lc) * kChunk / sh.group) * 8 + g;
-                        sc[p][x][0] = __ldg(s);
-                        if (sh.group == 32) sc[p][x][1] = __ldg(s + 8);
+                        const unsigned char *src = a.packed + sh.at(ft, c0 + lc) + lane * 16;
+                        cp_async16(slot + x * CB + lane * 16, src);
+                        if (lane < 2 * PC) cp_async16(slot + x * CB + 512 + lane * 16, src + 512);
                     }
                     if (++lc == nc) {
                         lc = 0;
@@ -260,29 +301,45 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     }
                     ++lu;
                 }
+                cp_commit();
             };
 #pragma unroll
-            for (int p = 0; p < kDepth; ++p) load(p);
+            for (int p = 0; p < S - 1; ++p) issue();
 
             // ---- x of this slice, once
             if (sh.chunks > a.slice || tile == tile0) {
                 const int k0 = c0 * kChunk, kn = nc * kChunk;
-                for (int r0 = 0; r0 < M; r0 += rows_at_once) {   // columns past M rows keep what they hold
+                for (int r0 = 0; r0 < M; r0 += rows_at_once) {    // columns past M rows keep what they hold
                     const int m = r0 + warp / wpr;
                     const bool live = m < M;
                     const size_t row = (size_t)(live ? m : 0) * K;
                     float mu = 0.0f, rstd = 1.0f;
                     if (a.gamma) {
                         if (c0 == 0 && tile == tile0) {
+                            float4 held[kHeld];
                             float s = 0.0f;
-                            for (int k = first; k < K; k += step) s += load_x(a, row + k);
-                            mu = row_reduce<false>(s, scratch, w0, wpr) / K;
-                            float v = 0.0f;
-                            for (int k = first; k < K; k += step) {
-                                const float d = load_x(a, row + k) - mu;
-                                v = fmaf(d, d, v);
+#pragma unroll
+                            for (int i = 0; i < kHeld; ++i) {
+                                held[i] = load_x4(a, row, first + i * step, K);
+                                s += (held[i].x + held[i].y) + (held[i].z + held[i].w);
                             }
-                            rstd = rsqrtf(row_reduce<false>(v, scratch, w0, wpr) / K + 1e-5f);
+                            for (int k = first + kHeld * step; k < K; k += step) {
+                                const float4 v = load_x4(a, row, k, K);
+                                s += (v.x + v.y) + (v.z + v.w);
+                            }
+                            mu = row_reduce<false>(s, scratch, w0, wpr) / K;
+                            float q = 0.0f;
+                            auto square = [&](const float4 &v, int k) {
+                                const float d0 = v.x - mu, d1 = v.y - mu, d2 = v.z - mu, d3 = v.w - mu;
+                                if (k < K) q = fmaf(d0, d0, q);
+                                if (k + 1 < K) q = fmaf(d1, d1, q);
+                                if (k + 2 < K) q = fmaf(d2, d2, q);
+                                if (k + 3 < K) q = fmaf(d3, d3, q);
+                            };
+#pragma unroll
+                            for (int i = 0; i < kHeld; ++i) square(held[i], first + i * step);
+                            for (int k = first + kHeld * step; k < K; k += step) square(load_x4(a, row, k, K), k);
+                            rstd = rsqrtf(row_reduce<false>(q, scratch, w0, wpr) / K + 1e-5f);
                             if (live && first == 0) {
                                 mean_s[m] = mu;
                                 rstd_s[m] = rstd;
@@ -292,27 +349,58 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                             rstd = rstd_s[live ? m : 0];
                         }
                     }
-                    auto value = [&](int k) -> float {
-                        if (k >= K) return 0.0f;
-                        float v = load_x(a, row + k);
-                        if (a.gamma) v = fmaf((v - mu) * rstd, a.gamma[k], a.beta[k]);
+                    auto value = [&](int k) -> float4 {           // x'[m][k .. k + 3], 0 past K
+                        float4 v = load_x4(a, row, k, K);
+                        if (a.gamma) {
+                            const float4 ga = load_f4(a, a.gamma, k, K), be = load_f4(a, a.beta, k, K);
+                            v.x = fmaf((v.x - mu) * rstd, ga.x, be.x);
+                            v.y = fmaf((v.y - mu) * rstd, ga.y, be.y);
+                            v.z = fmaf((v.z - mu) * rstd, ga.z, be.z);
+                            v.w = fmaf((v.w - mu) * rstd, ga.w, be.w);
+                        }
                         return v;
                     };
+                    const int begin = live ? first : kn;
                     if (NP == 1) {
-                        for (int k = live ? first : kn; k < kn; k += step) xs[m * stride + k] = __float2half_rn(value(k0 + k));
+                        for (int k = begin; k < kn; k += step) {
+                            const float4 v = value(k0 + k);
+                            uint2 o;
+                            o.x = bits(__floats2half2_rn(v.x, v.y));
+                            o.y = bits(__floats2half2_rn(v.z, v.w));
+                            *reinterpret_cast<uint2 *>(xs + m * stride + k) = o;
+                        }
                     } else {
+                        float4 held[kHeld];
                         float peak = 0.0f;
-                        for (int k = live ? first : kn; k < kn; k += step) peak = fmaxf(peak, fabsf(value(k0 + k)));
+                        auto larger = [&](const float4 &v) {
+                            peak = fmaxf(fmaxf(peak, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                        };
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i) {
+                            held[i] = value(k0 + first + i * step);
+                            if (first + i * step < kn) larger(held[i]);
+                        }
+                        for (int k = begin + kHeld * step; k < kn; k += step) larger(value(k0 + k));
                         peak = row_reduce<true>(peak, scratch, w0, wpr);
                         const int e = max(-126, min(126, (int)(__float_as_uint(peak) >> 23) - 127));
                         const float down = __uint_as_float((unsigned)(127 - e) << 23);
                         if (live && first == 0) up_s[m] = __uint_as_float((unsigned)(127 + e) << 23);
-                        for (int k = live ? first : kn; k < kn; k += step) {
-                            const float v = value(k0 + k) * down;
-                            const __half h = __float2half_rn(v);
-                            xs[2 * m * stride + k] = h;
-                            xs[(2 * m + 1) * stride + k] = __float2half_rn((v - __half2float(h)) * kLoScale);
-                        }
+                        auto put = [&](const float4 &v, int k) {
+                            const float x0 = v.x * down, x1 = v.y * down, x2 = v.z * down, x3 = v.w * down;
+                            const __half2 a0 = __floats2half2_rn(x0, x1), a1 = __floats2half2_rn(x2, x3);
+                            const float2 b0 = __half22float2(a0), b1 = __half22float2(a1);
+                            uint2 hi, lo;
+                            hi.x = bits(a0);
+                            hi.y = bits(a1);
+                            lo.x = bits(__floats2half2_rn((x0 - b0.x) * kLoScale, (x1 - b0.y) * kLoScale));
+                            lo.y = bits(__floats2half2_rn((x2 - b1.x) * kLoScale, (x3 - b1.y) * kLoScale));
+                            *reinterpret_cast<uint2 *>(xs + 2 * m * stride + k) = hi;
+                            *reinterpret_cast<uint2 *>(xs + (2 * m + 1) * stride + k) = lo;
+                        };
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i)
+                            if (live && first + i * step < kn) put(held[i], first + i * step);
+                        for (int k = begin + kHeld * step; k < kn; k += step) put(value(k0 + k), k);
                     }
                 }
             }
@@ -324,79 +412,81 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             for (int x = 0; x < TP; ++x)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) tot[x][n][0] = tot[x][n][1] = tot[x][n][2] = tot[x][n][3] = 0.0f;
-            int r = nc ? u0 / nc : 0, c = nc ? u0 % nc : 0;
-            auto flush = [&]() {   // a tile's (part of a) sum to its piece
-                float *o = pieces + (size_t)(r + warp) * M * 16 * TP;
+            int r = u0 / nc, c = u0 % nc, stage = 0;
+            const __half *xcol = xs + g * stride + t * 8;
+            for (int u = u0; u < u1; ++u) {
+                cp_wait<S - 2>();
+                __syncwarp();
+                issue();
+                const unsigned char *slot = ring + stage * TP * CB;
+                stage = stage + 1 == S ? 0 : stage + 1;
+                uint4 b[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int x = 0; x < TP; ++x) {
-                        float (&v)[4] = tot[x][n];
-                        if (NP == 2) {
-                            const int m = n * 4 + t;
-                            if (m < M) {
-                                o[m * 16 * TP + x * 16 + g] = fmaf(v[1], kLoUnscale, v[0]);
-                                o[m * 16 * TP + x * 16 + g + 8] = fmaf(v[3], kLoUnscale, v[2]);
-                            }
-                        } else {
+                    for (int half = 0; half < 2; ++half)
+                        b[n][half] = *reinterpret_cast<const uint4 *>(xcol + n * 8 * stride + c * kChunk + half * 32);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int m = n * 8 + 2 * t + (i & 1);
-                                if (m < M) o[m * 16 * TP + x * 16 + g + (i >> 1) * 8] = v[i];
-                            }
-                        }
-                        v[0] = v[1] = v[2] = v[3] = 0.0f;
-                    }
-            };
-            for (int u = u0; u < u1; u += kDepth) {
+                for (int x = 0; x < TP; ++x) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
+                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+                    unsigned sc[PC];
 #pragma unroll
-                for (int p = 0; p < kDepth; ++p) {
-                    if (u + p < u1) {
-                        uint4 b[NT][2];
+                    for (int i = 0; i < PC; ++i) sc[i] = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + i * 32 + g * 4);
+                    float acc[NT][4];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int half = 0; half < 2; ++half)
-                                b[n][half] = *reinterpret_cast<const uint4 *>(xs + (n * 8 + g) * stride + c * kChunk + half * 32 + t * 8);
-#pragma unroll
-                        for (int x = 0; x < TP; ++x) {
-                            const unsigned words[4] = {w[p][x].x, w[p][x].y, w[p][x].z, w[p][x].w};
-                            float acc[NT][4];
+                    for (int i = 0; i < 4; ++i) {
+                        if (i == 0 || (PC == 2 && i == 2))
 #pragma unroll
                             for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-                            auto scaled = [&](unsigned s) {
-                                const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+                        unsigned f[4];
+                        codes_to_half(words[i], f);
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    tot[x][n][0] = fmaf(acc[n][0], lo, tot[x][n][0]);
-                                    tot[x][n][1] = fmaf(acc[n][1], lo, tot[x][n][1]);
-                                    tot[x][n][2] = fmaf(acc[n][2], hi, tot[x][n][2]);
-                                    tot[x][n][3] = fmaf(acc[n][3], hi, tot[x][n][3]);
-                                    acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-                                }
-                            };
+                        for (int n = 0; n < NT; ++n) {
+                            const uint4 &v = b[n][i >> 1];
+                            mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
+                        }
+                        if (i == 3 || (PC == 2 && i == 1)) {      // the group's sum, scaled
+                            const unsigned s = sc[PC == 2 ? i >> 1 : 0];
+                            const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                unsigned f[4];
-                                codes_to_half(words[i], f);
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    const uint4 &v = b[n][i >> 1];
-                                    mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
-                                }
-                                if (i == 1 && sh.group == 32) scaled(sc[p][x][0]);
+                            for (int n = 0; n < NT; ++n) {
+                                tot[x][n][0] = fmaf(acc[n][0], lo, tot[x][n][0]);
+                                tot[x][n][1] = fmaf(acc[n][1], lo, tot[x][n][1]);
+                                tot[x][n][2] = fmaf(acc[n][2], hi, tot[x][n][2]);
+                                tot[x][n][3] = fmaf(acc[n][3], hi, tot[x][n][3]);
                             }
-                            scaled(sh.group == 32 ? sc[p][x][1] : sc[p][x][0]);
                         }
-                        if (++c == nc || u + p == u1 - 1) flush();
-                        if (c == nc) {
-                            c = 0;
-                            ++r;
-                        }
-                        load(p);
                     }
                 }
+                ++c;
+                if (c == nc || u == u1 - 1) {                     // (this warp's part of) a tile is done
+                    float *o = pieces + (size_t)(r + warp) * M * 16 * TP + g;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int x = 0; x < TP; ++x) {
+                            float (&v)[4] = tot[x][n];
+                            if (NP == 2) {
+                                const int m = n * 4 + t;
+                                if (m < M) {
+                                    o[m * 16 * TP + x * 16] = fmaf(v[1], kLoUnscale, v[0]);
+                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[3], kLoUnscale, v[2]);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int m = n * 8 + 2 * t + (i & 1);
+                                    if (m < M) o[m * 16 * TP + x * 16 + (i >> 1) * 8] = v[i];
+                                }
+                            }
+                            v[0] = v[1] = v[2] = v[3] = 0.0f;
+                        }
+                    c = 0;
+                    ++r;
+                }
             }
+            cp_wait<0>();
             __syncthreads();
 
             // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
@@ -436,20 +526,31 @@ int q4_sms() {
     return n;
 }
 
-template <int NT, int TP, int NP>
+template <int NT, int TP, int NP, int PC>
 int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
-    auto kernel = q4_matvec_kernel<NT, TP, NP>;
+    auto kernel = q4_matvec_kernel<NT, TP, NP, PC>;
     const int ntiles = (sh.tiles + TP - 1) / TP, grid = std::min(q4_sms(), ntiles);
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
-    // equal slices of at most kXBytes of staged columns
-    const int fit = (kXBytes / (8 * NT * 2) - 32) / kChunk, slices = (sh.chunks + fit - 1) / fit;
+    // x in equal slices that fit beside the ring and the sums
+    const size_t ring = (size_t)kQ4Warps * Q4Ring<TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)a.M * 16 * TP * 4;
+    size_t sums = (a.most + kQ4Warps) * tile;
+    int fit = (int)((kQ4Smem - ring - sums) / (8 * NT * 2) - 32) / kChunk;
+    if (fit < sh.chunks) {
+        sums += a.most * tile;
+        fit = (int)((kQ4Smem - ring - sums) / (8 * NT * 2) - 32) / kChunk;
+    }
+    const int slices = (sh.chunks + fit - 1) / fit;
     a.slice = (sh.chunks + slices - 1) / slices;
-    const size_t smem = (size_t)8 * NT * (a.slice * kChunk + 32) * 2 +
-                        (size_t)(a.most + kQ4Warps + (slices > 1 ? a.most : 0)) * a.M * 16 * TP * 4;
+    const size_t smem = ring + (size_t)8 * NT * (a.slice * kChunk + 32) * 2 + sums;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
     kernel<<<grid, kQ4Threads, smem, st>>>(a, sh);
     return launch_status("g2k_matvec_q4");
+}
+
+template <int NT, int TP, int NP>
+int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
+    return sh.per_chunk == 2 ? launch_q4<NT, TP, NP, 2>(a, sh, st) : launch_q4<NT, TP, NP, 1>(a, sh, st);
 }
 
 bool bad_shape(int N, int K, int group) {
@@ -483,14 +584,13 @@ extern "C" int g2k_q4_pack(const void *W, int dtype, int transposed, void *packe
     if (!aligned(W, dtype == G2_F32 ? 4 : 2)) return arg_error(G2_ERR_ARG, who, "W is not aligned to its elements");
     if ((rc = check_device_ptrs(who, {W, packed}))) return rc;
     const Q4Shape sh(N, K, group);
-    unsigned *codes = static_cast<unsigned *>(packed);
-    auto *scales = reinterpret_cast<__nv_bfloat16 *>(static_cast<char *>(packed) + sh.scale_off);
-    const dim3 grid(sh.tiles, sh.groups);
+    unsigned char *out = static_cast<unsigned char *>(packed);
+    const dim3 grid(sh.tiles, (sh.chunks * kChunk + group - 1) / group);   // groups past K too: their codes are 0
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == G2_F32)
-        q4_pack_kernel<float><<<grid, kPackThreads, 0, st>>>(static_cast<const float *>(W), transposed, codes, scales, sh);
+        q4_pack_kernel<float><<<grid, kPackThreads, 0, st>>>(static_cast<const float *>(W), transposed, out, sh);
     else
-        q4_pack_kernel<__half><<<grid, kPackThreads, 0, st>>>(static_cast<const __half *>(W), transposed, codes, scales, sh);
+        q4_pack_kernel<__half><<<grid, kPackThreads, 0, st>>>(static_cast<const __half *>(W), transposed, out, sh);
     return launch_status(who);
 }
 
@@ -501,11 +601,9 @@ extern "C" int g2k_q4_unpack(const void *packed, float *W, int N, int K, int gro
     if ((rc = check_packed(who, packed, N, K, group))) return rc;
     if ((rc = check_device_ptrs(who, {W, packed}))) return rc;
     const Q4Shape sh(N, K, group);
-    const unsigned *codes = static_cast<const unsigned *>(packed);
-    auto *scales = reinterpret_cast<const __nv_bfloat16 *>(static_cast<const char *>(packed) + sh.scale_off);
     const long long blocks = ((long long)K * N + 255) / 256;
     if (blocks > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "matrix too large");
-    q4_unpack_kernel<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(codes, scales, W, sh);
+    q4_unpack_kernel<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(static_cast<const unsigned char *>(packed), W, sh);
     return launch_status(who);
 }
 
@@ -525,9 +623,9 @@ extern "C" int g2k_matvec_q4(const void *x, const void *packed, const float *bia
         return arg_error(G2_ERR_ARG, who, "an array is not aligned to its elements");
     if ((rc = check_device_ptrs(who, {x, packed, bias, residual, y, ln_gamma, ln_beta}))) return rc;
     const Q4Shape sh(N, K, group);
-    const Q4Args a{x, static_cast<const uint4 *>(packed),
-                   reinterpret_cast<const unsigned *>(static_cast<const char *>(packed) + sh.scale_off), bias, ln_gamma,
-                   ln_beta, residual, y, M, apply_gelu, dtype == G2_F16, 0};
+    const bool vec = K % 4 == 0 && aligned(x, 4 * es) && aligned(ln_gamma, 16) && aligned(ln_beta, 16);
+    const Q4Args a{x, static_cast<const unsigned char *>(packed), bias, ln_gamma, ln_beta, residual, y, M, apply_gelu,
+                   dtype == G2_F16, vec, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     // more rows than one n tile holds: two feature tiles share each operand of x, which halves its reads
     if (dtype == G2_F16 && !ln_gamma) return M <= 8 ? launch_q4<1, 1, 1>(a, sh, st) : launch_q4<2, 2, 1>(a, sh, st);

@@ -22,9 +22,11 @@ def code(f, *a):
 
 
 def test_q4_sizes():
-    assert g2.q4_bytes(16, 64, 64) == 512 + 32
-    assert g2.q4_bytes(17, 65, 32) == 2 * 2 * 512 + 2 * 4 * 32
-    assert g2.q4_bytes(1, 32768, 128) == 512 * 512 + 256 * 32
+    for n, k in ((16, 64), (17, 65), (1, 32768), (50257, 1600)):
+        pad = -(-n // 16) * 16 * (-(-k // 64) * 64)            # whole tiles of 16 columns and 64 rows
+        for g in (32, 64, 128):
+            scales = 2 * pad // min(g, 64)                     # a scale for each part of 64 rows at least
+            assert g2.q4_bytes(n, k, g) == pad // 2 + scales
     for n, k, g in ((0, 1, 32), (1, 0, 32), (1, 1, 16), (1, 1, 0), (1, 32769, 32), (-4, 64, 64), (2 ** 31 - 1, 64, 64)):
         assert g2.q4_bytes(n, k, g) == 0
 
