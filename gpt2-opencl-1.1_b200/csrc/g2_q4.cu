@@ -17,7 +17,7 @@
 // so that nibbles j and j + 4 are register j of the A operand of a 16 x 8 x 16
 // tensor-core product whose k index is a permutation of the rows, and the x of
 // a lane's words s and s + 1 are eight consecutive ones.  Rows past K and columns
-// past N hold code 0.
+// past N, up to a multiple of 32, hold code 0.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -37,7 +37,7 @@ struct Q4Shape {
     int per_chunk;       // scale groups of a chunk
     int chunk_bytes;
     __host__ __device__ Q4Shape(int N_, int K_, int group_) : N(N_), K(K_), group(group_) {
-        tiles = (N + kTile - 1) / kTile;
+        tiles = (N + 2 * kTile - 1) / (2 * kTile) * 2;   // in pairs
         chunks = (K + kChunk - 1) / kChunk;
         per_chunk = group == 32 ? 2 : 1;
         chunk_bytes = 512 + 32 * per_chunk;
@@ -172,6 +172,7 @@ struct Q4Args {
     void *y;
     int M, gelu, f16;
     int vec;                               // rows of x, gamma and beta can be read four elements at a time
+    int copy;                              // fp16 rows of x can be copied 16 bytes at a time
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
 };
@@ -205,8 +206,8 @@ __device__ __forceinline__ float4 load_f4(const Q4Args &a, const float *p, int k
 }
 
 __device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(unsigned dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp_async16(unsigned dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     constexpr int kHeld = 2;                                      // groups of four x that a thread keeps between passes
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float scratch[kQ4Warps], mean_s[G2_Q4_MAX_ROWS], rstd_s[G2_Q4_MAX_ROWS], up_s[G2_Q4_MAX_ROWS];
+    __shared__ unsigned char range_s[kMaxTiles][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int M = a.M, K = sh.K;
     const int stride = a.slice * kChunk + 32;                     // halves of a column; 64 bytes past a multiple of 128
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     float *pieces = reinterpret_cast<float *>(xs + (size_t)8 * NT * stride);          // [tiles + warps][M][16 TP]
     float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;                // [M][tiles][16 TP], only with slices
     const unsigned ring_addr = smem_addr(ring);
-    const int ntiles = (sh.tiles + TP - 1) / TP;                  // of TP feature tiles
+    const int ntiles = sh.tiles / TP;                             // of TP feature tiles
     const int tile0 = (int)((long long)blockIdx.x * ntiles / gridDim.x), tile1 = (int)((long long)(blockIdx.x + 1) * ntiles / gridDim.x);
     // warps of a row of x in the passes over it
     int wpr = kQ4Warps;
@@ -283,23 +285,36 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             const int U = R * nc, W = min(kQ4Warps, U);
             const int u0 = warp < W ? warp * U / W : 0, u1 = warp < W ? (warp + 1) * U / W : 0;
 
+            const bool stage_x = sh.chunks > a.slice || tile == tile0;
+            if (NP == 1 && a.copy && stage_x) {                   // x as it is, ahead of the codes
+                const int per_row = nc * (kChunk / 8);
+                for (int i = tid; i < M * per_row; i += kQ4Threads) {
+                    const int m = i / per_row, k = i % per_row * 8, left = K - c0 * kChunk - k;
+                    cp_async16(smem_addr(xs + m * stride + k),
+                               static_cast<const __half *>(a.x) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
+                }
+            }
+            cp_commit();
+
             // ---- the first copies of the codes
-            int lr = u0 / nc, lc = u0 % nc, lu = u0;
+            const size_t tile_bytes = (size_t)sh.chunks * CB;
+            const unsigned char *src = a.packed + sh.at((tile + u0 / nc) * TP, c0 + u0 % nc) + lane * 16;
+            int left = u1 - u0, lc = nc - u0 % nc, put = 0;       // units to copy, chunks left of the tile, slot
             auto issue = [&]() {
-                if (lu < u1) {
-                    const unsigned slot = ring_addr + (unsigned)((lu - u0) % S) * TP * CB;
+                if (left > 0) {
+                    const unsigned slot = ring_addr + put * (TP * CB) + lane * 16;
 #pragma unroll
                     for (int x = 0; x < TP; ++x) {
-                        const int ft = min((tile + lr) * TP + x, sh.tiles - 1);   // a last odd tile is read twice
-                        const unsigned char *src = a.packed + sh.at(ft, c0 + lc) + lane * 16;
-                        cp_async16(slot + x * CB + lane * 16, src);
-                        if (lane < 2 * PC) cp_async16(slot + x * CB + 512 + lane * 16, src + 512);
+                        cp_async16(slot + x * CB, src + x * tile_bytes, 16);
+                        if (lane < 2 * PC) cp_async16(slot + x * CB + 512, src + x * tile_bytes + 512, 16);
                     }
-                    if (++lc == nc) {
-                        lc = 0;
-                        ++lr;
+                    src += CB;
+                    if (--lc == 0) {
+                        lc = nc;
+                        src += TP * tile_bytes - nc * CB;
                     }
-                    ++lu;
+                    put = put + 1 == S ? 0 : put + 1;
+                    --left;
                 }
                 cp_commit();
             };
@@ -307,7 +322,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             for (int p = 0; p < S - 1; ++p) issue();
 
             // ---- x of this slice, once
-            if (sh.chunks > a.slice || tile == tile0) {
+            if (stage_x && !(NP == 1 && a.copy)) {
                 const int k0 = c0 * kChunk, kn = nc * kChunk;
                 for (int r0 = 0; r0 < M; r0 += rows_at_once) {    // columns past M rows keep what they hold
                     const int m = r0 + warp / wpr;
@@ -404,6 +419,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     }
                 }
             }
+            cp_wait<S - 1>();                                     // x, where it was copied
             __syncthreads();
 
             // ---- the warp's units
@@ -412,20 +428,19 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             for (int x = 0; x < TP; ++x)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) tot[x][n][0] = tot[x][n][1] = tot[x][n][2] = tot[x][n][3] = 0.0f;
-            int r = u0 / nc, c = u0 % nc, stage = 0;
-            const __half *xcol = xs + g * stride + t * 8;
+            int r = u0 / nc, c = nc - u0 % nc;                    // tile, chunks left of it
+            const __half *xk = xs + g * stride + t * 8 + u0 % nc * kChunk;
+            const unsigned char *slot = ring;
             for (int u = u0; u < u1; ++u) {
                 cp_wait<S - 2>();
                 __syncwarp();
                 issue();
-                const unsigned char *slot = ring + stage * TP * CB;
-                stage = stage + 1 == S ? 0 : stage + 1;
                 uint4 b[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
-                        b[n][half] = *reinterpret_cast<const uint4 *>(xcol + n * 8 * stride + c * kChunk + half * 32);
+                        b[n][half] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride + half * 32);
 #pragma unroll
                 for (int x = 0; x < TP; ++x) {
                     const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
@@ -459,8 +474,9 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                         }
                     }
                 }
-                ++c;
-                if (c == nc || u == u1 - 1) {                     // (this warp's part of) a tile is done
+                slot = slot + TP * CB == ring + S * TP * CB ? ring : slot + TP * CB;
+                xk += kChunk;
+                if (--c == 0 || u == u1 - 1) {                    // (this warp's part of) a tile is done
                     float *o = pieces + (size_t)(r + warp) * M * 16 * TP + g;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -482,38 +498,43 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                             }
                             v[0] = v[1] = v[2] = v[3] = 0.0f;
                         }
-                    c = 0;
+                    c = nc;
+                    xk -= nc * kChunk;
                     ++r;
                 }
             }
             cp_wait<0>();
+            if (tid < R) {                                        // the warps that have units of each tile
+                range_s[tid][0] = (unsigned char)(((tid * nc + 1) * W - 1) / U);
+                range_s[tid][1] = (unsigned char)(((tid + 1) * nc * W - 1) / U);
+            }
             __syncthreads();
 
             // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
-            for (int o = tid; o < R * M * 16 * TP; o += kQ4Threads) {
-                const int f = o % (16 * TP), rr = o / (16 * TP) % R, m = o / (16 * TP * R);
-                const int wa = ((rr * nc + 1) * W - 1) / U, wb = ((rr * nc + nc) * W - 1) / U;   // the warps of its units
-                float v = 0.0f;
-                for (int x = wa; x <= wb; ++x) v += pieces[((size_t)(rr + x) * M + m) * 16 * TP + f];
-                if (NP == 2) v *= up_s[m];
-                if (c0 > 0) v += total[o];
-                if (c0 + nc < sh.chunks) {
-                    total[o] = v;
-                    continue;
+            const int span = R * 16 * TP, together = max(1, kQ4Threads / span);   // rows of y taken at once
+            const int i0 = together == 1 ? tid : tid < together * span ? tid % span : span;
+            for (int m = together == 1 ? 0 : tid / span; m < M; m += together)
+                for (int i = i0; i < span; i += together == 1 ? kQ4Threads : span) {
+                    const int f = i % (16 * TP), rr = i / (16 * TP), o = m * span + i, n = (tile + rr) * 16 * TP + f;
+                    float v = 0.0f;
+                    for (int x = range_s[rr][0]; x <= range_s[rr][1]; ++x) v += pieces[((rr + x) * M + m) * 16 * TP + f];
+                    if (NP == 2) v *= up_s[m];
+                    if (c0 > 0) v += total[o];
+                    if (c0 + nc < sh.chunks) {
+                        total[o] = v;
+                    } else if (n < sh.N) {
+                        if (a.bias) v += a.bias[n];
+                        if (a.gelu) v = gelu_f(v);
+                        const size_t at = (size_t)m * sh.N + n;
+                        if (a.f16) {
+                            if (a.residual) v += __half2float(static_cast<const __half *>(a.residual)[at]);
+                            static_cast<__half *>(a.y)[at] = __float2half_rn(v);
+                        } else {
+                            if (a.residual) v += static_cast<const float *>(a.residual)[at];
+                            static_cast<float *>(a.y)[at] = v;
+                        }
+                    }
                 }
-                const int n = (tile + rr) * 16 * TP + f;
-                if (n >= sh.N) continue;
-                if (a.bias) v += a.bias[n];
-                if (a.gelu) v = gelu_f(v);
-                const size_t at = (size_t)m * sh.N + n;
-                if (a.f16) {
-                    if (a.residual) v += __half2float(static_cast<const __half *>(a.residual)[at]);
-                    static_cast<__half *>(a.y)[at] = __float2half_rn(v);
-                } else {
-                    if (a.residual) v += static_cast<const float *>(a.residual)[at];
-                    static_cast<float *>(a.y)[at] = v;
-                }
-            }
             __syncthreads();
         }
     }
@@ -529,7 +550,7 @@ int q4_sms() {
 template <int NT, int TP, int NP, int PC>
 int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     auto kernel = q4_matvec_kernel<NT, TP, NP, PC>;
-    const int ntiles = (sh.tiles + TP - 1) / TP, grid = std::min(q4_sms(), ntiles);
+    const int ntiles = sh.tiles / TP, grid = std::min(q4_sms(), ntiles);
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
     // x in equal slices that fit beside the ring and the sums
     const size_t ring = (size_t)kQ4Warps * Q4Ring<TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)a.M * 16 * TP * 4;
@@ -555,7 +576,7 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
 
 bool bad_shape(int N, int K, int group) {
     return N < 1 || K < 1 || K > G2_Q4_MAX_K || (group != 32 && group != 64 && group != 128) ||
-           ((long long)N + kTile - 1) / kTile > 0x7fffffff / kTile;
+           (long long)N + 2 * kTile > 0x7fffffff;
 }
 
 }  // namespace
@@ -625,9 +646,13 @@ extern "C" int g2k_matvec_q4(const void *x, const void *packed, const float *bia
     const Q4Shape sh(N, K, group);
     const bool vec = K % 4 == 0 && aligned(x, 4 * es) && aligned(ln_gamma, 16) && aligned(ln_beta, 16);
     const Q4Args a{x, static_cast<const unsigned char *>(packed), bias, ln_gamma, ln_beta, residual, y, M, apply_gelu,
-                   dtype == G2_F16, vec, 0, 0};
+                   dtype == G2_F16, vec, K % 8 == 0 && !ln_gamma && aligned(x, 16), 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
-    // more rows than one n tile holds: two feature tiles share each operand of x, which halves its reads
-    if (dtype == G2_F16 && !ln_gamma) return M <= 8 ? launch_q4<1, 1, 1>(a, sh, st) : launch_q4<2, 2, 1>(a, sh, st);
-    return M <= 4 ? launch_q4<1, 1, 2>(a, sh, st) : M <= 8 ? launch_q4<2, 2, 2>(a, sh, st) : launch_q4<4, 2, 2>(a, sh, st);
+    // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
+    // matrices of fewer pairs than SMs (and one n tile) are better spread one by one.
+    const bool one = sh.tiles / 2 < q4_sms();
+    if (dtype == G2_F16 && !ln_gamma)
+        return M > 8 ? launch_q4<2, 2, 1>(a, sh, st) : one ? launch_q4<1, 1, 1>(a, sh, st) : launch_q4<1, 2, 1>(a, sh, st);
+    return M > 8 ? launch_q4<4, 2, 2>(a, sh, st) : M > 4 ? launch_q4<2, 2, 2>(a, sh, st)
+         : one ? launch_q4<1, 1, 2>(a, sh, st) : launch_q4<1, 2, 2>(a, sh, st);
 }

@@ -23,7 +23,7 @@ def code(f, *a):
 
 def test_q4_sizes():
     for n, k in ((16, 64), (17, 65), (1, 32768), (50257, 1600)):
-        pad = -(-n // 16) * 16 * (-(-k // 64) * 64)            # whole tiles of 16 columns and 64 rows
+        pad = -(-n // 32) * 32 * (-(-k // 64) * 64)            # whole blocks of 32 columns and 64 rows
         for g in (32, 64, 128):
             scales = 2 * pad // min(g, 64)                     # a scale for each part of 64 rows at least
             assert g2.q4_bytes(n, k, g) == pad // 2 + scales
