@@ -10,14 +10,14 @@
 //   [tile][chunk] { codes [lane 0..31][4 words], scales [1, or 2 for groups of 32][8][2] bf16 }
 // A scale pair is that of features g and g + 8; a group of 128 rows has its scale
 // in both of its chunks (3% more bytes, and a chunk needs nothing but itself).
-// Word s of lane (g = lane / 4, t = lane % 4) holds features g and g + 8 at rows
-// 64 chunk + 32 (s / 2) + 8 t + 4 (s % 2) + {0, 1, 2, 3}, as code + 8 in nibbles
-//   0, 4: feature g,     rows +0, +1      1, 5: feature g + 8, rows +0, +1
-//   2, 6: feature g,     rows +2, +3      3, 7: feature g + 8, rows +2, +3
-// so that nibbles j and j + 4 are register j of the A operand of a 16 x 8 x 16
-// tensor-core product whose k index is a permutation of the rows, and the x of
-// a lane's words s and s + 1 are eight consecutive ones.  Rows past K and columns
-// past N, up to a multiple of 32, hold code 0.
+// Word s of lane (g = lane / 4, t = lane % 4) holds features g (upper nibbles) and
+// g + 8 (lower nibbles) at rows 64 chunk + 32 (s / 2) + 8 t + 4 (s % 2) + {0, 2, 1, 3}
+// of its bytes 0..3, as two's complement.  Such a word is a thread's part of the A
+// operand of one 16 x 8 x 16 product of fp16 (registers: upper and lower nibbles of
+// bytes 0 and 2, of bytes 1 and 3), or half of it of one 16 x 8 x 32 product of int8
+// (registers: upper nibbles, lower nibbles); the k index is a permutation of the rows,
+// under which the x of a lane are consecutive.  Rows past K and columns past N, up
+// to a multiple of 32, hold code 0.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
         const float s = step[f];
         int c = 0;
         if (s > 0.0f && peak[f] < 0x7f800000u) c = max(-7, min(7, round_quotient(load(f, k), s)));
-        code[k][f] = (unsigned char)(c + 8);
+        code[k][f] = (unsigned char)(c & 15);
     }
     __syncthreads();
     // 32 lanes per 16 rows
@@ -117,9 +117,8 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(const T *W, int t
         unsigned w = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int f = g + (j & 1) * 8, k = r + (j >> 1) * 2;
-            w |= (unsigned)code[k][f] << (4 * j);
-            w |= (unsigned)code[k + 1][f] << (4 * j + 16);
+            const int shift = 16 * (j & 1) + 8 * (j >> 1);
+            w |= (unsigned)(code[r + j][g] << 4 | code[r + j][g + 8]) << shift;
         }
         reinterpret_cast<unsigned *>(packed + sh.at(tile, chunk))[lane * 4 + s] = w;
     }
@@ -133,35 +132,40 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
     const int lane = (f & 7) * 4 + ((kc >> 3) & 3), s = (kc >> 5) * 2 + ((kc >> 2) & 1);
     const unsigned char *chunk = packed + sh.at(n / kTile, k / kChunk);
     const unsigned w = reinterpret_cast<const unsigned *>(chunk)[lane * 4 + s];
-    const int nib = (f >> 3) + (r >> 1) * 2 + (r & 1) * 4;
+    const int shift = 16 * (r & 1) + 8 * (r >> 1) + (f < 8 ? 4 : 0);
     const auto *scale = reinterpret_cast<const __nv_bfloat16 *>(chunk + 512 + (sh.per_chunk == 2 ? kc / 32 * 32 : 0));
-    W[i] = (float)((int)((w >> (4 * nib)) & 15u) - 8) * __bfloat162float(scale[(f & 7) * 2 + (f >> 3)]);
+    W[i] = (float)((int)(w << (28 - shift)) >> 28) * __bfloat162float(scale[(f & 7) * 2 + (f >> 3)]);
 }
 
 // ---- the product ----------------------------------------------------------------
 // One CTA of 16 warps per SM takes an equal share of the tiles.  Its x is staged
-// in shared memory once, as columns of fp16 operands of m16n8k16 products
-// (features on m, rows of x on n): an fp16 x as it is, an fp32 one (or a
-// LayerNorm's result) as two columns, the fp16 rounding and 2^11 times the rest,
-// after a power of two has brought the row's largest below 2 (22 bits in all; the
-// columns of a few rows would be idle otherwise).
+// in shared memory once, as columns of the tensor cores' B operand (features on m,
+// rows of x on n).  A few rows leave columns idle, so each takes several:
+//   NP = 4  int8: x as a 30-bit fixed-point number below a power of two over the
+//           row's largest, one column for each of its bytes.  Codes times bytes are
+//           summed exactly in int32, and unpacking eight codes costs three
+//           instructions.  Up to 4 rows.
+//   NP = 2  fp16: the rounding of x (after a power of two has brought the row's
+//           largest below 2) and 2^11 times the rest, 22 bits in all.  Eight codes
+//           cost nine instructions.  More than 4 rows.
+//   NP = 1  fp16 x as it is.  More than 4 rows.
+// A group's sum is scaled once, in fp32.
 //
 // The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
 // that each warp streams one contiguous piece of the packed matrix whatever the
 // shape, through a ring of its own in shared memory (cp.async; registers as the
 // ring left at most a few loads in flight).  The weights are read once, and
-// nothing else is large.  Codes become fp16 exactly (0x6400 | code is 1024 +
-// code); a group's sum is taken in fp32 and scaled once.  A tile that crosses
-// warps is summed in warp order, so the bits do not depend on timing.
+// nothing else is large.  A tile that crosses warps is summed in warp order, so
+// the bits do not depend on timing.
 constexpr int kQ4Warps = 16, kQ4Threads = 32 * kQ4Warps;
 constexpr int kMaxTiles = 32;              // tiles of a CTA summed at a time
 constexpr int kQ4Smem = 220 * 1024;
 constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
 
 // One stage: a chunk of each of TP feature tiles.
-template <int TP>
+template <int NT, int TP>
 struct Q4Ring {
-    static constexpr int kStages = TP == 1 ? 8 : 5;
+    static constexpr int kStages = TP == 1 ? 8 : NT == 4 ? 4 : 5;
 };
 
 struct Q4Args {
@@ -170,39 +174,35 @@ struct Q4Args {
     const float *bias, *gamma, *beta;
     const void *residual;
     void *y;
-    int M, gelu, f16;
-    int vec;                               // rows of x, gamma and beta can be read four elements at a time
+    int M, gelu;
     int copy;                              // fp16 rows of x can be copied 16 bytes at a time
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
+    int share, extra;                      // tiles of a CTA, CTAs that have one more
 };
 
-// x[m][k .. k + 3] (0 past K) and the same of gamma or beta
-__device__ __forceinline__ float4 load_x4(const Q4Args &a, size_t row, int k, int K) {
+// p[k .. k + 3] as fp32, 0 past K; VEC: in one load (K a multiple of 4, p aligned to it)
+template <bool VEC, typename T>
+__device__ __forceinline__ float4 load_4(const T *p, int k, int K) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (a.vec) {
+    if (VEC) {
         if (k < K) {
-            if (a.f16) {
-                const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.x) + row + k);
-                const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
-                const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-                v = make_float4(p.x, p.y, q.x, q.y);
+            if (sizeof(T) == 2) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(p + k);
+                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
+                const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+                v = make_float4(a.x, a.y, b.x, b.y);
             } else {
-                v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.x) + row + k);
+                v = *reinterpret_cast<const float4 *>(p + k);
             }
         }
-        return v;
+    } else {
+        if (k < K) v.x = tof(p[k]);
+        if (k + 1 < K) v.y = tof(p[k + 1]);
+        if (k + 2 < K) v.z = tof(p[k + 2]);
+        if (k + 3 < K) v.w = tof(p[k + 3]);
     }
-    float *e = &v.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (k + i < K)
-            e[i] = a.f16 ? __half2float(static_cast<const __half *>(a.x)[row + k + i]) : static_cast<const float *>(a.x)[row + k + i];
     return v;
-}
-__device__ __forceinline__ float4 load_f4(const Q4Args &a, const float *p, int k, int K) {
-    if (a.vec) return k < K ? *reinterpret_cast<const float4 *>(p + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    return make_float4(k < K ? p[k] : 0.0f, k + 1 < K ? p[k + 1] : 0.0f, k + 2 < K ? p[k + 2] : 0.0f, k + 3 < K ? p[k + 3] : 0.0f);
 }
 
 __device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -221,57 +221,80 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&w)[4], 
                  : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
 }
 
-// (w & mask) | 0x64006400: two fp16 of 1024 + (16 times, for the upper nibbles) a code
-__device__ __forceinline__ __half2 nibbles(unsigned w, unsigned mask) {
+__device__ __forceinline__ void mma16832(int (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
+}
+
+// Two codes as two fp16 of 1024 + (16 times, for upper nibbles) code + 8: flipping a
+// two's complement nibble's sign bit adds 8, and 0x6400 | n is 1024 + n.
+__device__ __forceinline__ __half2 nibbles(unsigned w, unsigned mask, unsigned flip) {
     unsigned r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(w), "r"(mask), "r"(flip));   // (w & mask) ^ flip
     return *reinterpret_cast<__half2 *>(&r);
 }
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned *>(&v); }
 __device__ __forceinline__ void codes_to_half(unsigned w, unsigned (&f)[4]) {
-    const __half2 even = __half2half2(__ushort_as_half((unsigned short)0x6408));   // 1032
-    const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2c00)), odd = __half2half2(__ushort_as_half((unsigned short)0xd480));   // -72
-    f[0] = bits(__hsub2(nibbles(w, 0x000f000fu), even));
-    f[1] = bits(__hfma2(nibbles(w, 0x00f000f0u), sixteenth, odd));
+    const __half2 low = __half2half2(__ushort_as_half((unsigned short)0x6408));   // 1032
+    const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2c00)), up = __half2half2(__ushort_as_half((unsigned short)0xd480));   // -72
+    f[0] = bits(__hfma2(nibbles(w, 0x00f000f0u, 0x64806480u), sixteenth, up));
+    f[1] = bits(__hsub2(nibbles(w, 0x000f000fu, 0x64086408u), low));
     w >>= 8;
-    f[2] = bits(__hsub2(nibbles(w, 0x000f000fu), even));
-    f[3] = bits(__hfma2(nibbles(w, 0x00f000f0u), sixteenth, odd));
+    f[2] = bits(__hfma2(nibbles(w, 0x00f000f0u, 0x64806480u), sixteenth, up));
+    f[3] = bits(__hsub2(nibbles(w, 0x000f000fu, 0x64086408u), low));
 }
 
-// Sum (or largest) over the `n` warps of a row, which begin at warp `w0`: every lane gets it.
-template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float *scratch, int w0, int n) {
-    for (int o = 16; o; o >>= 1) {
-        const float x = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? fmaxf(v, x) : v + x;
+// Sum of v over the `n` warps of a row, a power of two that begins at warp `w0`: every lane gets it.
+// `scratch` must not be in use by an earlier reduction.
+__device__ __forceinline__ float row_sum(float v, float *scratch, int w0, int n) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (n > 1) {
+        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = scratch[w0 + (threadIdx.x & (n - 1))];
+        for (int o = n >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
-    if (n == 1) return v;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[w0];
-    for (int i = 1; i < n; ++i) v = MAX ? fmaxf(v, scratch[w0 + i]) : v + scratch[w0 + i];
+    return v;
+}
+__device__ __forceinline__ unsigned row_largest(unsigned v, unsigned *scratch, int w0, int n) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (n > 1) {
+        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = __reduce_max_sync(0xffffffffu, scratch[w0 + (threadIdx.x & (n - 1))]);
+    }
     return v;
 }
 
+// Bytes of a staged column: 64 past a multiple of 128, so that eight columns' reads meet no bank twice.
+template <int NP>
+__host__ __device__ __forceinline__ int x_stride(int slice) {
+    return NP == 4 ? (slice * kChunk + 127) / 128 * 128 + 64 : slice * kChunk * 2 + 64;
+}
+
 // NT n tiles of 8 columns, TP feature tiles that share an operand of x, NP columns a row, PC scale groups a chunk.
-template <int NT, int TP, int NP, int PC>
+template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
-    constexpr int S = Q4Ring<TP>::kStages, CB = 512 + 32 * PC;
-    constexpr int kHeld = 2;                                      // groups of four x that a thread keeps between passes
+    constexpr int S = Q4Ring<NT, TP>::kStages, CB = 512 + 32 * PC;
+    constexpr bool INT = NP == 4;
+    constexpr int kHeld = INT ? 4 : NT == 4 ? 13 : 8;             // groups of four x that a thread reads once
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float scratch[kQ4Warps], mean_s[G2_Q4_MAX_ROWS], rstd_s[G2_Q4_MAX_ROWS], up_s[G2_Q4_MAX_ROWS];
+    __shared__ float sums[kQ4Warps], squares[kQ4Warps], up_s[G2_Q4_MAX_ROWS];
+    __shared__ unsigned peaks[kQ4Warps];
+    __shared__ float2 row_stats[G2_Q4_MAX_ROWS];
     __shared__ unsigned char range_s[kMaxTiles][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int M = a.M, K = sh.K;
-    const int stride = a.slice * kChunk + 32;                     // halves of a column; 64 bytes past a multiple of 128
+    const int stride = x_stride<NP>(a.slice);                     // bytes of a column
     unsigned char *ring = smem + (size_t)warp * S * TP * CB;      // [stage][TP] chunks
-    __half *xs = reinterpret_cast<__half *>(smem + (size_t)kQ4Warps * S * TP * CB);   // [8 NT][stride]
+    unsigned char *xs = smem + (size_t)kQ4Warps * S * TP * CB;    // [8 NT][stride]
     float *pieces = reinterpret_cast<float *>(xs + (size_t)8 * NT * stride);          // [tiles + warps][M][16 TP]
     float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;                // [M][tiles][16 TP], only with slices
     const unsigned ring_addr = smem_addr(ring);
-    const int ntiles = sh.tiles / TP;                             // of TP feature tiles
-    const int tile0 = (int)((long long)blockIdx.x * ntiles / gridDim.x), tile1 = (int)((long long)(blockIdx.x + 1) * ntiles / gridDim.x);
+    const int b = blockIdx.x;                                     // tiles of TP feature tiles: a.share, or one more
+    const int tile0 = b * a.share + min(b, a.extra), tile1 = tile0 + a.share + (b < a.extra);
     // warps of a row of x in the passes over it
     int wpr = kQ4Warps;
     while (wpr * M > kQ4Warps && wpr > 1) wpr >>= 1;
@@ -282,15 +305,16 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
         const int R = min(a.most, tile1 - tile);
         for (int c0 = 0; c0 < sh.chunks; c0 += a.slice) {
             const int nc = min(a.slice, sh.chunks - c0);          // chunks of this slice
-            const int U = R * nc, W = min(kQ4Warps, U);
-            const int u0 = warp < W ? warp * U / W : 0, u1 = warp < W ? (warp + 1) * U / W : 0;
+            const int U = R * nc;                                 // units, in 16 ranges, or one a warp
+            auto range_begin = [&](int w) { return U < kQ4Warps ? min(w, U) : w * U / kQ4Warps; };
+            const int u0 = range_begin(warp), u1 = range_begin(warp + 1), r_first = u0 / nc, c_first = u0 - r_first * nc;
 
             const bool stage_x = sh.chunks > a.slice || tile == tile0;
             if (NP == 1 && a.copy && stage_x) {                   // x as it is, ahead of the codes
                 const int per_row = nc * (kChunk / 8);
                 for (int i = tid; i < M * per_row; i += kQ4Threads) {
                     const int m = i / per_row, k = i % per_row * 8, left = K - c0 * kChunk - k;
-                    cp_async16(smem_addr(xs + m * stride + k),
+                    cp_async16(smem_addr(xs + m * stride + 2 * k),
                                static_cast<const __half *>(a.x) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
                 }
             }
@@ -298,8 +322,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
 
             // ---- the first copies of the codes
             const size_t tile_bytes = (size_t)sh.chunks * CB;
-            const unsigned char *src = a.packed + sh.at((tile + u0 / nc) * TP, c0 + u0 % nc) + lane * 16;
-            int left = u1 - u0, lc = nc - u0 % nc, put = 0;       // units to copy, chunks left of the tile, slot
+            const unsigned char *src = a.packed + sh.at((tile + r_first) * TP, c0 + c_first) + lane * 16;
+            int left = u1 - u0, lc = nc - c_first, put = 0;       // units to copy, chunks left of the tile, slot
             auto issue = [&]() {
                 if (left > 0) {
                     const unsigned slot = ring_addr + put * (TP * CB) + lane * 16;
@@ -327,120 +351,168 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                 for (int r0 = 0; r0 < M; r0 += rows_at_once) {    // columns past M rows keep what they hold
                     const int m = r0 + warp / wpr;
                     const bool live = m < M;
-                    const size_t row = (size_t)(live ? m : 0) * K;
-                    float mu = 0.0f, rstd = 1.0f;
-                    if (a.gamma) {
-                        if (c0 == 0 && tile == tile0) {
-                            float4 held[kHeld];
-                            float s = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < kHeld; ++i) {
-                                held[i] = load_x4(a, row, first + i * step, K);
-                                s += (held[i].x + held[i].y) + (held[i].z + held[i].w);
-                            }
-                            for (int k = first + kHeld * step; k < K; k += step) {
-                                const float4 v = load_x4(a, row, k, K);
-                                s += (v.x + v.y) + (v.z + v.w);
-                            }
-                            mu = row_reduce<false>(s, scratch, w0, wpr) / K;
-                            float q = 0.0f;
-                            auto square = [&](const float4 &v, int k) {
-                                const float d0 = v.x - mu, d1 = v.y - mu, d2 = v.z - mu, d3 = v.w - mu;
-                                if (k < K) q = fmaf(d0, d0, q);
-                                if (k + 1 < K) q = fmaf(d1, d1, q);
-                                if (k + 2 < K) q = fmaf(d2, d2, q);
-                                if (k + 3 < K) q = fmaf(d3, d3, q);
-                            };
-#pragma unroll
-                            for (int i = 0; i < kHeld; ++i) square(held[i], first + i * step);
-                            for (int k = first + kHeld * step; k < K; k += step) square(load_x4(a, row, k, K), k);
-                            rstd = rsqrtf(row_reduce<false>(q, scratch, w0, wpr) / K + 1e-5f);
-                            if (live && first == 0) {
-                                mean_s[m] = mu;
-                                rstd_s[m] = rstd;
-                            }
-                        } else {
-                            mu = mean_s[live ? m : 0];
-                            rstd = rstd_s[live ? m : 0];
-                        }
-                    }
-                    auto value = [&](int k) -> float4 {           // x'[m][k .. k + 3], 0 past K
-                        float4 v = load_x4(a, row, k, K);
-                        if (a.gamma) {
-                            const float4 ga = load_f4(a, a.gamma, k, K), be = load_f4(a, a.beta, k, K);
-                            v.x = fmaf((v.x - mu) * rstd, ga.x, be.x);
-                            v.y = fmaf((v.y - mu) * rstd, ga.y, be.y);
-                            v.z = fmaf((v.z - mu) * rstd, ga.z, be.z);
-                            v.w = fmaf((v.w - mu) * rstd, ga.w, be.w);
-                        }
-                        return v;
-                    };
-                    const int begin = live ? first : kn;
+                    const T *row = static_cast<const T *>(a.x) + (size_t)(live ? m : 0) * K;
                     if (NP == 1) {
-                        for (int k = begin; k < kn; k += step) {
-                            const float4 v = value(k0 + k);
+                        for (int k = live ? first : kn; k < kn; k += step) {
+                            const float4 v = load_4<VEC>(row, k0 + k, K);
                             uint2 o;
                             o.x = bits(__floats2half2_rn(v.x, v.y));
                             o.y = bits(__floats2half2_rn(v.z, v.w));
-                            *reinterpret_cast<uint2 *>(xs + m * stride + k) = o;
+                            *reinterpret_cast<uint2 *>(xs + m * stride + 2 * k) = o;
                         }
-                    } else {
-                        float4 held[kHeld];
-                        float peak = 0.0f;
-                        auto larger = [&](const float4 &v) {
-                            peak = fmaxf(fmaxf(peak, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                        };
-#pragma unroll
-                        for (int i = 0; i < kHeld; ++i) {
-                            held[i] = value(k0 + first + i * step);
-                            if (first + i * step < kn) larger(held[i]);
-                        }
-                        for (int k = begin + kHeld * step; k < kn; k += step) larger(value(k0 + k));
-                        peak = row_reduce<true>(peak, scratch, w0, wpr);
-                        const int e = max(-126, min(126, (int)(__float_as_uint(peak) >> 23) - 127));
-                        const float down = __uint_as_float((unsigned)(127 - e) << 23);
-                        if (live && first == 0) up_s[m] = __uint_as_float((unsigned)(127 + e) << 23);
-                        auto put = [&](const float4 &v, int k) {
-                            const float x0 = v.x * down, x1 = v.y * down, x2 = v.z * down, x3 = v.w * down;
-                            const __half2 a0 = __floats2half2_rn(x0, x1), a1 = __floats2half2_rn(x2, x3);
-                            const float2 b0 = __half22float2(a0), b1 = __half22float2(a1);
-                            uint2 hi, lo;
-                            hi.x = bits(a0);
-                            hi.y = bits(a1);
-                            lo.x = bits(__floats2half2_rn((x0 - b0.x) * kLoScale, (x1 - b0.y) * kLoScale));
-                            lo.y = bits(__floats2half2_rn((x2 - b1.x) * kLoScale, (x3 - b1.y) * kLoScale));
-                            *reinterpret_cast<uint2 *>(xs + 2 * m * stride + k) = hi;
-                            *reinterpret_cast<uint2 *>(xs + (2 * m + 1) * stride + k) = lo;
-                        };
-#pragma unroll
-                        for (int i = 0; i < kHeld; ++i)
-                            if (live && first + i * step < kn) put(held[i], first + i * step);
-                        for (int k = begin + kHeld * step; k < kn; k += step) put(value(k0 + k), k);
+                        continue;
                     }
+                    // groups past the slice are skipped by whole warps; few rows have registers for LayerNorm's weights too
+                    float4 held[kHeld], ga[INT ? kHeld : 1], be[INT ? kHeld : 1];
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i)
+                        if (i * step < kn) {
+                            const int k = min(k0 + first + i * step, K);
+                            held[i] = load_4<VEC>(row, k, K);
+                            if (INT && a.gamma) {
+                                ga[INT ? i : 0] = load_4<VEC>(a.gamma, k, K);
+                                be[INT ? i : 0] = load_4<VEC>(a.beta, k, K);
+                            }
+                        }
+                    float mu = 0.0f, rstd = 1.0f;
+                    if (a.gamma) {
+                        if (c0 == 0 && tile == tile0) {
+                            const bool in_regs = kn >= K && K <= kHeld * step;
+                            float s = 0.0f, q = 0.0f;
+                            if (in_regs) {
+#pragma unroll
+                                for (int i = 0; i < kHeld; ++i)
+                                    if (i * step < kn) s += (held[i].x + held[i].y) + (held[i].z + held[i].w);
+                            } else {
+#pragma unroll 4
+                                for (int k = first; k < K; k += step) {
+                                    const float4 v = load_4<VEC>(row, k, K);
+                                    s += (v.x + v.y) + (v.z + v.w);
+                                }
+                            }
+                            mu = row_sum(s, sums, w0, wpr) / K;
+                            auto square = [&](const float4 &v, int k) {
+                                const float d0 = v.x - mu, d1 = v.y - mu, d2 = v.z - mu, d3 = v.w - mu;
+                                if (VEC) {
+                                    if (k < K) q += fmaf(d0, d0, d1 * d1) + fmaf(d2, d2, d3 * d3);
+                                } else {
+                                    if (k < K) q = fmaf(d0, d0, q);
+                                    if (k + 1 < K) q = fmaf(d1, d1, q);
+                                    if (k + 2 < K) q = fmaf(d2, d2, q);
+                                    if (k + 3 < K) q = fmaf(d3, d3, q);
+                                }
+                            };
+                            if (in_regs) {
+#pragma unroll
+                                for (int i = 0; i < kHeld; ++i)
+                                    if (i * step < kn) square(held[i], first + i * step);
+                            } else {
+#pragma unroll 4
+                                for (int k = first; k < K; k += step) square(load_4<VEC>(row, k, K), k);
+                            }
+                            rstd = rsqrtf(row_sum(q, squares, w0, wpr) / K + 1e-5f);
+                            if (live && first == 0) row_stats[m] = make_float2(mu, rstd);
+                        } else {
+                            mu = row_stats[live ? m : 0].x;
+                            rstd = row_stats[live ? m : 0].y;
+                        }
+                    }
+                    auto norm = [&](const float4 &v, const float4 &gv, const float4 &bv) -> float4 {
+                        return make_float4(fmaf((v.x - mu) * rstd, gv.x, bv.x), fmaf((v.y - mu) * rstd, gv.y, bv.y),
+                                           fmaf((v.z - mu) * rstd, gv.z, bv.z), fmaf((v.w - mu) * rstd, gv.w, bv.w));
+                    };
+                    auto value = [&](int k) -> float4 {           // x'[m][k .. k + 3], 0 past K
+                        const float4 v = load_4<VEC>(row, k0 + k, K);
+                        return a.gamma ? norm(v, load_4<VEC>(a.gamma, k0 + k, K), load_4<VEC>(a.beta, k0 + k, K)) : v;
+                    };
+                    unsigned peak = 0;                            // as integers: NaN above infinity above finite
+                    auto larger = [&](const float4 &v) {
+                        auto mag = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
+                        peak = max(max(peak, max(mag(v.x), mag(v.y))), max(mag(v.z), mag(v.w)));
+                    };
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i)
+                        if (i * step < kn) {
+                            const int k = min(k0 + first + i * step, K);      // past K: 0 * 0 + 0
+                            if (a.gamma)
+                                held[i] = INT ? norm(held[i], ga[INT ? i : 0], be[INT ? i : 0])
+                                              : norm(held[i], load_4<VEC>(a.gamma, k, K), load_4<VEC>(a.beta, k, K));
+                            larger(held[i]);
+                        }
+#pragma unroll 4
+                    for (int k = first + kHeld * step; k < kn; k += step) larger(value(k));
+                    if (wpr > 1 && r0) __syncthreads();           // the last rows' peaks have been read
+                    peak = row_largest(peak, peaks, w0, wpr);
+                    // 2^e <= the largest < 2^(e + 1); INT: 29 bits below it, and the codes are 16 times theirs
+                    const int e = max(INT ? -96 : -126, min(126, (int)(peak >> 23) - 127)), bits_down = INT ? 29 : 0;
+                    const float down = __uint_as_float((unsigned)(127 + bits_down - e) << 23);
+                    if (live && first == 0)
+                        up_s[m] = INT && peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
+                                                             : __uint_as_float((unsigned)(127 + e) << 23) * (INT ? 0x1p-33f : 1.0f);
+                    auto put = [&](const float4 &v, int k) {
+                        const float x0 = v.x * down, x1 = v.y * down, x2 = v.z * down, x3 = v.w * down;
+                        if (INT) {
+                            // signed bytes: adding 128 to each of the lower three carries into the next
+                            auto digits = [](float x) { return ((unsigned)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u; };
+                            const unsigned q0 = digits(x0), q1 = digits(x1), q2 = digits(x2), q3 = digits(x3);
+                            const unsigned l01 = __byte_perm(q0, q2, 0x5140), l23 = __byte_perm(q1, q3, 0x5140);   // bytes 0 and 1 of both
+                            const unsigned h01 = __byte_perm(q0, q2, 0x7362), h23 = __byte_perm(q1, q3, 0x7362);   // bytes 2 and 3
+                            // rows k, k + 2, k + 1, k + 3, the most significant bytes first
+                            unsigned char *o = xs + 4 * m * stride + (k & ~63) + ((k >> 3) & 3) * 16 + ((k >> 5) & 1) * 8 + (k & 7);
+                            *reinterpret_cast<unsigned *>(o) = __byte_perm(h01, h23, 0x7632);
+                            *reinterpret_cast<unsigned *>(o + stride) = __byte_perm(h01, h23, 0x5410);
+                            *reinterpret_cast<unsigned *>(o + 2 * stride) = __byte_perm(l01, l23, 0x7632);
+                            *reinterpret_cast<unsigned *>(o + 3 * stride) = __byte_perm(l01, l23, 0x5410);
+                            return;
+                        }
+                        const __half2 a0 = __floats2half2_rn(x0, x1), a1 = __floats2half2_rn(x2, x3);
+                        const float2 b0 = __half22float2(a0), b1 = __half22float2(a1);
+                        uint2 hi, lo;
+                        hi.x = bits(a0);
+                        hi.y = bits(a1);
+                        lo.x = bits(__floats2half2_rn((x0 - b0.x) * kLoScale, (x1 - b0.y) * kLoScale));
+                        lo.y = bits(__floats2half2_rn((x2 - b1.x) * kLoScale, (x3 - b1.y) * kLoScale));
+                        *reinterpret_cast<uint2 *>(xs + 2 * m * stride + 2 * k) = hi;
+                        *reinterpret_cast<uint2 *>(xs + (2 * m + 1) * stride + 2 * k) = lo;
+                    };
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i)
+                        if (i * step < kn && live && first + i * step < kn) put(held[i], first + i * step);
+#pragma unroll 4
+                    for (int k = live ? first + kHeld * step : kn; k < kn; k += step) put(value(k), k);
                 }
+            }
+            if (tid < R) {                                        // the warps that have units of each tile
+                const int W = min(kQ4Warps, U);                   // unit u is warp ((u + 1) W - 1) / U's
+                range_s[tid][0] = (unsigned char)(((tid * nc + 1) * W - 1) / U);
+                range_s[tid][1] = (unsigned char)(((tid + 1) * nc * W - 1) / U);
             }
             cp_wait<S - 1>();                                     // x, where it was copied
             __syncthreads();
 
             // ---- the warp's units
-            float tot[TP][NT][4];
+            constexpr int kTot = INT ? 2 : 4;
+            float tot[TP][NT][kTot];
 #pragma unroll
             for (int x = 0; x < TP; ++x)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) tot[x][n][0] = tot[x][n][1] = tot[x][n][2] = tot[x][n][3] = 0.0f;
-            int r = u0 / nc, c = nc - u0 % nc;                    // tile, chunks left of it
-            const __half *xk = xs + g * stride + t * 8 + u0 % nc * kChunk;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < kTot; ++i) tot[x][n][i] = 0.0f;
+            int r = r_first, c = nc - c_first;                    // tile, chunks left of it
+            constexpr int kStep = INT ? kChunk : 2 * kChunk;      // bytes of a column in a chunk
+            const unsigned char *xk = xs + g * stride + t * 16 + c_first * kStep;
             const unsigned char *slot = ring;
             for (int u = u0; u < u1; ++u) {
                 cp_wait<S - 2>();
                 __syncwarp();
                 issue();
-                uint4 b[NT][2];
+                uint4 xv[NT][INT ? 1 : 2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        b[n][half] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride + half * 32);
+                    for (int half = 0; half < (INT ? 1 : 2); ++half)
+                        xv[n][half] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride + half * 64);
 #pragma unroll
                 for (int x = 0; x < TP; ++x) {
                     const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
@@ -448,93 +520,119 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     unsigned sc[PC];
 #pragma unroll
                     for (int i = 0; i < PC; ++i) sc[i] = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + i * 32 + g * 4);
-                    float acc[NT][4];
+                    if constexpr (INT) {
+                        int acc[NT][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (i == 0 || (PC == 2 && i == 2))
+                        for (int i = 0; i < 2; ++i) {
+                            if (i == 0 || PC == 2)
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-                        unsigned f[4];
-                        codes_to_half(words[i], f);
+                                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+                            const unsigned u0 = words[2 * i], u1 = words[2 * i + 1];
+                            const unsigned f[4] = {u0 & 0xf0f0f0f0u, (u0 << 4) & 0xf0f0f0f0u, u1 & 0xf0f0f0f0u, (u1 << 4) & 0xf0f0f0f0u};
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 &v = b[n][i >> 1];
-                            mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
+                            for (int n = 0; n < NT; ++n) mma16832(acc[n], f, i ? xv[n][0].z : xv[n][0].x, i ? xv[n][0].w : xv[n][0].y);
+                            if (i == 1 || PC == 2) {              // the group's sums of two neighbouring bytes, below 2^29
+                                const unsigned s = sc[PC == 2 ? i : 0];
+                                const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    tot[x][n][0] = fmaf((float)(acc[n][0] * 256 + acc[n][1]), lo, tot[x][n][0]);
+                                    tot[x][n][1] = fmaf((float)(acc[n][2] * 256 + acc[n][3]), hi, tot[x][n][1]);
+                                }
+                            }
                         }
-                        if (i == 3 || (PC == 2 && i == 1)) {      // the group's sum, scaled
-                            const unsigned s = sc[PC == 2 ? i >> 1 : 0];
-                            const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+                    } else {
+                        float acc[NT][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (i == 0 || (PC == 2 && i == 2))
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+                            unsigned f[4];
+                            codes_to_half(words[i], f);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                tot[x][n][0] = fmaf(acc[n][0], lo, tot[x][n][0]);
-                                tot[x][n][1] = fmaf(acc[n][1], lo, tot[x][n][1]);
-                                tot[x][n][2] = fmaf(acc[n][2], hi, tot[x][n][2]);
-                                tot[x][n][3] = fmaf(acc[n][3], hi, tot[x][n][3]);
+                                const uint4 &v = xv[n][INT ? 0 : i >> 1];
+                                mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
+                            }
+                            if (i == 3 || (PC == 2 && i == 1)) {  // the group's sum, scaled
+                                const unsigned s = sc[PC == 2 ? i >> 1 : 0];
+                                const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    tot[x][n][0] = fmaf(acc[n][0], lo, tot[x][n][0]);
+                                    tot[x][n][1] = fmaf(acc[n][1], lo, tot[x][n][1]);
+                                    tot[x][n][2] = fmaf(acc[n][2], hi, tot[x][n][2]);
+                                    tot[x][n][3] = fmaf(acc[n][3], hi, tot[x][n][3]);
+                                }
                             }
                         }
                     }
                 }
                 slot = slot + TP * CB == ring + S * TP * CB ? ring : slot + TP * CB;
-                xk += kChunk;
+                xk += kStep;
                 if (--c == 0 || u == u1 - 1) {                    // (this warp's part of) a tile is done
                     float *o = pieces + (size_t)(r + warp) * M * 16 * TP + g;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int x = 0; x < TP; ++x) {
-                            float (&v)[4] = tot[x][n];
-                            if (NP == 2) {
+                            float (&v)[kTot] = tot[x][n];
+                            if (INT) {                            // columns 2t, 2t + 1: the upper or the lower half of row t / 2
+                                const float lo = __shfl_down_sync(0xffffffffu, v[0], 1), hi = __shfl_down_sync(0xffffffffu, v[1], 1);
+                                const int m = n * 2 + (t >> 1);
+                                if (m < M && !(t & 1)) {
+                                    o[m * 16 * TP + x * 16] = fmaf(v[0], 65536.0f, lo);
+                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[1], 65536.0f, hi);
+                                }
+                            } else if (NP == 2) {
                                 const int m = n * 4 + t;
                                 if (m < M) {
                                     o[m * 16 * TP + x * 16] = fmaf(v[1], kLoUnscale, v[0]);
-                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[3], kLoUnscale, v[2]);
+                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[3 % kTot], kLoUnscale, v[2 % kTot]);
                                 }
                             } else {
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
+                                for (int i = 0; i < kTot; ++i) {
                                     const int m = n * 8 + 2 * t + (i & 1);
                                     if (m < M) o[m * 16 * TP + x * 16 + (i >> 1) * 8] = v[i];
                                 }
                             }
-                            v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < kTot; ++i) v[i] = 0.0f;
                         }
                     c = nc;
-                    xk -= nc * kChunk;
+                    xk -= nc * kStep;
                     ++r;
                 }
             }
             cp_wait<0>();
-            if (tid < R) {                                        // the warps that have units of each tile
-                range_s[tid][0] = (unsigned char)(((tid * nc + 1) * W - 1) / U);
-                range_s[tid][1] = (unsigned char)(((tid + 1) * nc * W - 1) / U);
-            }
             __syncthreads();
 
             // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
-            const int span = R * 16 * TP, together = max(1, kQ4Threads / span);   // rows of y taken at once
-            const int i0 = together == 1 ? tid : tid < together * span ? tid % span : span;
-            for (int m = together == 1 ? 0 : tid / span; m < M; m += together)
-                for (int i = i0; i < span; i += together == 1 ? kQ4Threads : span) {
-                    const int f = i % (16 * TP), rr = i / (16 * TP), o = m * span + i, n = (tile + rr) * 16 * TP + f;
-                    float v = 0.0f;
-                    for (int x = range_s[rr][0]; x <= range_s[rr][1]; ++x) v += pieces[((rr + x) * M + m) * 16 * TP + f];
-                    if (NP == 2) v *= up_s[m];
-                    if (c0 > 0) v += total[o];
-                    if (c0 + nc < sh.chunks) {
-                        total[o] = v;
-                    } else if (n < sh.N) {
-                        if (a.bias) v += a.bias[n];
-                        if (a.gelu) v = gelu_f(v);
-                        const size_t at = (size_t)m * sh.N + n;
-                        if (a.f16) {
-                            if (a.residual) v += __half2float(static_cast<const __half *>(a.residual)[at]);
-                            static_cast<__half *>(a.y)[at] = __float2half_rn(v);
-                        } else {
-                            if (a.residual) v += static_cast<const float *>(a.residual)[at];
-                            static_cast<float *>(a.y)[at] = v;
-                        }
-                    }
+            constexpr int kPer = 2 / TP;                          // (row, tile) pairs of a warp: 32 features of one, 16 of two
+            const int f = lane % (16 * TP);
+            int m = 0, rr = warp * kPer + lane / (16 * TP);
+            for (;; rr += kQ4Warps * kPer) {
+                for (; rr >= R && m < M; rr -= R) ++m;
+                if (m >= M) break;
+                const int o = (m * R + rr) * 16 * TP + f, n = (tile + rr) * 16 * TP + f;
+                const size_t at = (size_t)m * sh.N + n;
+                const bool last = c0 + nc == sh.chunks, there = last && n < sh.N;
+                const float bias = there && a.bias ? a.bias[n] : 0.0f;
+                const float res = there && a.residual ? tof(static_cast<const T *>(a.residual)[at]) : 0.0f;
+                float v = 0.0f;
+                for (int x = range_s[rr][0]; x <= range_s[rr][1]; ++x) v += pieces[((rr + x) * M + m) * 16 * TP + f];
+                if (NP > 1) v *= up_s[m];
+                if (c0 > 0) v += total[o];
+                if (!last) total[o] = v;
+                if (there) {
+                    v += bias;
+                    if (a.gelu) v = gelu_f(v);
+                    if (a.residual) v += res;
+                    static_cast<T *>(a.y)[at] = fromf<T>(v);
                 }
+            }
             __syncthreads();
         }
     }
@@ -547,31 +645,46 @@ int q4_sms() {
     return n;
 }
 
-template <int NT, int TP, int NP, int PC>
+template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
-    auto kernel = q4_matvec_kernel<NT, TP, NP, PC>;
+    auto kernel = q4_matvec_kernel<T, VEC, NT, TP, NP, PC>;
     const int ntiles = sh.tiles / TP, grid = std::min(q4_sms(), ntiles);
+    a.share = ntiles / grid;
+    a.extra = ntiles % grid;
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
     // x in equal slices that fit beside the ring and the sums
-    const size_t ring = (size_t)kQ4Warps * Q4Ring<TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)a.M * 16 * TP * 4;
+    const size_t ring = (size_t)kQ4Warps * Q4Ring<NT, TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)a.M * 16 * TP * 4;
     size_t sums = (a.most + kQ4Warps) * tile;
-    int fit = (int)((kQ4Smem - ring - sums) / (8 * NT * 2) - 32) / kChunk;
-    if (fit < sh.chunks) {
+    auto bytes = [&](int slice) { return ring + (size_t)8 * NT * x_stride<NP>(slice) + sums; };
+    a.slice = sh.chunks;
+    if (bytes(a.slice) > kQ4Smem) {
         sums += a.most * tile;
-        fit = (int)((kQ4Smem - ring - sums) / (8 * NT * 2) - 32) / kChunk;
+        int slices = 2;
+        while (bytes((sh.chunks + slices - 1) / slices) > kQ4Smem) ++slices;   // ends: one chunk fits
+        a.slice = (sh.chunks + slices - 1) / slices;
     }
-    const int slices = (sh.chunks + fit - 1) / fit;
-    a.slice = (sh.chunks + slices - 1) / slices;
-    const size_t smem = ring + (size_t)8 * NT * (a.slice * kChunk + 32) * 2 + sums;
+    const size_t smem = bytes(a.slice);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
     kernel<<<grid, kQ4Threads, smem, st>>>(a, sh);
     return launch_status("g2k_matvec_q4");
 }
 
-template <int NT, int TP, int NP>
+template <typename T, bool VEC, int NT, int TP, int NP>
 int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
-    return sh.per_chunk == 2 ? launch_q4<NT, TP, NP, 2>(a, sh, st) : launch_q4<NT, TP, NP, 1>(a, sh, st);
+    return sh.per_chunk == 2 ? launch_q4<T, VEC, NT, TP, NP, 2>(a, sh, st) : launch_q4<T, VEC, NT, TP, NP, 1>(a, sh, st);
+}
+
+template <typename T, bool VEC>
+int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
+    // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
+    // matrices of fewer pairs than SMs (and few rows) are better spread one by one.
+    const bool one = sh.tiles / 2 < q4_sms();
+    if (a.M <= 2) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
+    if (a.M <= 4) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
+    if constexpr (sizeof(T) == 2)
+        if (!a.gamma) return a.M <= 8 ? launch_q4<T, VEC, 1, 2, 1>(a, sh, st) : launch_q4<T, VEC, 2, 2, 1>(a, sh, st);
+    return a.M <= 8 ? launch_q4<T, VEC, 2, 2, 2>(a, sh, st) : launch_q4<T, VEC, 4, 2, 2>(a, sh, st);
 }
 
 bool bad_shape(int N, int K, int group) {
@@ -646,13 +759,8 @@ extern "C" int g2k_matvec_q4(const void *x, const void *packed, const float *bia
     const Q4Shape sh(N, K, group);
     const bool vec = K % 4 == 0 && aligned(x, 4 * es) && aligned(ln_gamma, 16) && aligned(ln_beta, 16);
     const Q4Args a{x, static_cast<const unsigned char *>(packed), bias, ln_gamma, ln_beta, residual, y, M, apply_gelu,
-                   dtype == G2_F16, vec, K % 8 == 0 && !ln_gamma && aligned(x, 16), 0, 0};
+                   dtype == G2_F16 && K % 8 == 0 && !ln_gamma && aligned(x, 16), 0, 0, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
-    // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
-    // matrices of fewer pairs than SMs (and one n tile) are better spread one by one.
-    const bool one = sh.tiles / 2 < q4_sms();
-    if (dtype == G2_F16 && !ln_gamma)
-        return M > 8 ? launch_q4<2, 2, 1>(a, sh, st) : one ? launch_q4<1, 1, 1>(a, sh, st) : launch_q4<1, 2, 1>(a, sh, st);
-    return M > 8 ? launch_q4<4, 2, 2>(a, sh, st) : M > 4 ? launch_q4<2, 2, 2>(a, sh, st)
-         : one ? launch_q4<1, 1, 2>(a, sh, st) : launch_q4<1, 2, 2>(a, sh, st);
+    if (dtype == G2_F32) return vec ? launch_q4<float, true>(a, sh, st) : launch_q4<float, false>(a, sh, st);
+    return vec ? launch_q4<__half, true>(a, sh, st) : launch_q4<__half, false>(a, sh, st);
 }
