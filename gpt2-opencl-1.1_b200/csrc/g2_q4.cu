@@ -144,11 +144,11 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 //   NP = 4  int8: x as a 30-bit fixed-point number below a power of two over the
 //           row's largest, one column for each of its bytes.  Codes times bytes are
 //           summed exactly in int32, and unpacking eight codes costs three
-//           instructions.  Up to 4 rows.
+//           instructions.  Up to 4 rows (2 of fp16).
 //   NP = 2  fp16: the rounding of x (after a power of two has brought the row's
 //           largest below 2) and 2^11 times the rest, 22 bits in all.  Eight codes
 //           cost nine instructions.  More than 4 rows.
-//   NP = 1  fp16 x as it is.  More than 4 rows.
+//   NP = 1  fp16 x as it is.  More than 2 rows.
 // A group's sum is scaled once, in fp32.
 //
 // The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
@@ -680,10 +680,12 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
     // matrices of fewer pairs than SMs (and few rows) are better spread one by one.
     const bool one = sh.tiles / 2 < q4_sms();
+    if constexpr (sizeof(T) == 2)
+        if (!a.gamma && a.M > 2 && a.M <= 8) return one ? launch_q4<T, VEC, 1, 1, 1>(a, sh, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, st);
     if (a.M <= 2) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
     if (a.M <= 4) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
     if constexpr (sizeof(T) == 2)
-        if (!a.gamma) return a.M <= 8 ? launch_q4<T, VEC, 1, 2, 1>(a, sh, st) : launch_q4<T, VEC, 2, 2, 1>(a, sh, st);
+        if (!a.gamma && a.M > 8) return launch_q4<T, VEC, 2, 2, 1>(a, sh, st);
     return a.M <= 8 ? launch_q4<T, VEC, 2, 2, 2>(a, sh, st) : launch_q4<T, VEC, 4, 2, 2>(a, sh, st);
 }
 
