@@ -338,7 +338,7 @@ __device__ __forceinline__ void group_sync(int group) {
 // Units of sequence s (0 where it has no rows or is out of range).
 struct SeqWork {
     int first, n, len, units, col_groups;
-    long long total;
+    unsigned total;
 };
 template <int COLS>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
@@ -355,7 +355,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
     }
     w.units = max(1, (w.len + a.unit - 1) / a.unit);   // a row that sees nothing is still written
     w.col_groups = (w.n * a.group + COLS - 1) / COLS;
-    w.total = (long long)w.units * w.col_groups * a.c.n_kv_head;
+    w.total = (unsigned)w.units * w.col_groups * a.c.n_kv_head;   // below 2^31 over all sequences: checked on the host
     return w;
 }
 
@@ -365,47 +365,66 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
     constexpr int PART = COLS * (D + 2);
     static_assert(WPR * PART * 4 <= WPR * S * TILE, "the merge buffer lies in the ring");
     extern __shared__ __align__(128) unsigned char ring[];
-    __shared__ long long prefix[kAttnWarps * 32 + 1];
-    __shared__ long long warp_sum[kAttnWarps];
+    __shared__ unsigned prefix[kAttnWarps * 32];
+    __shared__ unsigned warp_sum[kAttnWarps];
     __shared__ int arrived[GROUPS];
+    __shared__ SeqWork cached[kAttnWarps * 32];   // of the first sequences
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int grp = warp / WPR, wr = warp % WPR, gt = tid - grp * 32 * WPR;
     const int H = a.c.n_kv_head, P = a.c.page_size, n_seq = a.r.n_seq;
 
     // ---- the units before every `per` sequences
     const int per = (n_seq + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
-    long long mine = 0;
-    for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) mine += seq_work<COLS>(a, s).total;
-    long long sum = mine;
+    unsigned mine = 0;
+    if (per == 1) {
+        if (tid < n_seq) {
+            cached[tid] = seq_work<COLS>(a, tid);
+            mine = cached[tid].total;
+        }
+    } else {
+        for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) mine += seq_work<COLS>(a, s).total;
+    }
+    unsigned sum = mine;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+        const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += x;
     }
     if (lane == 31) warp_sum[warp] = sum;
     __syncthreads();
-    long long before = 0;
-    for (int i = 0; i < warp; ++i) before += warp_sum[i];
-    prefix[tid] = before + sum - mine;
-    if (tid == kAttnWarps * 32 - 1) prefix[kAttnWarps * 32] = before + sum;
-    __syncthreads();
-    const long long total = prefix[kAttnWarps * 32];
-    const long long W = min((long long)a.workers, total);
-    const int worker = blockIdx.x * GROUPS + grp;
-    if (worker >= W) return;   // whole groups leave; later barriers are the groups' own
-    long long u = worker * total / W;
-    const long long u_end = (worker + 1) * total / W;
-    auto worker_of = [&](long long unit) { return (int)(((unit + 1) * W - 1) / total); };
-
-    // ---- the share's first sequence
-    int lo = 0, hi = kAttnWarps * 32 - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (prefix[mid] <= u) lo = mid;
-        else hi = mid - 1;
+    unsigned before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < kAttnWarps; ++i) {
+        const unsigned x = warp_sum[i];
+        before += i < warp ? x : 0;
+        total += x;
     }
-    int s = lo * per;
-    long long seq_begin = prefix[lo];
-    SeqWork sw = seq_work<COLS>(a, s);
+    prefix[tid] = before + sum - mine;
+    __syncthreads();
+    const unsigned W = min((unsigned)a.workers, total);
+    const unsigned worker = blockIdx.x * GROUPS + grp;
+    if (worker >= W) return;   // whole groups leave; later barriers are the groups' own
+    const unsigned share = total / W, extra = total - share * W;   // the first `extra` workers have one unit more
+    auto share_begin = [&](unsigned w) { return w * share + min(w, extra); };
+    auto worker_of = [&](unsigned unit) {
+        const unsigned in_long = extra * (share + 1);
+        return unit < in_long ? unit / (share + 1) : extra + (unit - in_long) / share;
+    };
+    unsigned u = share_begin(worker);
+    const unsigned u_end = share_begin(worker + 1);
+    auto work_of = [&](int s) { return per == 1 ? cached[s] : seq_work<COLS>(a, s); };
+
+    // ---- the share's first sequence: the last whose units begin at or before u
+    int s;
+    unsigned seq_begin;
+    {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kAttnWarps; ++i) n += __popc(__ballot_sync(0xffffffffu, prefix[i * 32 + lane] <= u));
+        s = (n - 1) * per;
+        seq_begin = prefix[n - 1];
+    }
+    SeqWork sw = work_of(s);
     bool first_piece = true;
 
     unsigned char *slots = ring + warp * S * TILE;
@@ -423,13 +442,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
     while (u < u_end) {
         while (u >= seq_begin + sw.total) {   // only past sequences without units or the end of one
             seq_begin += sw.total;
-            sw = seq_work<COLS>(a, ++s);
+            sw = work_of(++s);
         }
-        const long long rem = u - seq_begin;
-        const int run = (int)(rem / sw.units), unit0 = (int)(rem % sw.units);
+        const unsigned rem = u - seq_begin;
+        const int run = (int)(rem / (unsigned)sw.units), unit0 = (int)rem - run * sw.units;
         const int h = run / sw.col_groups, col0 = run % sw.col_groups * COLS;
-        const int n_units = (int)min((long long)(sw.units - unit0), u_end - u);
-        const long long run_begin = u - unit0;
+        const int n_units = (int)min((unsigned)(sw.units - unit0), u_end - u);
+        const unsigned run_begin = u - unit0;
         const int cols = min(COLS, sw.n * a.group - col0);
         // key limits of the columns; `lim` of this thread's (column t of each n tile)
         const int lim_first = sw.len - sw.n + col0 / a.group + 1, lim_last = sw.len - sw.n + (col0 + cols - 1) / a.group + 1;
@@ -661,12 +680,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
         group_sync<WPR>(grp);
 
         const bool whole = n_units == sw.units;
-        const int w0 = worker_of(run_begin), w1 = worker_of(run_begin + sw.units - 1);
-        float *part = a.parts + ((long long)worker * 2 + (first_piece ? 0 : 1)) * PART;
-        auto store = [&](int c, int d, float v) {
-            const int col = col0 + c;
-            const long long o = (long long)(sw.first + col / a.group) * a.out_stride +
-                                (long long)(h * a.group + col % a.group) * D + d;
+        float *part = a.parts + ((size_t)worker * 2 + (first_piece ? 0 : 1)) * PART;
+        auto store = [&](int i, float v) {
+            const int c = i / D, d = i % D, col = col0 + c, row = col / a.group;
+            const long long o = (long long)(sw.first + row) * a.out_stride + (long long)(h * a.group + col - row * a.group) * D + d;
             if (a.f16) static_cast<__half *>(a.out)[o] = __float2half_rn(v);
             else static_cast<float *>(a.out)[o] = v;
         };
@@ -682,7 +699,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
                 sum_o = fmaf(merge[x * PART + c * D + d], fix, sum_o);
             }
             if (whole) {
-                store(c, d, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
+                store(i, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
             } else {
                 part[i] = sum_o;
                 if (d == 0) {
@@ -692,30 +709,44 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
             }
         }
         if (!whole) {
-            __threadfence();
+            const unsigned w0 = worker_of(run_begin), w1 = worker_of(run_begin + sw.units - 1);
             group_sync<WPR>(grp);
-            if (gt == 0) arrived[grp] = (int)atomicAdd(&a.counters[w0], 1u);
+            if (gt == 0) {   // releases the group's results and acquires the others'
+                unsigned seen;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(seen) : "l"(a.counters + w0) : "memory");
+                arrived[grp] = (int)seen;
+            }
             group_sync<WPR>(grp);
-            if (arrived[grp] == w1 - w0) {   // every other piece is there
-                __threadfence();
+            if (arrived[grp] == (int)(w1 - w0)) {   // every other piece is there
                 if (gt == 0) a.counters[w0] = 0;
                 // piece of worker x: its first one, or, where the run begins inside the share, its last
-                auto piece = [&](int x) {
-                    const bool later = x == w0 && run_begin > x * total / W;
-                    return a.parts + ((long long)x * 2 + (later ? 1 : 0)) * PART;
-                };
+                const float *piece0 = a.parts + ((size_t)w0 * 2 + (run_begin > share_begin(w0) ? 1 : 0)) * PART;
+                const float *pieces = a.parts + (size_t)w0 * 2 * PART;
+                const int n = (int)(w1 - w0) + 1;
                 for (int i = gt; i < cols * D; i += 32 * WPR) {
-                    const int c = i / D, d = i % D;
+                    const int c = i / D;
                     float m = kNoMax, sum_w = 0.0f, sum_o = 0.0f;
-                    for (int x = w0; x <= w1; ++x) {
-                        const float *p = piece(x);
-                        const float pm = __ldcg(p + COLS * D + c), nm = fmaxf(m, pm);
-                        const float f0 = exp2_fast(m - nm), f1 = exp2_fast(pm - nm);
-                        sum_w = sum_w * f0 + __ldcg(p + COLS * (D + 1) + c) * f1;
-                        sum_o = sum_o * f0 + __ldcg(p + i) * f1;
+                    for (int x = 0; x < n; x += 4) {   // four pieces' loads at a time; in order
+                        float pm[4], pw[4], po[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float *p = x + y == 0 ? piece0 : pieces + (size_t)(x + y) * 2 * PART;
+                            pm[y] = x + y < n ? __ldcg(p + COLS * D + c) : kNoMax;
+                            pw[y] = x + y < n ? __ldcg(p + COLS * (D + 1) + c) : 0.0f;
+                            po[y] = x + y < n ? __ldcg(p + i) : 0.0f;
+                        }
+                        const float nm = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), f = exp2_fast(m - nm);
                         m = nm;
+                        sum_w *= f;
+                        sum_o *= f;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float fix = exp2_fast(pm[y] - nm);
+                            sum_w = fmaf(pw[y], fix, sum_w);
+                            sum_o = fmaf(po[y], fix, sum_o);
+                        }
                     }
-                    store(c, d, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
+                    store(i, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
                 }
             }
         }
@@ -905,6 +936,12 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, n_head, q, out, dtype, &q_stride, &out_stride, r, seq_len))) return rc;
     if ((long long)max_q * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
+    {   // the kernel counts units in 32 bits
+        const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, 1);
+        const double units = ((double)table_stride * cache->page_size / p.unit + 1) * n_seq * cache->n_kv_head *
+                             ((double)max_q * (n_head / cache->n_kv_head) / (4 * p.nt) + 1);
+        if (units > 2147483647.0) return arg_error(G2_ERR_RANGE, who, "too much work for one call");
+    }
     if (!workspace || !aligned(workspace, 256)) return arg_error(G2_ERR_ARG, who, "workspace not 256-byte aligned");
     if (workspace_bytes < g2k_kv8_attention_workspace(cache, n_head, n_seq, max_q))
         return arg_error(G2_ERR_ARG, who, "workspace too small");
