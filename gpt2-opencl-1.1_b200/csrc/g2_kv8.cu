@@ -34,8 +34,9 @@ __device__ __forceinline__ void bad(const Rows8 &r) {
 __device__ __forceinline__ Span seq_rows(const Rows8 &r, int s) {
     Span p{s, 1};
     if (r.q_start) {
+        const int next = r.q_start[s + 1];
         p.first = r.q_start[s];
-        const long long n = (long long)r.q_start[s + 1] - p.first;
+        const long long n = (long long)next - p.first;
         if (n < 0 || n > r.max_q || p.first < 0 || p.first + n > r.n_rows) {
             bad(r);
             return Span{0, 0};
@@ -230,17 +231,19 @@ __global__ void __launch_bounds__(256)
 // A warp takes tiles of 16 keys.  Each tile's codes and scales are copied by
 // cp.async into the warp's own ring of kStages slots, so that the copies of the
 // next tiles are always in flight and no barrier is needed beyond the warp.
-// Both products run on the tensor cores (m16n8k16, fp16 operands, fp32 sums):
+// Both products run on the tensor cores:
 //   scores   keys on m, query columns on n;
 //   outputs  dimensions on m, query columns on n, keys on k.
-// 8-bit codes are exact in fp16.  Each query and each weight takes two columns,
-// its fp16 rounding and 2^11 times the rest (22 bits together), which fill
-// columns that a few queries leave idle.  Both lie in the same thread, so
-// neither product needs a shuffle, and `movmatrix` turns the weights into the
-// second product's operand.  Operand orders are permuted (dimensions of the
-// scores' k, of the outputs' m) so that every thread reads 8 or 16 consecutive
-// bytes; the ring's slots are swizzled so that those reads have no bank
-// conflicts.
+// Eight columns are more than a few queries fill, so each query takes several.
+// int8 keys meet the four bytes of a fixed-point q (30 bits below a power of two
+// over its largest) in m16n8k32 products, exactly and without any conversion of
+// the keys.  e4m3 keys, and the values of both formats, become fp16 exactly and
+// meet two fp16 columns, the rounding of q or of a weight and 2^11 times the rest
+// (22 bits).  All columns of a query lie in the same threads, so neither product
+// needs a shuffle; `movmatrix` turns the weights into the second one's operand.
+// Operand orders are permuted (dimensions of the scores' k, of the outputs' m) so
+// that every thread reads 8 or 16 consecutive bytes; the ring's slots are swizzled
+// so that those reads have no bank conflicts.
 //
 // The running reference m is raised only when a score exceeds it by 2^8: one
 // vote a tile in place of a maximum over the warp.
@@ -249,11 +252,12 @@ constexpr int kMaxWorkers = 4096;   // counters at the start of the workspace
 constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
 constexpr float kNoMax = -1e30f;    // reference of a column that has seen no key
 
-template <int D>
+template <int D, int NT>
 struct AttnRing {
-    static constexpr int kStages = D == 64 ? 6 : 3;
-    static constexpr int kTileBytes = 32 * D;   // 16 keys' K and V codes
-    static constexpr int kSmem = kAttnWarps * kStages * (kTileBytes + 16);
+    static constexpr int kBlocks = D * NT >= 256 ? 1 : 2;   // CTAs per SM; wide column groups need the registers of two
+    static constexpr int kStages = (D == 64 ? 6 : 3) * (kBlocks == 1 ? 2 : 1);
+    static constexpr int kTileBytes = 32 * D;               // 16 keys' K and V codes
+    static constexpr int kSmem = kAttnWarps * kStages * (kTileBytes + 8);
 };
 
 struct AttnArgs {
@@ -287,6 +291,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
     unsigned r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -295,6 +304,11 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float log2_fast(float x) {
@@ -327,6 +341,16 @@ __device__ __forceinline__ unsigned split_half(float v) {
     return *reinterpret_cast<const unsigned *>(&p);
 }
 
+// The same of two, sharing the conversions.
+__device__ __forceinline__ void split_half2(float v0, float v1, unsigned &s0, unsigned &s1) {
+    const __half2 h = __floats2half2_rn(v0, v1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(fmaf(f.x, -kLoScale, v0 * kLoScale), fmaf(f.y, -kLoScale, v1 * kLoScale));
+    const unsigned hb = *reinterpret_cast<const unsigned *>(&h), lb = *reinterpret_cast<const unsigned *>(&l);
+    s0 = __byte_perm(hb, lb, 0x5410);
+    s1 = __byte_perm(hb, lb, 0x7632);
+}
+
 template <int WPR>
 __device__ __forceinline__ void group_sync(int group) {
     if (WPR == 1)
@@ -343,11 +367,11 @@ struct SeqWork {
 template <int COLS>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
     SeqWork w{};
+    w.len = a.seq_len[s];   // requested beside the rows' numbers
     const Span sp = seq_rows(a.r, s);
     w.first = sp.first;
     w.n = sp.n;
     if (!sp.n) return w;
-    w.len = a.seq_len[s];
     if (w.len < 0 || w.len > (long long)a.r.table_stride * a.c.page_size) {
         bad(a.r);
         w.n = 0;
@@ -360,15 +384,19 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
 }
 
 template <int FMT, int D, int NT, int WPR>
-__global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnArgs a) {
-    constexpr int COLS = 4 * NT, KS = D / 16, S = AttnRing<D>::kStages, TILE = AttnRing<D>::kTileBytes, GROUPS = kAttnWarps / WPR;
+__global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) kv8_attention_kernel(AttnArgs a) {
+    constexpr int COLS = 4 * NT, KS = D / 16, S = AttnRing<D, NT>::kStages, TILE = AttnRing<D, NT>::kTileBytes, GROUPS = kAttnWarps / WPR;
     constexpr int PART = COLS * (D + 2);
+    constexpr bool INT = FMT == G2_KV_I8;
+    // slots of a group's first warp that are empty while its queries are staged there
+    constexpr int FREE = (NT * KS * 256 + TILE - 1) / TILE;
     static_assert(WPR * PART * 4 <= WPR * S * TILE, "the merge buffer lies in the ring");
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ unsigned prefix[kAttnWarps * 32];
     __shared__ unsigned warp_sum[kAttnWarps];
     __shared__ int arrived[GROUPS];
     __shared__ SeqWork cached[kAttnWarps * 32];   // of the first sequences
+    __shared__ float qfac_s[GROUPS][COLS];        // scores' factor of each query column
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int grp = warp / WPR, wr = warp % WPR, gt = tid - grp * 32 * WPR;
     const int H = a.c.n_kv_head, P = a.c.page_size, n_seq = a.r.n_seq;
@@ -428,9 +456,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
     bool first_piece = true;
 
     unsigned char *slots = ring + warp * S * TILE;
-    float *meta = reinterpret_cast<float *>(ring + kAttnWarps * S * TILE) + warp * S * 4;   // K scale, V scale, valid
+    float *meta = reinterpret_cast<float *>(ring + kAttnWarps * S * TILE) + warp * S * 2;   // K and V scale; -1: no page
     float *merge = reinterpret_cast<float *>(ring + grp * WPR * S * TILE);                  // [WPR][PART]
-    const unsigned slots_addr = smem_addr(slots), meta_addr = smem_addr(meta);
+    const unsigned slots_addr = smem_addr(slots), meta_addr = smem_addr(meta) + lane * 4;   // lanes 0 and 1 bring the scales
+    const unsigned char *k_lane = static_cast<const unsigned char *>(a.c.k) + lane * 16, *v_lane = static_cast<const unsigned char *>(a.c.v) + lane * 16;
+    const float *scale_lane = lane ? a.c.v_scale : a.c.k_scale;
 
     // this lane's places in a slot: where it copies to and reads from
     const int crow = lane / (D / 16), ccol = lane % (D / 16);
@@ -473,79 +503,102 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
             bad(a.r);
             return -1;
         };
-        int pages = load_pages(0), pages_next = load_pages(32);
-        auto issue = [&](int j) {
-            if (j < my_tiles) {
-                if (j && (j & 31) == 0) {
+        int pages = load_pages(0), pages_next = my_tiles > 32 ? load_pages(32) : -1;
+        int next = 0, key_next = kbeg + wr * 16, put = 0;   // the next tile to copy, its first key, its slot
+        auto issue = [&]() {
+            if (next < my_tiles) {
+                if (next && (next & 31) == 0) {
                     pages = pages_next;
-                    pages_next = load_pages(j + 32);
+                    pages_next = load_pages(next + 32);
                 }
-                const int key0 = kbeg + (j * WPR + wr) * 16;
-                const int page = __shfl_sync(0xffffffffu, pages, j & 31);
-                const long long at = (long long)max(page, 0) * H + h;
-                const long long off = (at * P + key0 % P) * D + lane * 16;
-                const unsigned char *ks = static_cast<const unsigned char *>(a.c.k) + off;
-                const unsigned char *vs = static_cast<const unsigned char *>(a.c.v) + off;
-                const unsigned slot = slots_addr + (j % S) * TILE;
-                const int rows = page >= 0 ? sw.len - key0 : 0;   // rows from here on are not the sequence's
+                const int page = __shfl_sync(0xffffffffu, pages, next & 31);
+                const unsigned at = (unsigned)max(page, 0) * H + h, row = at * P + (key_next & (P - 1));   // rows fit 32 bits: memory ends first
+                const unsigned char *ks = k_lane + (size_t)row * D, *vs = v_lane + (size_t)row * D;
+                const unsigned slot = slots_addr + put * TILE, m = meta_addr + put * 8;
+                const int rows = page >= 0 ? sw.len - key_next : 0;   // rows from here on are not the sequence's
+                if (rows >= 16) {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int bytes = crow + i * (512 / D) < rows ? 16 : 0;
-                    cp_async16(slot + k_put + i * 512, ks + i * 512, bytes);
-                    cp_async16(slot + (D == 64 ? v_put : v_put ^ ((i & 1) << 6)) + i * 512, vs + i * 512, bytes);
+                    for (int i = 0; i < D / 32; ++i) {
+                        cp_async16(slot + k_put + i * 512, ks + i * 512, 16);
+                        cp_async16(slot + (D == 64 ? v_put : v_put ^ ((i & 1) << 6)) + i * 512, vs + i * 512, 16);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const int bytes = crow + i * (512 / D) < rows ? 16 : 0;
+                        cp_async16(slot + k_put + i * 512, ks + i * 512, bytes);
+                        cp_async16(slot + (D == 64 ? v_put : v_put ^ ((i & 1) << 6)) + i * 512, vs + i * 512, bytes);
+                    }
                 }
-                const unsigned m = meta_addr + (j % S) * 16;
-                if (lane == 0) cp_async4(m, a.c.k_scale + at, 4);
-                if (lane == 1) cp_async4(m + 4, a.c.v_scale + at, 4);
-                if (lane == 2) meta[(j % S) * 4 + 2] = page >= 0 ? 1.0f : 0.0f;
+                if (lane < 2) {
+                    if (page >= 0) cp_async4(m, scale_lane + at, 4);
+                    else asm volatile("st.shared.f32 [%0], %1;" ::"r"(m), "f"(-1.0f) : "memory");
+                }
+                ++next;
+                key_next += 16 * WPR;
+                put = put + 1 == S ? 0 : put + 1;
             }
             cp_commit();
         };
-#pragma unroll
-        for (int j = 0; j < S - 1; ++j) issue(j);
+#pragma unroll 1
+        for (int j = 0; j < S - FREE; ++j) issue();
 
-        // ---- queries: column n of an n tile is part n & 1 of query n >> 1
+        // ---- queries, a warp each: into the order of the operands' registers.  Columns 2i and 2i + 1 are of
+        // query i; int8 keys have two n tiles, for the upper two and the lower two of the four bytes
+        unsigned *qs = reinterpret_cast<unsigned *>(ring + grp * WPR * S * TILE + (S - FREE) * TILE);   // [NT][KS][2][lane]
+        for (int c = wr; c < cols; c += WPR) {
+            const int col = col0 + c, row = col / a.group, d = lane * 4;
+            const long long o = (long long)(sw.first + row) * a.q_stride + (long long)(h * a.group + col - row * a.group) * D + d;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (d < D) x = a.f16 ? load4<__half>(static_cast<const __half *>(a.q) + o) : load4<float>(static_cast<const float *>(a.q) + o);
+            const unsigned peak = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
+            // a power of two below the largest (2^e <= it < 2^(e + 1)), so that no type's range matters
+            const int e = max(INT ? -96 : -126, min(126, (int)(peak >> 23) - 127));
+            const float down = __uint_as_float((unsigned)(127 + (INT ? 29 : 0) - e) << 23);
+            const float up = __uint_as_float((unsigned)(127 + e) << 23) * (INT ? 0x1p-29f : 1.0f);
+            if (lane == 0) qfac_s[grp][c] = (peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : up) * a.scale_log2e;
+            const int k = (d >> 6) * 4 + ((d >> 2) & 3);   // thread (d & 63) >> 4 of a quad has these four dimensions
+            unsigned *at = qs + ((c >> 2) * KS * 2) * 32 + (c & 3) * 8 + ((d & 63) >> 4);
+            if (d < D) {
+                if (INT) {
+                    // signed bytes: adding 128 to each of the lower three carries into the next
+                    auto digits = [&](float v) { return ((unsigned)__float2int_rn(v * down) + 0x00808080u) ^ 0x00808080u; };
+                    const unsigned y0 = digits(x.x), y1 = digits(x.y), y2 = digits(x.z), y3 = digits(x.w);
+                    const unsigned a01 = __byte_perm(y0, y1, 0x7362), a23 = __byte_perm(y2, y3, 0x7362);   // bytes 2 and 3
+                    const unsigned b01 = __byte_perm(y0, y1, 0x5140), b23 = __byte_perm(y2, y3, 0x5140);   // bytes 0 and 1
+                    at += ((k >> 1) * 2 + (k & 1)) * 32;
+                    at[0] = __byte_perm(a01, a23, 0x7632);
+                    at[4] = __byte_perm(a01, a23, 0x5410);
+                    at[KS * 32] = __byte_perm(b01, b23, 0x7632);
+                    at[KS * 32 + 4] = __byte_perm(b01, b23, 0x5410);
+                } else {
+                    const __half2 h0 = __floats2half2_rn(x.x * down, x.y * down), h1 = __floats2half2_rn(x.z * down, x.w * down);
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    const __half2 l0 = __floats2half2_rn((x.x * down - f0.x) * kLoScale, (x.y * down - f0.y) * kLoScale);
+                    const __half2 l1 = __floats2half2_rn((x.z * down - f1.x) * kLoScale, (x.w * down - f1.y) * kLoScale);
+                    at += k * 2 * 32;
+                    at[0] = *reinterpret_cast<const unsigned *>(&h0);
+                    at[4] = *reinterpret_cast<const unsigned *>(&l0);
+                    at[32] = *reinterpret_cast<const unsigned *>(&h1);
+                    at[36] = *reinterpret_cast<const unsigned *>(&l1);
+                }
+            }
+        }
+        group_sync<WPR>(grp);
         unsigned qf[NT][KS][2];
         float qfac[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int c = n * 4 + (g >> 1);
-            float x[D / 4];
+        for (int n = 0; n < NT; ++n) {   // columns past the last hold anything: they are not written
+            qfac[n] = n * 4 + t < cols ? qfac_s[grp][n * 4 + t] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
-            if (c < cols) {
-                const int col = col0 + c;
-                const long long o = (long long)(sw.first + col / a.group) * a.q_stride +
-                                    (long long)(h * a.group + col % a.group) * D + t * 16;
-#pragma unroll
-                for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 v = a.f16 ? load4<__half>(static_cast<const __half *>(a.q) + o + b * 64 + i * 4)
-                                               : load4<float>(static_cast<const float *>(a.q) + o + b * 64 + i * 4);
-                        x[b * 16 + i * 4] = v.x;
-                        x[b * 16 + i * 4 + 1] = v.y;
-                        x[b * 16 + i * 4 + 2] = v.z;
-                        x[b * 16 + i * 4 + 3] = v.w;
-                    }
+            for (int k = 0; k < KS; ++k) {
+                qf[n][k][0] = qs[((n * KS + k) * 2) * 32 + lane];
+                qf[n][k][1] = qs[((n * KS + k) * 2 + 1) * 32 + lane];
             }
-            unsigned peak = 0;
-#pragma unroll
-            for (int i = 0; i < D / 4; ++i) peak = max(peak, abs_bits(x[i]));
-            peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-            peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-            // a power of two that brings the largest below 2, so that fp16's range does not matter
-            const int e = max(-126, min(126, (int)(peak >> 23) - 127));
-            const float down = __uint_as_float((unsigned)(127 - e) << 23), up = __uint_as_float((unsigned)(127 + e) << 23);
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const unsigned p0 = split_half(x[k * 4 + b * 2] * down), p1 = split_half(x[k * 4 + b * 2 + 1] * down);
-                    qf[n][k][b] = __byte_perm(p0, p1, (g & 1) ? 0x7632 : 0x5410);
-                }
-            qfac[n] = __shfl_sync(0xffffffffu, up, t * 8) * a.scale_log2e;   // of query t
         }
+        group_sync<WPR>(grp);
+#pragma unroll
+        for (int j = 1; j < FREE; ++j) issue();
 
         float acc[NT][KS][4], mref[NT], l[NT];
 #pragma unroll
@@ -558,44 +611,77 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
                 for (int x = 0; x < 4; ++x) acc[n][i][x] = 0.0f;
         }
 
-        for (int j = 0; j < my_tiles; ++j) {
+        const unsigned char *slot = slots;
+        const float *mt = meta;
+        for (int j = 0, key0 = kbeg + wr * 16; j < my_tiles; ++j, key0 += 16 * WPR) {
             cp_wait<S - 2>();
             __syncwarp();
-            issue(j + S - 1);
-            const unsigned char *slot = slots + (j % S) * TILE;
-            const float *mt = meta + (j % S) * 4;
+            issue();
             // ---- scores
-            float sc[NT][4];
+            float sc[NT][2];   // of keys g and g + 8
+            if constexpr (INT) {
+                int s[NT][2][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int b = 0; b < D / 64; ++b) {
-                const int c = D == 64 ? t : (b * 4 + t) ^ ((g & 1) << 2);
-                const uint4 r0 = *reinterpret_cast<const uint4 *>(slot + g * D + c * 16);
-                const uint4 r1 = *reinterpret_cast<const uint4 *>(slot + (g + 8) * D + c * 16);
-                const unsigned w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+                    for (int i = 0; i < 2; ++i) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unsigned f[4];
-                    codes_to_half<FMT>(w0[i], f[0], f[2]);
-                    codes_to_half<FMT>(w1[i], f[1], f[3]);
+                for (int b = 0; b < D / 64; ++b) {
+                    const int c = D == 64 ? t : (b * 4 + t) ^ ((g & 1) << 2);
+                    const uint4 r0 = *reinterpret_cast<const uint4 *>(slot + g * D + c * 16);
+                    const uint4 r1 = *reinterpret_cast<const uint4 *>(slot + (g + 8) * D + c * 16);
+                    const unsigned f0[4] = {r0.x, r1.x, r0.y, r1.y}, f1[4] = {r0.z, r1.z, r0.w, r1.w};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816(sc[n], f, qf[n][b * 4 + i][0], qf[n][b * 4 + i][1]);
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma16832(s[n][i], f0, qf[n][i * (KS / 2) + b * 2][0], qf[n][i * (KS / 2) + b * 2][1]);
+                            mma16832(s[n][i], f1, qf[n][i * (KS / 2) + b * 2 + 1][0], qf[n][i * (KS / 2) + b * 2 + 1][1]);
+                        }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    sc[n][0] = fmaf((float)(s[n][0][0] * 256 + s[n][0][1]), 65536.0f, (float)(s[n][1][0] * 256 + s[n][1][1]));
+                    sc[n][1] = fmaf((float)(s[n][0][2] * 256 + s[n][0][3]), 65536.0f, (float)(s[n][1][2] * 256 + s[n][1][3]));
+                }
+            } else {
+                float s[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b) {
+                    const int c = D == 64 ? t : (b * 4 + t) ^ ((g & 1) << 2);
+                    const uint4 r0 = *reinterpret_cast<const uint4 *>(slot + g * D + c * 16);
+                    const uint4 r1 = *reinterpret_cast<const uint4 *>(slot + (g + 8) * D + c * 16);
+                    const unsigned w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        unsigned f[4];
+                        codes_to_half<FMT>(w0[i], f[0], f[2]);
+                        codes_to_half<FMT>(w1[i], f[1], f[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][b * 4 + i][0], qf[n][b * 4 + i][1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    sc[n][0] = fmaf(s[n][1], kLoUnscale, s[n][0]);
+                    sc[n][1] = fmaf(s[n][3], kLoUnscale, s[n][2]);
                 }
             }
             // ---- weights
-            const int key0 = kbeg + (j * WPR + wr) * 16;
-            const float ks = mt[0], vs = fmaxf(mt[1], kScaleFloor) + (mt[1] - mt[1]);   // NaN stays NaN
-            const bool there = mt[2] != 0.0f;
-            const float lvs = there ? log2_fast(vs) : -INFINITY, rvs = there ? __frcp_rn(vs) : 0.0f;
+            const float2 scales = *reinterpret_cast<const float2 *>(mt);
+            const bool there = !(scales.y < 0.0f);                              // a NaN scale is there
+            const float vs = scales.y < kScaleFloor ? kScaleFloor : scales.y;   // and stays NaN
+            const float lvs = there ? log2_fast(vs) : -INFINITY, rvs = rcp_fast(vs);
             const bool all = key0 + 16 <= lim_first;
             float w[NT][2];
             bool raise = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float f = there ? ks * qfac[n] : 0.0f;
-                w[n][0] = fmaf(fmaf(sc[n][1], kLoUnscale, sc[n][0]), f, lvs);
-                w[n][1] = fmaf(fmaf(sc[n][3], kLoUnscale, sc[n][2]), f, lvs);
+                const float f = there ? scales.x * qfac[n] : 0.0f;
+                w[n][0] = fmaf(sc[n][0], f, lvs);
+                w[n][1] = fmaf(sc[n][1], f, lvs);
                 if (!all) {
                     if (key0 + g >= lim[n]) w[n][0] = -INFINITY;
                     if (key0 + g + 8 >= lim[n]) w[n][1] = -INFINITY;
@@ -623,8 +709,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
             for (int n = 0; n < NT; ++n) {
                 const float p0 = exp2_fast(w[n][0] - mref[n]), p1 = exp2_fast(w[n][1] - mref[n]);
                 if (p0 + p1 != 0.0f) l[n] = fmaf(p0 + p1, rvs, l[n]);   // a NaN scale reaches only columns that see it
-                pb[n][0] = transpose8x8(split_half(p0));
-                pb[n][1] = transpose8x8(split_half(p1));
+                unsigned s0, s1;
+                split_half2(p0, p1, s0, s1);
+                pb[n][0] = transpose8x8(s0);
+                pb[n][1] = transpose8x8(s1);
             }
             // ---- outputs: keys 2t, 2t + 1, 2t + 8, 2t + 9 of this thread's D / 8 dimensions
             const unsigned char *vslot = slot + 16 * D;
@@ -653,6 +741,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma16816(acc[n][i], f, pb[n][0], pb[n][1]);
             }
+            slot = slot + TILE == slots + S * TILE ? slots : slot + TILE;
+            mt = mt + 2 == meta + S * 2 ? meta : mt + 2;
         }
         cp_wait<0>();
 
@@ -723,30 +813,48 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv8_attention_kernel(AttnA
                 const float *piece0 = a.parts + ((size_t)w0 * 2 + (run_begin > share_begin(w0) ? 1 : 0)) * PART;
                 const float *pieces = a.parts + (size_t)w0 * 2 * PART;
                 const int n = (int)(w1 - w0) + 1;
-                for (int i = gt; i < cols * D; i += 32 * WPR) {
-                    const int c = i / D;
-                    float m = kNoMax, sum_w = 0.0f, sum_o = 0.0f;
-                    for (int x = 0; x < n; x += 4) {   // four pieces' loads at a time; in order
-                        float pm[4], pw[4], po[4];
+                constexpr int TH = 32 * WPR, PER = COLS * D > TH ? 2 : 1;   // outputs of a thread taken together
+                for (int i0 = gt; i0 < cols * D; i0 += PER * TH) {
+                    float m[PER], sum_w[PER], sum_o[PER];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
+                    for (int z = 0; z < PER; ++z) {
+                        m[z] = kNoMax;
+                        sum_w[z] = sum_o[z] = 0.0f;
+                    }
+                    for (int x = 0; x < n; x += 8) {   // the loads of eight pieces at a time; summed in order
+                        float pm[PER][8], pw[PER][8], po[PER][8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
                             const float *p = x + y == 0 ? piece0 : pieces + (size_t)(x + y) * 2 * PART;
-                            pm[y] = x + y < n ? __ldcg(p + COLS * D + c) : kNoMax;
-                            pw[y] = x + y < n ? __ldcg(p + COLS * (D + 1) + c) : 0.0f;
-                            po[y] = x + y < n ? __ldcg(p + i) : 0.0f;
-                        }
-                        const float nm = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), f = exp2_fast(m - nm);
-                        m = nm;
-                        sum_w *= f;
-                        sum_o *= f;
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const float fix = exp2_fast(pm[y] - nm);
-                            sum_w = fmaf(pw[y], fix, sum_w);
-                            sum_o = fmaf(po[y], fix, sum_o);
+                            for (int z = 0; z < PER; ++z) {
+                                const int i = i0 + z * TH, c = i / D;
+                                const bool there = x + y < n && i < cols * D;
+                                pm[z][y] = there ? __ldcg(p + COLS * D + c) : kNoMax;
+                                pw[z][y] = there ? __ldcg(p + COLS * (D + 1) + c) : 0.0f;
+                                po[z][y] = there ? __ldcg(p + i) : 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int z = 0; z < PER; ++z) {
+                            float nm = m[z];
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) nm = fmaxf(nm, pm[z][y]);
+                            const float f = exp2_fast(m[z] - nm);
+                            m[z] = nm;
+                            sum_w[z] *= f;
+                            sum_o[z] *= f;
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) {
+                                const float fix = exp2_fast(pm[z][y] - nm);
+                                sum_w[z] = fmaf(pw[z][y], fix, sum_w[z]);
+                                sum_o[z] = fmaf(po[z][y], fix, sum_o[z]);
+                            }
                         }
                     }
-                    store(i, sum_w == 0.0f ? 0.0f : sum_o / sum_w);
+#pragma unroll
+                    for (int z = 0; z < PER; ++z)
+                        if (i0 + z * TH < cols * D) store(i0 + z * TH, sum_w[z] == 0.0f ? 0.0f : sum_o[z] / sum_w[z]);
                 }
             }
         }
@@ -768,7 +876,7 @@ AttnPlan attn_plan(const g2_kv8 &c, int n_head, int n_seq, int max_q, int sms) {
     const long long runs = (long long)n_seq * c.n_kv_head * ((cols + 4 * p.nt - 1) / (4 * p.nt));
     p.wpr = runs >= 2LL * sms * kAttnWarps ? 1 : 8;
     p.unit = p.wpr == 1 ? 64 : 128;
-    p.workers = sms * 2 * (kAttnWarps / p.wpr);
+    p.workers = sms * (c.head_dim * p.nt >= 256 ? 1 : 2) * (kAttnWarps / p.wpr);
     if (p.workers > kMaxWorkers) p.workers = kMaxWorkers;
     p.part_floats = (size_t)p.workers * 2 * 4 * p.nt * (c.head_dim + 2);
     return p;
@@ -786,10 +894,10 @@ int attn_sms() {
 template <int FMT, int D, int NT, int WPR>
 int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
     auto kernel = kv8_attention_kernel<FMT, D, NT, WPR>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnRing<D>::kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (AttnRing<D, NT>::kSmem)) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_kv8_attention", cudaGetErrorString(cudaGetLastError()));
     const int per_cta = kAttnWarps / WPR;
-    kernel<<<(a.workers + per_cta - 1) / per_cta, kAttnWarps * 32, AttnRing<D>::kSmem, st>>>(a);
+    kernel<<<(a.workers + per_cta - 1) / per_cta, kAttnWarps * 32, (AttnRing<D, NT>::kSmem), st>>>(a);
     return launch_status("g2k_kv8_attention");
 }
 
