@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(256)
 // 4 NT query columns (column c of a sequence: row c / group, head c % group).
 // Runs are cut into units of `unit` keys; all units, in order, are shared
 // equally among the workers (WPR warps each), so the shares do not depend on
-// how ragged the sequences are.  A run that crosses shares leaves partial
+// how ragged the sequences are.  Beginning a run costs as much as several units,
+// so each counts as `ahead` more, which hold no keys.  A run that crosses shares leaves partial
 // results (m, sum, accumulators) in the workspace; the last worker to arrive
 // merges them in order, so results do not depend on timing.
 //
@@ -269,7 +270,8 @@ struct AttnArgs {
     float scale_log2e;
     const int *seq_len;
     Rows8 r;
-    int unit, workers;       // most workers; fewer where there are fewer units
+    int unit, ahead;         // keys of a unit; units without keys ahead of a run's
+    int workers;             // most workers; fewer where there are fewer units
     unsigned *counters;      // [kMaxWorkers], zero between calls
     float *parts;            // [workers][2][columns * (D + 2)]
 };
@@ -353,10 +355,7 @@ __device__ __forceinline__ void split_half2(float v0, float v1, unsigned &s0, un
 
 template <int WPR>
 __device__ __forceinline__ void group_sync(int group) {
-    if (WPR == 1)
-        __syncwarp();
-    else
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * WPR) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * WPR) : "memory");
 }
 
 // Units of sequence s (0 where it has no rows or is out of range).
@@ -377,7 +376,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
         w.n = 0;
         return w;
     }
-    w.units = max(1, (w.len + a.unit - 1) / a.unit);   // a row that sees nothing is still written
+    w.units = max(1, (w.len + a.unit - 1) / a.unit) + a.ahead;   // a row that sees nothing is still written
     w.col_groups = (w.n * a.group + COLS - 1) / COLS;
     w.total = (unsigned)w.units * w.col_groups * a.c.n_kv_head;   // below 2^31 over all sequences: checked on the host
     return w;
@@ -475,10 +474,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             sw = work_of(++s);
         }
         const unsigned rem = u - seq_begin;
-        const int run = (int)(rem / (unsigned)sw.units), unit0 = (int)rem - run * sw.units;
+        const int run = (int)(rem / (unsigned)sw.units), unit = (int)rem - run * sw.units;
         const int h = run / sw.col_groups, col0 = run % sw.col_groups * COLS;
-        const int n_units = (int)min((unsigned)(sw.units - unit0), u_end - u);
-        const unsigned run_begin = u - unit0;
+        const unsigned run_begin = u - unit, piece_end = min(run_begin + sw.units, u_end);
+        // units with keys that are this piece's; the run's first ones may all lie in the next share
+        const int unit0 = max(unit - a.ahead, 0), unit1 = (int)(piece_end - run_begin) - a.ahead;
+        if (unit1 <= 0) break;
         const int cols = min(COLS, sw.n * a.group - col0);
         // key limits of the columns; `lim` of this thread's (column t of each n tile)
         const int lim_first = sw.len - sw.n + col0 / a.group + 1, lim_last = sw.len - sw.n + (col0 + cols - 1) / a.group + 1;
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             lim[n] = n * 4 + t < cols ? sw.len - sw.n + col / a.group + 1 : 0;
         }
         const int kbeg = unit0 * a.unit;
-        const int kend = (int)min((long long)min(sw.len, lim_last), (long long)(unit0 + n_units) * a.unit);
+        const int kend = (int)min((long long)min(sw.len, lim_last), (long long)unit1 * a.unit);
         const int n_tiles = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
         const int my_tiles = n_tiles > wr ? (n_tiles - wr + WPR - 1) / WPR : 0;
         const int *table = a.r.table + (long long)s * a.r.table_stride;
@@ -503,6 +504,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             bad(a.r);
             return -1;
         };
+        // the warp's (first) query, ahead of the codes that would delay it
+        auto load_query = [&](int c) -> float4 {
+            const int col = col0 + c, row = col / a.group, d = lane * 4;
+            if (c >= cols || d >= D) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const long long o = (long long)(sw.first + row) * a.q_stride + (long long)(h * a.group + col - row * a.group) * D + d;
+            return a.f16 ? load4<__half>(static_cast<const __half *>(a.q) + o) : load4<float>(static_cast<const float *>(a.q) + o);
+        };
+        float4 x = load_query(wr);
         int pages = load_pages(0), pages_next = my_tiles > 32 ? load_pages(32) : -1;
         int next = 0, key_next = kbeg + wr * 16, put = 0;   // the next tile to copy, its first key, its slot
         auto issue = [&]() {
@@ -547,10 +556,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         // query i; int8 keys have two n tiles, for the upper two and the lower two of the four bytes
         unsigned *qs = reinterpret_cast<unsigned *>(ring + grp * WPR * S * TILE + (S - FREE) * TILE);   // [NT][KS][2][lane]
         for (int c = wr; c < cols; c += WPR) {
-            const int col = col0 + c, row = col / a.group, d = lane * 4;
-            const long long o = (long long)(sw.first + row) * a.q_stride + (long long)(h * a.group + col - row * a.group) * D + d;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (d < D) x = a.f16 ? load4<__half>(static_cast<const __half *>(a.q) + o) : load4<float>(static_cast<const float *>(a.q) + o);
+            if (c != wr) x = load_query(c);
+            const int d = lane * 4;
             const unsigned peak = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
             // a power of two below the largest (2^e <= it < 2^(e + 1)), so that no type's range matters
             const int e = max(INT ? -96 : -126, min(126, (int)(peak >> 23) - 127));
@@ -769,7 +776,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         }
         group_sync<WPR>(grp);
 
-        const bool whole = n_units == sw.units;
+        const bool whole = unit0 == 0 && unit1 == sw.units - a.ahead;
         float *part = a.parts + ((size_t)worker * 2 + (first_piece ? 0 : 1)) * PART;
         auto store = [&](int i, float v) {
             const int c = i / D, d = i % D, col = col0 + c, row = col / a.group;
@@ -799,7 +806,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             }
         }
         if (!whole) {
-            const unsigned w0 = worker_of(run_begin), w1 = worker_of(run_begin + sw.units - 1);
+            const unsigned w0 = worker_of(run_begin + a.ahead), w1 = worker_of(run_begin + sw.units - 1);
             group_sync<WPR>(grp);
             if (gt == 0) {   // releases the group's results and acquires the others'
                 unsigned seen;
@@ -810,7 +817,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             if (arrived[grp] == (int)(w1 - w0)) {   // every other piece is there
                 if (gt == 0) a.counters[w0] = 0;
                 // piece of worker x: its first one, or, where the run begins inside the share, its last
-                const float *piece0 = a.parts + ((size_t)w0 * 2 + (run_begin > share_begin(w0) ? 1 : 0)) * PART;
+                const float *piece0 = a.parts + ((size_t)w0 * 2 + (share_begin(w0) < run_begin ? 1 : 0)) * PART;
                 const float *pieces = a.parts + (size_t)w0 * 2 * PART;
                 const int n = (int)(w1 - w0) + 1;
                 constexpr int TH = 32 * WPR, PER = COLS * D > TH ? 2 : 1;   // outputs of a thread taken together
@@ -860,13 +867,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         }
         group_sync<WPR>(grp);   // the merge buffer is the next piece's ring
         first_piece = false;
-        u += n_units;
+        u = piece_end;
     }
 }
 
 // Query columns a warp works on together, and how the work is cut.
 struct AttnPlan {
-    int nt, wpr, unit, workers;
+    int nt, wpr, unit, ahead, workers;
     size_t part_floats;
 };
 AttnPlan attn_plan(const g2_kv8 &c, int n_head, int n_seq, int max_q, int sms) {
@@ -874,8 +881,14 @@ AttnPlan attn_plan(const g2_kv8 &c, int n_head, int n_seq, int max_q, int sms) {
     const long long cols = (long long)max_q * (n_head / c.n_kv_head);
     p.nt = cols <= 4 ? 1 : cols <= 8 || c.head_dim == 128 ? 2 : 4;
     const long long runs = (long long)n_seq * c.n_kv_head * ((cols + 4 * p.nt - 1) / (4 * p.nt));
-    p.wpr = runs >= 2LL * sms * kAttnWarps ? 1 : 8;
-    p.unit = p.wpr == 1 ? 64 : 128;
+    // Few runs: eight warps share one, as each crosses many workers.  Many: pairs of warps, so that the
+    // beginnings and ends of runs overlap (32 x 16 runs of up to 1024 keys: 13.9 us, eight warps 16.6;
+    // 4 x 8 runs of up to 65536: 57.6, pairs 76).  `ahead` evens the workers' times where runs are short
+    // (9 x 25 runs of up to 2021 keys: 18.4, without it 24.7).
+    const bool many = runs >= 2LL * sms;
+    p.wpr = many ? 2 : 8;
+    p.unit = many ? 64 : 128;
+    p.ahead = many ? 2 : 3;
     p.workers = sms * (c.head_dim * p.nt >= 256 ? 1 : 2) * (kAttnWarps / p.wpr);
     if (p.workers > kMaxWorkers) p.workers = kMaxWorkers;
     p.part_floats = (size_t)p.workers * 2 * 4 * p.nt * (c.head_dim + 2);
@@ -903,7 +916,7 @@ int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
 
 template <int FMT, int D, int NT>
 int launch_attn(const AttnArgs &a, int wpr, int sms, cudaStream_t st) {
-    return wpr == 1 ? launch_attn<FMT, D, NT, 1>(a, sms, st) : launch_attn<FMT, D, NT, 8>(a, sms, st);
+    return wpr == 2 ? launch_attn<FMT, D, NT, 2>(a, sms, st) : launch_attn<FMT, D, NT, 8>(a, sms, st);
 }
 
 template <int FMT>
@@ -1046,7 +1059,7 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if ((long long)max_q * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
     {   // the kernel counts units in 32 bits
         const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, 1);
-        const double units = ((double)table_stride * cache->page_size / p.unit + 1) * n_seq * cache->n_kv_head *
+        const double units = ((double)table_stride * cache->page_size / p.unit + 1 + p.ahead) * n_seq * cache->n_kv_head *
                              ((double)max_q * (n_head / cache->n_kv_head) / (4 * p.nt) + 1);
         if (units > 2147483647.0) return arg_error(G2_ERR_RANGE, who, "too much work for one call");
     }
@@ -1060,7 +1073,7 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     const int sms = attn_sms();
     const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, sms);
     const AttnArgs a{*cache, q, out, q_stride, out_stride, dtype == G2_F16, n_head / cache->n_kv_head,
-                     scale * 1.4426950408889634f, seq_len, r, p.unit, p.workers, static_cast<unsigned *>(workspace),
+                     scale * 1.4426950408889634f, seq_len, r, p.unit, p.ahead, p.workers, static_cast<unsigned *>(workspace),
                      static_cast<float *>(workspace) + kMaxWorkers};
     return cache->format == G2_KV_I8 ? launch_attn<G2_KV_I8>(a, p, sms, (cudaStream_t)stream)
                                      : launch_attn<G2_KV_E4M3>(a, p, sms, (cudaStream_t)stream);
