@@ -6,6 +6,7 @@
 // (-127..127) or e4m3 (up to 448).
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "g2_args.h"
@@ -105,23 +106,62 @@ __device__ __forceinline__ float4 load4<__half>(const __half *p) {
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// A block's scale after rows whose largest magnitude has the bits `peak` (integers: NaN above infinity
+// above finite) join rows at scale `was` (0 where none stay).
+template <int FMT>
+__device__ __forceinline__ float joined_scale(unsigned peak, float was) {
+    if (peak >= 0x7f800000u || was != was) return __uint_as_float(0x7fc00000u);
+    return fmaxf(fmaxf(__fdiv_rn(__uint_as_float(peak), FMT == G2_KV_I8 ? 127.0f : 448.0f), kScaleFloor), was);
+}
+
+// A word of codes through the table of a magnitude's new code (rows that stay when the scale grows).
+template <int FMT>
+__device__ __forceinline__ unsigned recode_word(unsigned w, const unsigned char *table) {
+    unsigned r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned c = (w >> (8 * i)) & 0xffu;
+        if (FMT == G2_KV_I8) {
+            const int s = (int)(signed char)c, m = table[min(abs(s), 127)];
+            r |= ((unsigned)(s < 0 ? -m : m) & 0xffu) << (8 * i);
+        } else {
+            r |= (table[c & 0x7fu] | (c & 0x80u)) << (8 * i);
+        }
+    }
+    return r;
+}
+
+template <int FMT>
+__device__ __forceinline__ unsigned encode4(const float4 &x, float scale) {
+    if (scale != scale) return 0;
+    return encode<FMT>(div_odd(x.x, scale)) | encode<FMT>(div_odd(x.y, scale)) << 8 | encode<FMT>(div_odd(x.z, scale)) << 16 |
+           encode<FMT>(div_odd(x.w, scale)) << 24;
+}
+
 // ---- append -----------------------------------------------------------------------
-// One CTA for each (block of a sequence, head, K or V): the new rows' largest
-// magnitude as an integer maximum (NaN above infinity above finite), the scale,
-// the kept rows again if it grew, the new rows' codes.  A thread holds its
-// 4-element vectors of the block in registers between the two passes.
-constexpr int kAppendThreads = 256;
+// A *tile* is the K or V rows of one block and head.  Its new rows' largest magnitude
+// gives the scale; the rows that stay are rounded again if it grew; the new rows'
+// codes follow.  Bound by the rows read (2 or 4 bytes a value) and codes written.
+//
+// Several rows a sequence: one CTA takes the block's next tiles, as many as give a
+// thread kAppendVecs 4-element loads, all in flight together: a tile by itself
+// waits for its sequence's numbers, its page and its rows in turn (71 -> 26 us for
+// 8 prompts of up to 1000 tokens of 25 heads, reading the rows back included).
+constexpr int kAppendThreads = 256, kAppendVecs = 8;
 
 template <typename T, int FMT, int VPT>
 __global__ void __launch_bounds__(kAppendThreads)
     kv8_append_kernel(g2_kv8 c, const T *k, const T *v, long long stride, const int *pos, Rows8 r, int blocks_per_seq) {
-    __shared__ unsigned peaks[kAppendThreads / 32];
-    const int t = threadIdx.x;
-    const int s = blockIdx.x / blocks_per_seq, h = blockIdx.y, is_v = blockIdx.z;
+    constexpr int TILES = kAppendVecs / VPT > 0 ? kAppendVecs / VPT : 1;
+    __shared__ unsigned peaks[TILES][kAppendThreads / 32];
+    __shared__ float scale_s[TILES][2];                 // before, after
+    __shared__ unsigned char table[TILES][128];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int s = blockIdx.x / blocks_per_seq, tile0 = blockIdx.y * TILES, n_tiles = min(TILES, 2 * c.n_kv_head - tile0);
     const int P = c.page_size, D = c.head_dim, per_row = D / 4;
+    const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
     if (sp.n == 0) return;
-    const int p0 = pos[s];
     if (p0 < 0 || (long long)p0 + sp.n > (long long)r.table_stride * P) {
         bad(r);
         return;
@@ -129,88 +169,162 @@ __global__ void __launch_bounds__(kAppendThreads)
     const int block = p0 / P + blockIdx.x % blocks_per_seq;
     const long long start = (long long)block * P;
     if (start >= (long long)p0 + sp.n) return;
-    const int page = page_of(r, c, s, block);
-    if (page < 0) return;
     const int kept = max(0, (int)(p0 - start));                        // rows 0..kept-1 stay
     const int end = (int)min((long long)P, (long long)p0 + sp.n - start);   // rows kept..end-1 are new
-    const T *src = (is_v ? v : k) + (sp.first + start - p0) * stride + (long long)h * D;
-    const long long at = (long long)page * c.n_kv_head + h;
-    unsigned char *dst = static_cast<unsigned char *>(is_v ? c.v : c.k) + at * P * D;
-    float *scale = (is_v ? c.v_scale : c.k_scale) + at;
+    const int page = page_of(r, c, s, block);
+    if (page < 0) return;
+    const long long first = sp.first + start - p0;                     // row 0 of the block, in k and v
 
-    float4 x[VPT];
-    unsigned peak = 0;
+    float4 x[TILES][VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int vec = t + i * kAppendThreads, row = vec / per_row;
-        if (row >= kept && row < end) {
-            x[i] = load4<T>(src + (long long)row * stride + (vec % per_row) * 4);
-            peak = max(max(peak, max(abs_bits(x[i].x), abs_bits(x[i].y))), max(abs_bits(x[i].z), abs_bits(x[i].w)));
+    for (int j = 0; j < TILES; ++j) {
+        const int tile = tile0 + j, h = tile >> 1;
+        const T *src = (tile & 1 ? v : k) + first * stride + (long long)h * D;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int vec = t + i * kAppendThreads, row = vec / per_row;
+            x[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (j < n_tiles && row >= kept && row < end) x[j][i] = load4<T>(src + (long long)row * stride + (vec % per_row) * 4);
         }
     }
-    const float was = kept > 0 ? *scale : 0.0f;
-    peak = __reduce_max_sync(0xffffffffu, peak);
-    if ((t & 31) == 0) peaks[t >> 5] = peak;
+    if (t < n_tiles) {
+        const int tile = tile0 + t;
+        const long long at = (long long)page * c.n_kv_head + (tile >> 1);
+        scale_s[t][0] = kept > 0 ? (tile & 1 ? c.v_scale : c.k_scale)[at] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+        unsigned peak = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            peak = max(max(peak, max(abs_bits(x[j][i].x), abs_bits(x[j][i].y))), max(abs_bits(x[j][i].z), abs_bits(x[j][i].w)));
+        peak = __reduce_max_sync(0xffffffffu, peak);
+        if (lane == 0) peaks[j][warp] = peak;
+    }
     __syncthreads();
-    peak = peaks[0];
+    bool grown = false;
+    if (t < n_tiles) {
+        const int tile = tile0 + t;
+        const long long at = (long long)page * c.n_kv_head + (tile >> 1);
+        unsigned peak = 0;
 #pragma unroll
-    for (int i = 1; i < kAppendThreads / 32; ++i) peak = max(peak, peaks[i]);
-    float to = fmaxf(__fdiv_rn(__uint_as_float(peak), FMT == G2_KV_I8 ? 127.0f : 448.0f), kScaleFloor);
-    if (peak >= 0x7f800000u || was != was) to = __uint_as_float(0x7fc00000u);
-    else if (was > to) to = was;
-    const bool again = to > was;
+        for (int i = 0; i < kAppendThreads / 32; ++i) peak = max(peak, peaks[t][i]);
+        const float to = joined_scale<FMT>(peak, scale_s[t][0]);
+        scale_s[t][1] = to;
+        (tile & 1 ? c.v_scale : c.k_scale)[at] = to;
+        grown = kept > 0 && to > scale_s[t][0];
+    }
+    if (__syncthreads_or(grown)) {
+        for (int i = t; i < n_tiles * 128; i += kAppendThreads) {
+            const int j = i >> 7, m = i & 127;
+            if (scale_s[j][1] > scale_s[j][0]) table[j][m] = (unsigned char)recode<FMT>(m, scale_s[j][0], scale_s[j][1]);
+        }
+        __syncthreads();
+    }
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int vec = t + i * kAppendThreads, row = vec / per_row;
-        unsigned *out = reinterpret_cast<unsigned *>(dst) + vec;
-        if (row < kept) {
-            if (again) {
-                const unsigned w = *out;
-                *out = recode<FMT>(w & 0xffu, was, to) | recode<FMT>((w >> 8) & 0xffu, was, to) << 8 |
-                       recode<FMT>((w >> 16) & 0xffu, was, to) << 16 | recode<FMT>(w >> 24, was, to) << 24;
+    for (int j = 0; j < TILES; ++j) {
+        if (j >= n_tiles) break;
+        const int tile = tile0 + j;
+        const long long at = (long long)page * c.n_kv_head + (tile >> 1);
+        unsigned *dst = reinterpret_cast<unsigned *>(static_cast<unsigned char *>(tile & 1 ? c.v : c.k) + at * P * D);
+        const float was = scale_s[j][0], to = scale_s[j][1];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int vec = t + i * kAppendThreads, row = vec / per_row;
+            if (row < kept) {
+                if (to > was) dst[vec] = recode_word<FMT>(dst[vec], table[j]);
+            } else if (row < end) {
+                dst[vec] = encode4<FMT>(x[j][i], to);
             }
-        } else if (row < end) {
-            unsigned w = 0;
-            if (to == to)
-                w = encode<FMT>(div_odd(x[i].x, to)) | encode<FMT>(div_odd(x[i].y, to)) << 8 |
-                    encode<FMT>(div_odd(x[i].z, to)) << 16 | encode<FMT>(div_odd(x[i].w, to)) << 24;
-            *out = w;
         }
     }
-    if (t == 0) *scale = to;
+}
+
+// One row a sequence (a decode step): one warp for each (sequence, tile).
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(256) kv8_append_token_kernel(g2_kv8 c, const T *k, const T *v, long long stride, const int *pos, Rows8 r) {
+    __shared__ unsigned char table[8][128];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int s = blockIdx.x, tile = blockIdx.y * 8 + warp, h = tile >> 1, P = c.page_size;
+    if (tile >= 2 * c.n_kv_head) return;
+    const int p = pos[s];
+    const Span sp = seq_rows(r, s);
+    if (sp.n == 0) return;
+    if (p < 0 || p >= (long long)r.table_stride * P) {
+        bad(r);
+        return;
+    }
+    const int page = page_of(r, c, s, p / P), kept = p & (P - 1);
+    if (page < 0) return;
+    const long long at = (long long)page * c.n_kv_head + h;
+    unsigned *dst = reinterpret_cast<unsigned *>(static_cast<unsigned char *>(tile & 1 ? c.v : c.k) + at * P * D);
+    float *scale = (tile & 1 ? c.v_scale : c.k_scale) + at;
+    const float was = kept > 0 ? *scale : 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (lane < D / 4) x = load4<T>((tile & 1 ? v : k) + sp.first * stride + (long long)h * D + lane * 4);
+    const unsigned peak = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
+    const float to = joined_scale<FMT>(peak, was);
+    if (kept > 0 && to > was) {
+        // the new code of each magnitude, then the rows that stay
+#pragma unroll
+        for (int i = 0; i < 4; ++i) table[warp][lane + 32 * i] = (unsigned char)recode<FMT>(lane + 32 * i, was, to);
+        __syncwarp();
+#pragma unroll 4
+        for (int i = lane; i < kept * (D / 4); i += 32) dst[i] = recode_word<FMT>(dst[i], table[warp]);
+    }
+    if (lane < D / 4) dst[kept * (D / 4) + lane] = encode4<FMT>(x, to);
+    if (lane == 0) *scale = to;
 }
 
 // ---- gather -----------------------------------------------------------------------
+// One CTA for 16 positions of a sequence and 256 groups of four of a row's values (K
+// and V), a group per thread: a thread's page and scale are the same for all its
+// rows, its loads are in flight together and its stores 16 bytes (8 of fp16).
 constexpr int kGatherRows = 16;
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
-    kv8_gather_kernel(g2_kv8 c, T *k, T *v, long long stride, const int *pos, Rows8 r, int groups_per_seq) {
-    const int s = blockIdx.x / groups_per_seq, h = blockIdx.y;
-    const int P = c.page_size, D = c.head_dim, per_row = D / 4;
+    kv8_gather_kernel(g2_kv8 c, T *k, T *v, long long stride, const int *pos, Rows8 r, int chunks_per_seq) {
+    const int s = blockIdx.x / chunks_per_seq;
+    const int P = c.page_size, D = c.head_dim, per_row = c.n_kv_head * D / 4;
+    const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
     if (sp.n == 0) return;
-    const int p0 = pos[s];
     if (p0 < 0 || (long long)p0 + sp.n > (long long)r.table_stride * P) {
         bad(r);
         return;
     }
-    const int j0 = blockIdx.x % groups_per_seq * kGatherRows, j1 = min(sp.n, j0 + kGatherRows);
-    for (int i = threadIdx.x; i < (j1 - j0) * per_row * 2; i += 256) {
-        const int is_v = i >= (j1 - j0) * per_row, q = is_v ? i - (j1 - j0) * per_row : i;
-        const int j = j0 + q / per_row, d = q % per_row * 4, p = p0 + j;
-        const int page = page_of(r, c, s, p / P);
-        if (page < 0) continue;
-        const long long at = (long long)page * c.n_kv_head + h;
-        const unsigned w = *reinterpret_cast<const unsigned *>(static_cast<const unsigned char *>(is_v ? c.v : c.k) +
-                                                               (at * P + p % P) * D + d);
-        const float sc = (is_v ? c.v_scale : c.k_scale)[at];
-        T *o = (is_v ? v : k) + (sp.first + j) * stride + (long long)h * D + d;
-        o[0] = fromf<T>(decode<FMT>(w & 0xffu) * sc);
-        o[1] = fromf<T>(decode<FMT>((w >> 8) & 0xffu) * sc);
-        o[2] = fromf<T>(decode<FMT>((w >> 16) & 0xffu) * sc);
-        o[3] = fromf<T>(decode<FMT>(w >> 24) * sc);
-    }
+    const long long base = (long long)(p0 / kGatherRows + blockIdx.x % chunks_per_seq) * kGatherRows;   // a page holds whole chunks
+    const int j0 = (int)(max(base, (long long)p0) - base), j1 = (int)min((long long)kGatherRows, (long long)p0 + sp.n - base);
+    if (j1 <= j0) return;
+    const int page = page_of(r, c, s, (int)(base / P));
+    const int q = blockIdx.y * 256 + threadIdx.x, is_v = q >= per_row, e = (is_v ? q - per_row : q) * 4;
+    if (page < 0 || q >= 2 * per_row) return;
+    const int h = e / D, d = e % D;
+    const long long at = (long long)page * c.n_kv_head + h;
+    const unsigned *src = reinterpret_cast<const unsigned *>(static_cast<const unsigned char *>(is_v ? c.v : c.k) +
+                                                             (at * P + base % P) * D + d);
+    const float scale = (is_v ? c.v_scale : c.k_scale)[at];
+    T *dst = (is_v ? v : k) + (sp.first + base - p0) * stride + e;
+    unsigned w[kGatherRows];
+#pragma unroll
+    for (int j = 0; j < kGatherRows; ++j)
+        if (j >= j0 && j < j1) w[j] = __ldg(src + j * (D / 4));
+#pragma unroll
+    for (int j = 0; j < kGatherRows; ++j)
+        if (j >= j0 && j < j1) {
+            const float4 x = make_float4(decode<FMT>(w[j] & 0xffu) * scale, decode<FMT>((w[j] >> 8) & 0xffu) * scale,
+                                         decode<FMT>((w[j] >> 16) & 0xffu) * scale, decode<FMT>(w[j] >> 24) * scale);
+            if (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(dst + j * stride) = x;
+            } else {
+                const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+                uint2 o;
+                o.x = *reinterpret_cast<const unsigned *>(&a);
+                o.y = *reinterpret_cast<const unsigned *>(&b);
+                *reinterpret_cast<uint2 *>(dst + j * stride) = o;
+            }
+        }
 }
 
 // ---- attention --------------------------------------------------------------------
@@ -968,10 +1082,17 @@ int check_rows(const char *who, const g2_kv8 *c, int heads, const void *a, const
 template <typename T, int FMT>
 void launch_append(const g2_kv8 &c, const void *k, const void *v, long long stride, const int *pos, const Rows8 &r,
                    cudaStream_t st) {
-    const int per = (c.page_size - 1 + r.max_q - 1) / c.page_size + 1;   // blocks that max_q rows can touch
-    const dim3 grid((unsigned)per * r.n_seq, c.n_kv_head, 2);
     const T *kt = static_cast<const T *>(k), *vt = static_cast<const T *>(v);
-    switch (c.page_size * c.head_dim / (4 * kAppendThreads)) {
+    if (r.max_q == 1) {
+        const dim3 grid(r.n_seq, (2 * c.n_kv_head + 7) / 8);
+        if (c.head_dim == 64) kv8_append_token_kernel<T, FMT, 64><<<grid, 256, 0, st>>>(c, kt, vt, stride, pos, r);
+        else kv8_append_token_kernel<T, FMT, 128><<<grid, 256, 0, st>>>(c, kt, vt, stride, pos, r);
+        return;
+    }
+    const int per = (c.page_size + r.max_q - 2) / c.page_size + 1;   // blocks that max_q rows can touch
+    const int vpt = c.page_size * c.head_dim / (4 * kAppendThreads), tiles = std::max(1, kAppendVecs / vpt);
+    const dim3 grid((unsigned)per * r.n_seq, (2 * c.n_kv_head + tiles - 1) / tiles);
+    switch (vpt) {
         case 1: kv8_append_kernel<T, FMT, 1><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
         case 2: kv8_append_kernel<T, FMT, 2><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
         case 4: kv8_append_kernel<T, FMT, 4><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
@@ -982,9 +1103,9 @@ void launch_append(const g2_kv8 &c, const void *k, const void *v, long long stri
 
 template <typename T, int FMT>
 void launch_gather(const g2_kv8 &c, void *k, void *v, long long stride, const int *pos, const Rows8 &r, cudaStream_t st) {
-    const int per = (r.max_q + kGatherRows - 1) / kGatherRows;
-    kv8_gather_kernel<T, FMT><<<dim3((unsigned)per * r.n_seq, c.n_kv_head), 256, 0, st>>>(
-        c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
+    const int per = (r.max_q + kGatherRows - 2) / kGatherRows + 1;   // chunks that max_q rows can touch
+    const dim3 grid((unsigned)per * r.n_seq, (c.n_kv_head * c.head_dim / 2 + 255) / 256);
+    kv8_gather_kernel<T, FMT><<<grid, 256, 0, st>>>(c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
 }
 
 // dtype and format to template arguments
@@ -1014,7 +1135,7 @@ extern "C" int g2k_kv8_append(const g2_kv8 *cache, const void *k, const void *v,
     if ((rc = check_cache(who, cache))) return rc;
     const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, cache->n_kv_head, k, v, dtype, &row_stride, nullptr, r, pos))) return rc;
-    if (((long long)max_q / cache->page_size + 2) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many blocks");
+    if (((long long)max_q / cache->page_size + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many blocks");
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k, v, q_start, pos, table, status})))
         return rc;
@@ -1030,7 +1151,7 @@ extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int
     if ((rc = check_cache(who, cache))) return rc;
     const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, cache->n_kv_head, k_out, v_out, dtype, &row_stride, nullptr, r, pos))) return rc;
-    if (((long long)max_q / kGatherRows + 1) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
+    if (((long long)max_q / kGatherRows + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k_out, v_out, q_start, pos, table, status})))
         return rc;
