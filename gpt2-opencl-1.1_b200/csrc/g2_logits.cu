@@ -1,15 +1,19 @@
 // g2_logits.cu -- rules on rows of logits before a token is picked: penalties
 // for tokens of the context, biases and grammar masks (g2k_process_logits).
 //
-// One CTA for each slice of kSlice columns of a row.  It requests its logits and
-// mask words, then counts the context's ids that fall into its slice in shared
-// memory (integer additions, so their order does not matter) and notes for each
-// biased column the last pair that names it, and so passes over its columns once,
-// with the tables built while the logits are on their way.  The context and the
-// pairs are read by every slice of the row, from L2 after the first.  Bound by the
-// bytes of the logits, read and written once.  Slices begin where a row's address
-// is a multiple of 16 bytes, whatever the row stride, so that four columns move at
-// a time.
+// One CTA for each slice of kSlice columns of a row.
+//   1. The columns are copied, masked ones as G2_MASKED, four at a time (slices
+//      begin where a row's address is a multiple of 16 bytes, whatever the stride).
+//      In place only masked columns are written and nothing is read.
+//   2. Meanwhile the context's ids that fall into the slice are counted in shared
+//      memory (integer additions, so their order does not matter), and each biased
+//      column notes the last pair that names it.  Whoever touches a column first
+//      puts it on a list.
+//   3. The columns of the list are computed and written over the copy: a context
+//      touches about one column in a hundred, and testing all of them in the copy
+//      took longer than the copy (256 rows of 50257: 37 us).
+// The context and the pairs are read by every slice of the row, from L2 after the
+// first.  Bound by the bytes of the logits, read and written once.
 #include "g2_args.h"
 #include "g2_device.cuh"
 
@@ -38,125 +42,134 @@ __device__ __forceinline__ void span_of(const int *start, int row, int n, int &a
     }
 }
 
+constexpr unsigned kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffffffu;
+
 template <bool PENAL, bool BIAS, bool MASK>
 __global__ void __launch_bounds__(kRuleThreads) rules_kernel(RuleArgs a) {
-    __shared__ __align__(16) unsigned count[PENAL ? kSlice : 4];   // ids after the prompt; top bit: anywhere in the context
-    __shared__ __align__(16) int pair[BIAS ? kSlice : 4];          // last pair of the column + 1
+    constexpr bool SPARSE = PENAL || BIAS;
+    __shared__ __align__(16) unsigned count[SPARSE ? kSlice : 4];   // ids after the prompt, and kSeen / kBiased
+    __shared__ int pair[BIAS ? kSlice : 1];                         // last pair of a biased column
+    __shared__ unsigned short list[SPARSE ? kSlice : 1];            // touched columns
+    __shared__ unsigned n_list;
     const int t = threadIdx.x, row = blockIdx.y;
     const g2_logit_rules &r = a.r;
     const float *in = a.logits + row * a.ld;
     float *out = a.out + row * a.ld_out;
-    const int shift = (int)(reinterpret_cast<size_t>(in) / 4 & 3);
-    const bool same = (int)(reinterpret_cast<size_t>(out) / 4 & 3) == shift, in_place = in == out;
-    const int v0 = blockIdx.x * kSlice - shift;                    // below 0 in the first slice
-    if (v0 >= a.V) return;                                         // the last slice of a row without a shift
+    const bool in_place = in == out;
+    const int shift = (int)(reinterpret_cast<size_t>(out) / 4 & 3);
+    const bool same = (int)(reinterpret_cast<size_t>(in) / 4 & 3) == shift;
+    const int v0 = blockIdx.x * kSlice - shift;                     // below 0 in the first slice
+    if (v0 >= a.V) return;                                          // the last slice of a row without a shift
+    const unsigned *mask = MASK ? r.mask + (long long)row * r.mask_stride : nullptr;
 
+    // ---- requests of the copy
     float4 l[kVecs];
     unsigned allowed[kVecs];
     auto column = [&](int i) { return v0 + 4 * (t + i * kRuleThreads); };
+    auto whole = [&](int c) { return c >= 0 && c + 3 < a.V; };
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
         const int c = column(i);
-        if (c >= 0 && c + 3 < a.V) {
-            l[i] = __ldcs(reinterpret_cast<const float4 *>(in + c));
-        } else {
-            float *e = &l[i].x;
+        if (!in_place) {
+            if (same && whole(c)) {
+                l[i] = __ldcs(reinterpret_cast<const float4 *>(in + c));
+            } else {
+                float *e = &l[i].x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = c + j >= 0 && c + j < a.V ? in[c + j] : 0.0f;
+                for (int j = 0; j < 4; ++j) e[j] = c + j >= 0 && c + j < a.V ? in[c + j] : 0.0f;
+            }
         }
         if (MASK) {
-            const unsigned *mask = r.mask + (long long)row * r.mask_stride;
             const int w0 = max(c, 0) >> 5, w1 = min(max(c, 0) + 3, a.V - 1) >> 5;
             const unsigned lo = c < a.V ? mask[w0] : 0u, hi = c < a.V ? mask[w1] : 0u;
             // bits c .. c + 3; a first group that begins before column 0 has its bits moved up
             allowed[i] = c >= 0 ? __funnelshift_r(lo, hi, c & 31) : lo << -c;
         }
     }
-    if (PENAL)
-        for (int i = t; i < kSlice / 4; i += kRuleThreads) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
-    if (BIAS)
-        for (int i = t; i < kSlice / 4; i += kRuleThreads) reinterpret_cast<uint4 *>(pair)[i] = make_uint4(0, 0, 0, 0);
+    // ---- the tables
+    int c0 = 0, c1 = 0, b0 = 0, b1 = 0;
+    long long made = 0;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (SPARSE) {
+        for (int i = t; i < kSlice / 4; i += kRuleThreads) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
+        if (t == 0) n_list = 0;
+    }
+    if (BIAS)
+        for (int i = t; i < kSlice; i += kRuleThreads) pair[i] = -1;
     if (PENAL) {
+        span_of(r.ctx_start, row, r.n_ctx, c0, c1);
+        made = (long long)c0 + (r.n_prompt ? max(r.n_prompt[row], 0) : 0);
         if (r.rep_penalty) rep = r.rep_penalty[row];
         if (r.frequency) freq = r.frequency[row];
         if (r.presence) pres = r.presence[row];
         if (!(rep > 0.0f)) rep = 1.0f;
     }
-    if (PENAL || BIAS) __syncthreads();
-    const int n = min(kSlice, a.V - v0);
+    if (BIAS) span_of(r.bias_start, row, r.n_bias, b0, b1);
+    if (SPARSE) __syncthreads();
+    const unsigned n = min(kSlice, a.V - v0);
+    auto touched = [&](unsigned at, unsigned old) {
+        if (old == 0) list[atomicAdd(&n_list, 1u)] = (unsigned short)at;
+    };
     if (PENAL) {
-        int c0, c1;
-        span_of(r.ctx_start, row, r.n_ctx, c0, c1);
-        const long long made = (long long)c0 + (r.n_prompt ? max(r.n_prompt[row], 0) : 0);
 #pragma unroll 4
         for (int i = c0 + t; i < c1; i += kRuleThreads) {
             const int id = r.ctx[i];
             const unsigned at = (unsigned)(id - v0);
-            if (id >= 0 && at < (unsigned)n) {
+            if (id >= 0 && at < n) {
+                touched(at, atomicOr(&count[at], kSeen));
                 if (i >= made) atomicAdd(&count[at], 1u);
-                atomicOr(&count[at], 0x80000000u);
             }
         }
     }
     if (BIAS) {
-        int b0, b1;
-        span_of(r.bias_start, row, r.n_bias, b0, b1);
 #pragma unroll 4
         for (int i = b0 + t; i < b1; i += kRuleThreads) {
             const int id = r.bias_ids[i];
             const unsigned at = (unsigned)(id - v0);
-            if (id >= 0 && at < (unsigned)n) atomicMax(&pair[at], i + 1);
+            if (id >= 0 && at < n) {
+                touched(at, atomicOr(&count[at], kBiased));
+                atomicMax(&pair[at], i);
+            }
         }
     }
-    if (PENAL || BIAS) __syncthreads();
+    // ---- the copy
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
         const int c = column(i);
         if (c >= a.V) break;
         float *e = &l[i].x;
-        bool changed = !in_place;
-        if (PENAL) {
-            const uint4 q = reinterpret_cast<const uint4 *>(count)[t + i * kRuleThreads];
-            if (q.x | q.y | q.z | q.w) {
-                changed = true;
-                const unsigned cs[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (cs[j]) {
-                        e[j] = e[j] > 0.0f ? e[j] / rep : e[j] * rep;
-                        const unsigned k = cs[j] & 0x7fffffffu;
-                        if (k) {
-                            e[j] -= freq * (float)k;
-                            e[j] -= pres;
-                        }
-                    }
-            }
-        }
-        if (BIAS) {
-            const int4 q = reinterpret_cast<const int4 *>(pair)[t + i * kRuleThreads];
-            if (q.x | q.y | q.z | q.w) {
-                changed = true;
-                const int ps[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (ps[j]) e[j] += r.bias[ps[j] - 1];
-            }
-        }
-        if (MASK && (allowed[i] & 15u) != 15u) {
-            changed = true;
+        const unsigned ok = MASK ? allowed[i] & 15u : 15u;
+        if (in_place && ok == 15u) continue;
+        if (MASK) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (!((allowed[i] >> j) & 1u)) e[j] = G2_MASKED;
+                if (!((ok >> j) & 1u)) e[j] = G2_MASKED;
         }
-        if (!changed) continue;
-        if (same && c >= 0 && c + 3 < a.V) {
+        if (whole(c) && (!in_place || ok == 0)) {
             __stcs(reinterpret_cast<float4 *>(out + c), l[i]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (c + j >= 0 && c + j < a.V) out[c + j] = e[j];
+                if (c + j >= 0 && c + j < a.V && (!in_place || !((ok >> j) & 1u))) out[c + j] = e[j];
         }
+    }
+    if (!SPARSE) return;
+    __syncthreads();
+    // ---- the touched columns, after their copies
+    for (unsigned i = t; i < n_list; i += kRuleThreads) {
+        const int at = list[i], c = v0 + at;
+        if (MASK && !((mask[c >> 5] >> (c & 31)) & 1u)) continue;
+        const unsigned q = count[at];
+        float x = in[c];
+        if (PENAL && (q & kSeen)) {
+            x = x > 0.0f ? x / rep : x * rep;
+            if (q & kCount) {
+                x -= freq * (float)(q & kCount);
+                x -= pres;
+            }
+        }
+        if (BIAS && (q & kBiased)) x += r.bias[pair[at]];
+        out[c] = x;
     }
 }
 
