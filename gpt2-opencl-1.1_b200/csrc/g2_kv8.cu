@@ -178,16 +178,15 @@ __device__ __forceinline__ unsigned encode4(const float4 &x, float scale, float 
 // 8 prompts of up to 1000 tokens of 25 heads, reading the rows back included).
 constexpr int kAppendThreads = 256, kAppendVecs = 8;
 
-template <typename T, int FMT, int VPT>
+template <typename T, int FMT, int D, int VPT>
 __global__ void __launch_bounds__(kAppendThreads)
     kv8_append_kernel(g2_kv8 c, const T *k, const T *v, long long stride, const int *pos, Rows8 r, int blocks_per_seq) {
-    constexpr int TILES = kAppendVecs / VPT > 0 ? kAppendVecs / VPT : 1;
+    constexpr int TILES = kAppendVecs / VPT > 0 ? kAppendVecs / VPT : 1, P = VPT * 4 * kAppendThreads / D, per_row = D / 4;
     __shared__ unsigned peaks[TILES][kAppendThreads / 32];
     __shared__ float scale_s[TILES][2];                 // before, after
     __shared__ unsigned char table[TILES][128];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int s = blockIdx.x / blocks_per_seq, tile0 = blockIdx.y * TILES, n_tiles = min(TILES, 2 * c.n_kv_head - tile0);
-    const int P = c.page_size, D = c.head_dim, per_row = D / 4;
     const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
     if (sp.n == 0) return;
@@ -200,8 +199,7 @@ __global__ void __launch_bounds__(kAppendThreads)
     if (start >= (long long)p0 + sp.n) return;
     const int kept = max(0, (int)(p0 - start));                        // rows 0..kept-1 stay
     const int end = (int)min((long long)P, (long long)p0 + sp.n - start);   // rows kept..end-1 are new
-    const int page = page_of(r, c, s, block);
-    if (page < 0) return;
+    const int page = page_of(r, c, s, block);                          // on its way with the rows
     const long long first = sp.first + start - p0;                     // row 0 of the block, in k and v
 
     float4 x[TILES][VPT];
@@ -216,6 +214,7 @@ __global__ void __launch_bounds__(kAppendThreads)
             if (j < n_tiles && row >= kept && row < end) x[j][i] = load4<T>(src + (long long)row * stride + (vec % per_row) * 4);
         }
     }
+    if (page < 0) return;
     if (t < n_tiles) {
         const int tile = tile0 + t;
         const long long at = (long long)page * c.n_kv_head + (tile >> 1);
@@ -1123,12 +1122,21 @@ void launch_append(const g2_kv8 &c, const void *k, const void *v, long long stri
     const int per = (c.page_size + r.max_q - 2) / c.page_size + 1;   // blocks that max_q rows can touch
     const int vpt = c.page_size * c.head_dim / (4 * kAppendThreads), tiles = std::max(1, kAppendVecs / vpt);
     const dim3 grid((unsigned)per * r.n_seq, (2 * c.n_kv_head + tiles - 1) / tiles);
-    switch (vpt) {
-        case 1: kv8_append_kernel<T, FMT, 1><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
-        case 2: kv8_append_kernel<T, FMT, 2><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
-        case 4: kv8_append_kernel<T, FMT, 4><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
-        case 8: kv8_append_kernel<T, FMT, 8><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
-        default: kv8_append_kernel<T, FMT, 16><<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); break;
+    auto launch = [&](auto kernel) { kernel<<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); };
+    if (c.head_dim == 64) {
+        switch (vpt) {
+            case 1: launch(kv8_append_kernel<T, FMT, 64, 1>); break;
+            case 2: launch(kv8_append_kernel<T, FMT, 64, 2>); break;
+            case 4: launch(kv8_append_kernel<T, FMT, 64, 4>); break;
+            default: launch(kv8_append_kernel<T, FMT, 64, 8>); break;
+        }
+    } else {
+        switch (vpt) {
+            case 2: launch(kv8_append_kernel<T, FMT, 128, 2>); break;
+            case 4: launch(kv8_append_kernel<T, FMT, 128, 4>); break;
+            case 8: launch(kv8_append_kernel<T, FMT, 128, 8>); break;
+            default: launch(kv8_append_kernel<T, FMT, 128, 16>); break;
+        }
     }
 }
 
