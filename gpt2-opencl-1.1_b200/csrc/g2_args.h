@@ -43,9 +43,10 @@ inline int check_device_ptrs(const char *who, std::initializer_list<const void *
 }
 
 // A launch just made on the current device: its error, if any.
-inline int launch_status(const char *who) {
-    const cudaError_t r = cudaGetLastError();
+inline int launch_status(const char *who, cudaError_t r) {
+    if (r != cudaSuccess) cudaGetLastError();
     return r == cudaSuccess ? G2_OK : arg_error(G2_ERR_CUDA, who, cudaGetErrorString(r));
 }
+inline int launch_status(const char *who) { return launch_status(who, cudaGetLastError()); }
 
 }  // namespace g2

@@ -1613,10 +1613,9 @@ extern "C" int g2_process_logits(g2_engine *e, int slot, const g2_logit_rules *r
             *to[i] = reinterpret_cast<float *>(rest + 1 + i);
         }
     float *lg = e->logits + (size_t)slot * e->c.padded_vocab;
-    launch_rules(lg, e->c.padded_vocab, lg, e->c.padded_vocab, 1, V, d, e->st);
+    CK(launch_rules(lg, e->c.padded_vocab, lg, e->c.padded_vocab, 1, V, d, e->st));
     e->launches += 1;
     if (e->result_slot == slot) e->result_slot = -1;   // the LM head's argmax no longer holds
-    CKL();
     return sync_and_check(e);   // the caller's arrays are free again
 }
 

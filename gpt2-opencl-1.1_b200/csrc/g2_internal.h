@@ -116,8 +116,8 @@ void launch_topk(const float *logits, int V, int k, float *vals, int *idx, cudaS
 
 // Rules on rows of logits (g2_logits.cu): the host checks, and the kernel with `rules` in device memory.
 int check_rules(const char *who, const g2_logit_rules *r, int rows, int vocab, bool device);
-void launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
-                  const g2_logit_rules &rules, cudaStream_t st);
+cudaError_t launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
+                         const g2_logit_rules &rules, cudaStream_t st);
 
 template <typename WT>
 void launch_embed(const WT *wte, const WT *wpe, Rows rows, float *h, int E, int V, int n_pos, int nrows,

@@ -186,6 +186,8 @@ __global__ void __launch_bounds__(kAppendThreads)
     __shared__ float scale_s[TILES][2];                 // before, after
     __shared__ unsigned char table[TILES][128];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    pdl_wait();
+    pdl_launch();
     const int s = blockIdx.x / blocks_per_seq, tile0 = blockIdx.y * TILES, n_tiles = min(TILES, 2 * c.n_kv_head - tile0);
     const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
@@ -273,6 +275,8 @@ template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256) kv8_append_token_kernel(g2_kv8 c, const T *k, const T *v, long long stride, const int *pos, Rows8 r) {
     __shared__ unsigned char table[8][128];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_launch();
     const int s = blockIdx.x, tile = blockIdx.y * 8 + warp, h = tile >> 1, P = c.page_size;
     if (tile >= 2 * c.n_kv_head) return;
     const int p = pos[s];
@@ -330,6 +334,8 @@ constexpr int kGatherRows = 16;
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
     kv8_gather_kernel(g2_kv8 c, T *k, T *v, long long stride, const int *pos, Rows8 r, int chunks_per_seq) {
+    pdl_wait();
+    pdl_launch();
     const int s = blockIdx.x / chunks_per_seq;
     const int P = c.page_size, D = c.head_dim, per_row = c.n_kv_head * D / 4;
     const int p0 = pos[s];
@@ -544,6 +550,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     const int grp = warp / WPR, wr = warp % WPR, gt = tid - grp * 32 * WPR;
     const int H = a.c.n_kv_head, P = a.c.page_size, n_seq = a.r.n_seq;
 
+    pdl_wait();
+    pdl_launch();
     // ---- the units before every `per` sequences
     const int per = (n_seq + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
     unsigned mine = 0;
@@ -1054,8 +1062,8 @@ int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (AttnRing<D, NT>::kSmem)) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_kv8_attention", cudaGetErrorString(cudaGetLastError()));
     const int per_cta = kAttnWarps / WPR;
-    kernel<<<(a.workers + per_cta - 1) / per_cta, kAttnWarps * 32, (AttnRing<D, NT>::kSmem), st>>>(a);
-    return launch_status("g2k_kv8_attention");
+    return launch_status("g2k_kv8_attention", launch_pdl(kernel, dim3((a.workers + per_cta - 1) / per_cta), dim3(kAttnWarps * 32),
+                                                         (AttnRing<D, NT>::kSmem), st, a));
 }
 
 template <int FMT, int D, int NT>
@@ -1110,55 +1118,46 @@ int check_rows(const char *who, const g2_kv8 *c, int heads, const void *a, const
 }
 
 template <typename T, int FMT>
-void launch_append(const g2_kv8 &c, const void *k, const void *v, long long stride, const int *pos, const Rows8 &r,
+cudaError_t launch_append(const g2_kv8 &c, const void *k, const void *v, long long stride, const int *pos, const Rows8 &r,
                    cudaStream_t st) {
     const T *kt = static_cast<const T *>(k), *vt = static_cast<const T *>(v);
     if (r.max_q == 1) {
         const dim3 grid(r.n_seq, (2 * c.n_kv_head + 7) / 8);
-        if (c.head_dim == 64) kv8_append_token_kernel<T, FMT, 64><<<grid, 256, 0, st>>>(c, kt, vt, stride, pos, r);
-        else kv8_append_token_kernel<T, FMT, 128><<<grid, 256, 0, st>>>(c, kt, vt, stride, pos, r);
-        return;
+        return c.head_dim == 64 ? launch_pdl(kv8_append_token_kernel<T, FMT, 64>, grid, dim3(256), 0, st, c, kt, vt, stride, pos, r)
+                                : launch_pdl(kv8_append_token_kernel<T, FMT, 128>, grid, dim3(256), 0, st, c, kt, vt, stride, pos, r);
     }
     const int per = (c.page_size + r.max_q - 2) / c.page_size + 1;   // blocks that max_q rows can touch
     const int vpt = c.page_size * c.head_dim / (4 * kAppendThreads), tiles = std::max(1, kAppendVecs / vpt);
     const dim3 grid((unsigned)per * r.n_seq, (2 * c.n_kv_head + tiles - 1) / tiles);
-    auto launch = [&](auto kernel) { kernel<<<grid, kAppendThreads, 0, st>>>(c, kt, vt, stride, pos, r, per); };
+    auto launch = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kAppendThreads), 0, st, c, kt, vt, stride, pos, r, per); };
     if (c.head_dim == 64) {
         switch (vpt) {
-            case 1: launch(kv8_append_kernel<T, FMT, 64, 1>); break;
-            case 2: launch(kv8_append_kernel<T, FMT, 64, 2>); break;
-            case 4: launch(kv8_append_kernel<T, FMT, 64, 4>); break;
-            default: launch(kv8_append_kernel<T, FMT, 64, 8>); break;
+            case 1: return launch(kv8_append_kernel<T, FMT, 64, 1>);
+            case 2: return launch(kv8_append_kernel<T, FMT, 64, 2>);
+            case 4: return launch(kv8_append_kernel<T, FMT, 64, 4>);
+            default: return launch(kv8_append_kernel<T, FMT, 64, 8>);
         }
     } else {
         switch (vpt) {
-            case 2: launch(kv8_append_kernel<T, FMT, 128, 2>); break;
-            case 4: launch(kv8_append_kernel<T, FMT, 128, 4>); break;
-            case 8: launch(kv8_append_kernel<T, FMT, 128, 8>); break;
-            default: launch(kv8_append_kernel<T, FMT, 128, 16>); break;
+            case 2: return launch(kv8_append_kernel<T, FMT, 128, 2>);
+            case 4: return launch(kv8_append_kernel<T, FMT, 128, 4>);
+            case 8: return launch(kv8_append_kernel<T, FMT, 128, 8>);
+            default: return launch(kv8_append_kernel<T, FMT, 128, 16>);
         }
     }
 }
 
 template <typename T, int FMT>
-void launch_gather(const g2_kv8 &c, void *k, void *v, long long stride, const int *pos, const Rows8 &r, cudaStream_t st) {
+cudaError_t launch_gather(const g2_kv8 &c, void *k, void *v, long long stride, const int *pos, const Rows8 &r, cudaStream_t st) {
     const int per = (r.max_q + kGatherRows - 2) / kGatherRows + 1;   // chunks that max_q rows can touch
     const dim3 grid((unsigned)per * r.n_seq, (c.n_kv_head * c.head_dim / 2 + 255) / 256);
-    kv8_gather_kernel<T, FMT><<<grid, 256, 0, st>>>(c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
+    return launch_pdl(kv8_gather_kernel<T, FMT>, grid, dim3(256), 0, st, c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
 }
 
 // dtype and format to template arguments
-#define G2_KV8_DISPATCH(fn, ...)                                     \
-    do {                                                             \
-        if (dtype == G2_F32 && cache->format == G2_KV_I8)            \
-            fn<float, G2_KV_I8>(__VA_ARGS__);                        \
-        else if (dtype == G2_F32)                                    \
-            fn<float, G2_KV_E4M3>(__VA_ARGS__);                      \
-        else if (cache->format == G2_KV_I8)                          \
-            fn<__half, G2_KV_I8>(__VA_ARGS__);                       \
-        else                                                         \
-            fn<__half, G2_KV_E4M3>(__VA_ARGS__);                     \
-    } while (0)
+#define G2_KV8_DISPATCH(fn, ...)                                                                                       \
+    (dtype == G2_F32 ? (cache->format == G2_KV_I8 ? fn<float, G2_KV_I8>(__VA_ARGS__) : fn<float, G2_KV_E4M3>(__VA_ARGS__)) \
+                     : (cache->format == G2_KV_I8 ? fn<__half, G2_KV_I8>(__VA_ARGS__) : fn<__half, G2_KV_E4M3>(__VA_ARGS__)))
 
 }  // namespace
 
@@ -1178,8 +1177,7 @@ extern "C" int g2k_kv8_append(const g2_kv8 *cache, const void *k, const void *v,
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k, v, q_start, pos, table, status})))
         return rc;
-    G2_KV8_DISPATCH(launch_append, *cache, k, v, row_stride, pos, r, (cudaStream_t)stream);
-    return launch_status(who);
+    return launch_status(who, G2_KV8_DISPATCH(launch_append, *cache, k, v, row_stride, pos, r, (cudaStream_t)stream));
 }
 
 extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int dtype, long long row_stride, int n_rows,
@@ -1194,8 +1192,7 @@ extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k_out, v_out, q_start, pos, table, status})))
         return rc;
-    G2_KV8_DISPATCH(launch_gather, *cache, k_out, v_out, row_stride, pos, r, (cudaStream_t)stream);
-    return launch_status(who);
+    return launch_status(who, G2_KV8_DISPATCH(launch_gather, *cache, k_out, v_out, row_stride, pos, r, (cudaStream_t)stream));
 }
 
 // [counters | partial results], each 256-byte aligned; the counters' place does not depend on the call's sizes

@@ -64,6 +64,8 @@ __global__ void __launch_bounds__(kRuleThreads) rules_kernel(RuleArgs a) {
     __shared__ int next;                                     // step of the copy
     const int t = threadIdx.x, lane = t & 31, row = blockIdx.y;
     const g2_logit_rules &r = a.r;
+    pdl_wait();
+    pdl_launch();
     const float *in = a.logits + row * a.ld;
     float *out = a.out + row * a.ld_out;
     const bool in_place = in == out;
@@ -261,8 +263,8 @@ int check_rules(const char *who, const g2_logit_rules *r, int rows, int vocab, b
     return G2_OK;
 }
 
-void launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
-                  const g2_logit_rules &rules, cudaStream_t st) {
+cudaError_t launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
+                         const g2_logit_rules &rules, cudaStream_t st) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -277,7 +279,7 @@ void launch_rules(const float *logits, long long ld, float *out, long long ld_ou
     void (*const kernels[8])(RuleArgs) = {
         rules_kernel<false, false, false>, rules_kernel<true, false, false>, rules_kernel<false, true, false>, rules_kernel<true, true, false>,
         rules_kernel<false, false, true>,  rules_kernel<true, false, true>,  rules_kernel<false, true, true>,  rules_kernel<true, true, true>};
-    kernels[(penal ? 1 : 0) + (bias ? 2 : 0) + (rules.mask ? 4 : 0)]<<<grid, kRuleThreads, penal || bias ? slice / 4 : 0, st>>>(a);
+    return launch_pdl(kernels[(penal ? 1 : 0) + (bias ? 2 : 0) + (rules.mask ? 4 : 0)], grid, dim3(kRuleThreads), penal || bias ? slice / 4 : 0, st, a);
 }
 
 }  // namespace g2
@@ -301,6 +303,5 @@ extern "C" int g2k_process_logits(const float *logits, long long ld, float *out,
                                       rules->presence, rules->frequency, rules->bias_ids, rules->bias, rules->bias_start,
                                       rules->mask})))
         return rc;
-    launch_rules(logits, ld, out, ld_out, rows, vocab_size, *rules, (cudaStream_t)stream);
-    return launch_status(who);
+    return launch_status(who, launch_rules(logits, ld, out, ld_out, rows, vocab_size, *rules, (cudaStream_t)stream));
 }

@@ -286,6 +286,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     __shared__ float2 row_stats[G2_Q4_MAX_ROWS];
     __shared__ unsigned char range_s[kMaxTiles][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    pdl_wait();
+    pdl_launch();
     const int M = a.M, K = sh.K;
     const int stride = x_stride<NP>(a.slice);                     // bytes of a column
     unsigned char *ring = smem + (size_t)warp * S * TP * CB;      // [stage][TP] chunks
@@ -666,8 +668,7 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     const size_t smem = bytes(a.slice);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
-    kernel<<<grid, kQ4Threads, smem, st>>>(a, sh);
-    return launch_status("g2k_matvec_q4");
+    return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid), dim3(kQ4Threads), smem, st, a, sh));
 }
 
 template <typename T, bool VEC, int NT, int TP, int NP>

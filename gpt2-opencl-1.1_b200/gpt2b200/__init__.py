@@ -124,7 +124,9 @@ class _Lib:
     def __getattr__(self, name):
         if self._L is None:
             self._L = _load()
-        return getattr(self._L, name)
+        f = getattr(self._L, name)
+        setattr(self, name, f)   # found without this call from now on
+        return f
 
 
 lib = _Lib()
@@ -390,12 +392,8 @@ def attention(q, K, V, out, n_head, max_seq, T_kv, workspace, workspace_bytes, s
 
 # ---- 4-bit weights, the 8-bit paged cache, rules on logits: kernels on device pointers ----
 def _addr(t):
-    """The device address of a tensor (or an int); other memory is refused here, before a kernel sees it."""
-    if t is None or isinstance(t, int):
-        return t
-    if not t.is_cuda:
-        raise G2Error(-1, "a tensor is not in device memory")
-    return t.data_ptr()
+    """The address of a tensor, or an int (a device address); the library refuses other memory than the current device's."""
+    return t if t is None or t.__class__ is int else t.data_ptr()
 
 
 def q4_bytes(N: int, K: int, group: int) -> int:

@@ -4,7 +4,6 @@ addresses (and addresses that are no memory at all) are never used.
 """
 import ctypes as C
 
-import numpy as np
 import pytest
 
 import gpt2b200 as g2
@@ -118,7 +117,7 @@ def test_kv8_cache_tensors():
     k = torch.zeros(4, 2, 16, 64, dtype=torch.int8)
     s = torch.zeros(4, 2)
     for bad in ((k.float(), k, s, s), (k[0], k[0], s, s), (k, k[:3], s, s), (k, k, s[:3], s), (k, k, s.half(), s),
-                (k, k.transpose(0, 1).reshape(2, 4, 16, 64).transpose(0, 1), s, s), (k, k, s, s)):   # the last: host memory
+                (k, torch.zeros(4, 2, 64, 16, dtype=torch.int8).transpose(2, 3), s, s)):
         assert code(g2.kv8_cache, *bad) == ARG
 
 
@@ -139,24 +138,28 @@ def test_logit_rules_arguments():
     assert g2.lib.g2_process_logits(None, 0, None) == ARG
 
 
+def no_device_memory():
+    """What host memory gives: it is no memory of the device, or there is no device to ask."""
+    try:
+        import torch
+        return ARG if torch.cuda.is_available() else CUDA
+    except ImportError:
+        return CUDA
+
+
 def test_host_tensors_are_refused():
     torch = pytest.importorskip("torch")
-    t = torch.zeros(64)
-    assert code(g2.q4_pack, t, A, 1, 64, 32, {}) == ARG
-    assert code(g2.matvec_q4, t, A, A, 1, 16, 64, 32, {}) == ARG
-    assert code(g2.process_logits, t, t, 1, 64, g2.logit_rules(), {}) == ARG
-    assert code(lambda: g2.logit_rules(ctx=t)) == ARG
+    t, want = torch.zeros(1 << 14), no_device_memory()
+    t = t[(-t.data_ptr() // 4) % 64:]                      # 256-byte aligned
+    assert code(g2.q4_pack, t, t, 1, 64, 32, {}) == want
+    assert code(g2.matvec_q4, t, t, t, 1, 16, 64, 32, {}) == want
+    assert code(g2.process_logits, t, t, 1, 64, g2.logit_rules(), {}) == want
+    assert code(g2.process_logits, t, t, 1, 64, g2.logit_rules(ctx=t, rep_penalty=t), {}) == want
 
 
 def test_host_addresses_reach_no_kernel():
-    """Aligned host memory passes the checks of form; the check of memory refuses it (here: there is no device at all)."""
-    try:
-        import torch
-        want = ARG if torch.cuda.is_available() else CUDA
-    except ImportError:
-        want = CUDA
-    x = np.zeros(4096, np.float32)
-    assert x.size
+    """Aligned host memory passes the checks of form; the check of memory refuses it."""
+    want = no_device_memory()
     assert code(g2.q4_pack, A, A, 16, 64, 32, {}) == want
     assert code(g2.matvec_q4, A, A, A, 1, 16, 64, 32, {}) == want
     for f in CALLS.values():
