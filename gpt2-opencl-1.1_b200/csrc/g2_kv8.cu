@@ -389,12 +389,13 @@ __global__ void __launch_bounds__(256)
 //
 // A *run* is the keys of one sequence under one K/V head for a group of up to
 // 4 NT query columns (column c of a sequence: row c / group, head c % group).
-// Runs are cut into units of `unit` keys; all units, in order, are shared
-// equally among the workers (WPR warps each), so the shares do not depend on
-// how ragged the sequences are.  Beginning a run costs as much as several units,
-// so each counts as `ahead` more, which hold no keys.  A run that crosses shares leaves partial
-// results (m, sum, accumulators) in the workspace; the last worker to arrive
-// merges them in order, so results do not depend on timing.
+// Workers (WPR warps each) take whole runs where there are no more runs than workers
+// and the longest is hardly longer than an equal share.  Else runs are cut into
+// units of `unit` keys, and all units, in order, are shared equally, so the shares
+// do not depend on how ragged the sequences are.  Beginning a run costs as much as
+// several units, so each counts as `ahead` more, which hold no keys.  A run that
+// crosses shares leaves partial results (m, sum, accumulators) in the workspace;
+// the last worker to arrive merges them in order, so results do not depend on timing.
 //
 // A warp takes tiles of 16 keys.  Each tile's codes and scales are copied by
 // cp.async into the warp's own ring of kStages slots, so that the copies of the
@@ -511,7 +512,7 @@ __device__ __forceinline__ void group_sync(int group) {
 // Units of sequence s (0 where it has no rows or is out of range).
 struct SeqWork {
     int first, n, len, units, col_groups;
-    unsigned total;
+    unsigned runs, total;    // total: units of its runs
 };
 template <int COLS>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
@@ -528,7 +529,8 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
     }
     w.units = max(1, (w.len + a.unit - 1) / a.unit) + a.ahead;   // a row that sees nothing is still written
     w.col_groups = (w.n * a.group + COLS - 1) / COLS;
-    w.total = (unsigned)w.units * w.col_groups * a.c.n_kv_head;   // below 2^31 over all sequences: checked on the host
+    w.runs = (unsigned)w.col_groups * a.c.n_kv_head;
+    w.total = (unsigned)w.units * w.runs;   // below 2^31 over all sequences: checked on the host
     return w;
 }
 
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     static_assert(WPR * PART * 4 <= WPR * S * TILE, "the merge buffer lies in the ring");
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ unsigned prefix[kAttnWarps * 32];
-    __shared__ unsigned warp_sum[kAttnWarps];
+    __shared__ uint4 warp_sum[kAttnWarps];        // units, runs, longest sequence
     __shared__ int arrived[GROUPS];
     __shared__ SeqWork cached[kAttnWarps * 32];   // of the first sequences
     __shared__ float qfac_s[GROUPS][COLS];        // scores' factor of each query column
@@ -554,31 +556,43 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     pdl_launch();
     // ---- the units before every `per` sequences
     const int per = (n_seq + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
-    unsigned mine = 0;
-    if (per == 1) {
-        if (tid < n_seq) {
-            cached[tid] = seq_work<COLS>(a, tid);
-            mine = cached[tid].total;
-        }
-    } else {
-        for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) mine += seq_work<COLS>(a, s).total;
+    unsigned my_units = 0, my_runs = 0, longest = 0;
+    for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) {
+        const SeqWork w = seq_work<COLS>(a, s);
+        if (per == 1) cached[tid] = w;
+        my_units += w.total;
+        my_runs += w.runs;
+        if (w.runs) longest = max(longest, (unsigned)w.len);
     }
+    {
+        const uint4 x = make_uint4(__reduce_add_sync(0xffffffffu, my_units), __reduce_add_sync(0xffffffffu, my_runs),
+                                   __reduce_max_sync(0xffffffffu, longest), 0);
+        if (lane == 0) warp_sum[warp] = x;
+    }
+    __syncthreads();
+    uint4 before = make_uint4(0, 0, 0, 0), all = before;
+#pragma unroll
+    for (int i = 0; i < kAttnWarps; ++i) {
+        const uint4 x = warp_sum[i];
+        if (i < warp) before = make_uint4(before.x + x.x, before.y + x.y, 0, 0);
+        all = make_uint4(all.x + x.x, all.y + x.y, max(all.z, x.z), 0);
+    }
+    // Whole runs: the longest takes longest / (16 WPR) steps of a worker.  Equal shares are shorter, but partial
+    // results and second beginnings cost about kSplitSteps (12 runs of 200 keys: whole 5.2 us, shared 6.5;
+    // 12 runs of 1000 keys: whole 8.0, shared 6.7).
+    constexpr unsigned kSplitSteps = 4;
+    const bool by_run = all.y <= (unsigned)a.workers &&
+                        all.z / (16 * WPR) <= (unsigned)((float)all.x * a.unit / (16.0f * WPR * a.workers)) + kSplitSteps;
+    const unsigned total = by_run ? all.y : all.x;
+    const int unit_keys = by_run ? 1 << 30 : a.unit, ahead = by_run ? 0 : a.ahead;
+    const unsigned mine = by_run ? my_runs : my_units;
     unsigned sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += x;
     }
-    if (lane == 31) warp_sum[warp] = sum;
-    __syncthreads();
-    unsigned before = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kAttnWarps; ++i) {
-        const unsigned x = warp_sum[i];
-        before += i < warp ? x : 0;
-        total += x;
-    }
-    prefix[tid] = before + sum - mine;
+    prefix[tid] = (by_run ? before.y : before.x) + sum - mine;
     __syncthreads();
     const unsigned W = min((unsigned)a.workers, total);
     const unsigned worker = blockIdx.x * GROUPS + grp;
@@ -591,7 +605,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     };
     unsigned u = share_begin(worker);
     const unsigned u_end = share_begin(worker + 1);
-    auto work_of = [&](int s) { return per == 1 ? cached[s] : seq_work<COLS>(a, s); };
+    auto work_of = [&](int s) {
+        SeqWork w = per == 1 ? cached[s] : seq_work<COLS>(a, s);
+        if (by_run) {
+            w.units = w.runs ? 1 : 0;
+            w.total = w.runs;
+        }
+        return w;
+    };
 
     // ---- the share's first sequence: the last whose units begin at or before u
     int s;
@@ -630,7 +651,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         const int h = run / sw.col_groups, col0 = run % sw.col_groups * COLS;
         const unsigned run_begin = u - unit, piece_end = min(run_begin + sw.units, u_end);
         // units with keys that are this piece's; the run's first ones may all lie in the next share
-        const int unit0 = max(unit - a.ahead, 0), unit1 = (int)(piece_end - run_begin) - a.ahead;
+        const int unit0 = max(unit - ahead, 0), unit1 = (int)(piece_end - run_begin) - ahead;
         if (unit1 <= 0) break;
         const int cols = min(COLS, sw.n * a.group - col0);
         // key limits of the columns; `lim` of this thread's (column t of each n tile)
@@ -641,8 +662,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             const int col = col0 + n * 4 + t;
             lim[n] = n * 4 + t < cols ? sw.len - sw.n + col / a.group + 1 : 0;
         }
-        const int kbeg = unit0 * a.unit;
-        const int kend = (int)min((long long)min(sw.len, lim_last), (long long)unit1 * a.unit);
+        const int kbeg = unit0 * unit_keys;
+        const int kend = (int)min((long long)min(sw.len, lim_last), (long long)unit1 * unit_keys);
         const int n_tiles = kend > kbeg ? (kend - kbeg + 15) / 16 : 0;
         const int my_tiles = n_tiles > wr ? (n_tiles - wr + WPR - 1) / WPR : 0;
         const int *table = a.r.table + (long long)s * a.r.table_stride;
@@ -928,7 +949,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         }
         group_sync<WPR>(grp);
 
-        const bool whole = unit0 == 0 && unit1 == sw.units - a.ahead;
+        const bool whole = unit0 == 0 && unit1 == sw.units - ahead;
         float *part = a.parts + ((size_t)worker * 2 + (first_piece ? 0 : 1)) * PART;
         auto store = [&](int i, float v) {
             const int c = i / D, d = i % D, col = col0 + c, row = col / a.group;
@@ -958,7 +979,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             }
         }
         if (!whole) {
-            const unsigned w0 = worker_of(run_begin + a.ahead), w1 = worker_of(run_begin + sw.units - 1);
+            const unsigned w0 = worker_of(run_begin + ahead), w1 = worker_of(run_begin + sw.units - 1);
             group_sync<WPR>(grp);
             if (gt == 0) {   // releases the group's results and acquires the others'
                 unsigned seen;
