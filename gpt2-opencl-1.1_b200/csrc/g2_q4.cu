@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 //           instructions.  Up to 4 rows (2 of fp16).
 //   NP = 2  fp16: the rounding of x (after a power of two has brought the row's
 //           largest below 2) and 2^11 times the rest, 22 bits in all.  Eight codes
-//           cost nine instructions.  More than 4 rows.
+//           cost nine instructions.  More than 4 rows, eight at a time.
 //   NP = 1  fp16 x as it is.  More than 2 rows.
 // A group's sum is scaled once, in fp32.
 //
@@ -165,7 +165,7 @@ constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
 // One stage: a chunk of each of TP feature tiles.
 template <int NT, int TP>
 struct Q4Ring {
-    static constexpr int kStages = TP == 1 ? 8 : NT == 4 ? 4 : 5;
+    static constexpr int kStages = TP == 1 ? 8 : NT > 1 ? 4 : 5;
 };
 
 struct Q4Args {
@@ -279,7 +279,7 @@ template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
     constexpr int S = Q4Ring<NT, TP>::kStages, CB = 512 + 32 * PC;
     constexpr bool INT = NP == 4;
-    constexpr int kHeld = INT ? 4 : NT == 4 ? 13 : 8;             // groups of four x that a thread reads once
+    constexpr int kHeld = INT ? 4 : 8;             // groups of four x that a thread reads once
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[kQ4Warps], squares[kQ4Warps], up_s[G2_Q4_MAX_ROWS];
     __shared__ unsigned peaks[kQ4Warps];
@@ -288,7 +288,11 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch();
-    const int M = a.M, K = sh.K;
+    constexpr int kMost = 8 * NT / NP;                            // rows of x that the columns hold; others are other CTAs'
+    const int row0 = blockIdx.y * kMost, M = min(kMost, a.M - row0), K = sh.K;
+    const T *x_rows = static_cast<const T *>(a.x) + (size_t)row0 * K;
+    const T *residual = a.residual ? static_cast<const T *>(a.residual) + (size_t)row0 * sh.N : nullptr;
+    T *y = static_cast<T *>(a.y) + (size_t)row0 * sh.N;
     const int stride = x_stride<NP>(a.slice);                     // bytes of a column
     unsigned char *ring = smem + (size_t)warp * S * TP * CB;      // [stage][TP] chunks
     unsigned char *xs = smem + (size_t)kQ4Warps * S * TP * CB;    // [8 NT][stride]
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                 for (int i = tid; i < M * per_row; i += kQ4Threads) {
                     const int m = i / per_row, k = i % per_row * 8, left = K - c0 * kChunk - k;
                     cp_async16(smem_addr(xs + m * stride + 2 * k),
-                               static_cast<const __half *>(a.x) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
+                               reinterpret_cast<const __half *>(x_rows) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
                 }
             }
             cp_commit();
@@ -353,7 +357,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                 for (int r0 = 0; r0 < M; r0 += rows_at_once) {    // columns past M rows keep what they hold
                     const int m = r0 + warp / wpr;
                     const bool live = m < M;
-                    const T *row = static_cast<const T *>(a.x) + (size_t)(live ? m : 0) * K;
+                    const T *row = x_rows + (size_t)(live ? m : 0) * K;
                     if (NP == 1) {
                         for (int k = live ? first : kn; k < kn; k += step) {
                             const float4 v = load_4<VEC>(row, k0 + k, K);
@@ -612,27 +616,41 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             __syncthreads();
 
             // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
-            constexpr int kPer = 2 / TP;                          // (row, tile) pairs of a warp: 32 features of one, 16 of two
-            const int f = lane % (16 * TP);
-            int m = 0, rr = warp * kPer + lane / (16 * TP);
+            // (four rows, a tile) at a time: 32 features of one item, or 16 of two, a warp
+            constexpr int kPer = 2 / TP, kRows = NP == 4 ? 1 : 4;
+            const int f = lane % (16 * TP), row_groups = (M + kRows - 1) / kRows;
+            int mg = 0, rr = warp * kPer + lane / (16 * TP);
             for (;; rr += kQ4Warps * kPer) {
-                for (; rr >= R && m < M; rr -= R) ++m;
-                if (m >= M) break;
-                const int o = (m * R + rr) * 16 * TP + f, n = (tile + rr) * 16 * TP + f;
-                const size_t at = (size_t)m * sh.N + n;
+                for (; rr >= R && mg < row_groups; rr -= R) ++mg;
+                if (mg >= row_groups) break;
+                const int n = (tile + rr) * 16 * TP + f, m0 = mg * kRows, wa = range_s[rr][0], wb = range_s[rr][1];
                 const bool last = c0 + nc == sh.chunks, there = last && n < sh.N;
                 const float bias = there && a.bias ? a.bias[n] : 0.0f;
-                const float res = there && a.residual ? tof(static_cast<const T *>(a.residual)[at]) : 0.0f;
-                float v = 0.0f;
-                for (int x = range_s[rr][0]; x <= range_s[rr][1]; ++x) v += pieces[((rr + x) * M + m) * 16 * TP + f];
-                if (NP > 1) v *= up_s[m];
-                if (c0 > 0) v += total[o];
-                if (!last) total[o] = v;
-                if (there) {
-                    v += bias;
-                    if (a.gelu) v = gelu_f(v);
-                    if (a.residual) v += res;
-                    static_cast<T *>(a.y)[at] = fromf<T>(v);
+                float v[kRows], res[kRows];
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    v[j] = 0.0f;
+                    res[j] = there && residual && m0 + j < M ? tof(residual[(size_t)(m0 + j) * sh.N + n]) : 0.0f;
+                }
+                const float *o = pieces + ((rr + wa) * M + m0) * 16 * TP + f;
+                for (int x = wa; x <= wb; ++x, o += M * 16 * TP)
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j)
+                        if (kRows == 1 || m0 + j < M) v[j] += o[j * 16 * TP];
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    const int m = m0 + j;
+                    if (m >= M) break;
+                    float *so_far = total + (m * R + rr) * 16 * TP + f;
+                    if (NP > 1) v[j] *= up_s[m];
+                    if (c0 > 0) v[j] += *so_far;
+                    if (!last) *so_far = v[j];
+                    if (there) {
+                        v[j] += bias;
+                        if (a.gelu) v[j] = gelu_f(v[j]);
+                        if (residual) v[j] += res[j];
+                        y[(size_t)m * sh.N + n] = fromf<T>(v[j]);
+                    }
                 }
             }
             __syncthreads();
@@ -655,7 +673,7 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     a.extra = ntiles % grid;
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
     // x in equal slices that fit beside the ring and the sums
-    const size_t ring = (size_t)kQ4Warps * Q4Ring<NT, TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)a.M * 16 * TP * 4;
+    const size_t ring = (size_t)kQ4Warps * Q4Ring<NT, TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)std::min(a.M, 8 * NT / NP) * 16 * TP * 4;
     size_t sums = (a.most + kQ4Warps) * tile;
     auto bytes = [&](int slice) { return ring + (size_t)8 * NT * x_stride<NP>(slice) + sums; };
     a.slice = sh.chunks;
@@ -668,7 +686,7 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     const size_t smem = bytes(a.slice);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
-    return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid), dim3(kQ4Threads), smem, st, a, sh));
+    return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid, (a.M + 8 * NT / NP - 1) / (8 * NT / NP)), dim3(kQ4Threads), smem, st, a, sh));
 }
 
 template <typename T, bool VEC, int NT, int TP, int NP>
@@ -687,7 +705,9 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     if (a.M <= 4) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
     if constexpr (sizeof(T) == 2)
         if (!a.gamma && a.M > 8) return launch_q4<T, VEC, 2, 2, 1>(a, sh, st);
-    return a.M <= 8 ? launch_q4<T, VEC, 2, 2, 2>(a, sh, st) : launch_q4<T, VEC, 4, 2, 2>(a, sh, st);
+    // eight rows at a time: sixteen would leave room for half as much of x at once (16 rows of 8192 x 28672:
+    // 112 us instead of 162) and spill registers
+    return launch_q4<T, VEC, 2, 2, 2>(a, sh, st);
 }
 
 bool bad_shape(int N, int K, int group) {
