@@ -684,7 +684,8 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
         a.slice = (sh.chunks + slices - 1) / slices;
     }
     const size_t smem = bytes(a.slice);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    // the most that any call uses, so that calls from several host threads do not undo each other's
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4Smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
     return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid, (a.M + 8 * NT / NP - 1) / (8 * NT / NP)), dim3(kQ4Threads), smem, st, a, sh));
 }

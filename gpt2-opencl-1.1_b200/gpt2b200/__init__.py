@@ -396,6 +396,15 @@ def _addr(t):
     return t if t is None or t.__class__ is int else t.data_ptr()
 
 
+def _sized(t, size):
+    """_addr of a tensor whose elements have `size` bytes: a tensor of another type would be read past its end."""
+    if t is None or t.__class__ is int:
+        return t
+    if t.element_size() != size:
+        raise G2Error(-1, f"a tensor has elements of {t.element_size()} bytes, not {size}")
+    return t.data_ptr()
+
+
 def q4_bytes(N: int, K: int, group: int) -> int:
     """Bytes of a [K, N] weight matrix packed in 4 bits (0 for a bad shape or group)."""
     return lib.g2k_q4_bytes(N, K, group)
@@ -403,19 +412,20 @@ def q4_bytes(N: int, K: int, group: int) -> int:
 
 def q4_pack(W, packed, N, K, group, transposed=False, dtype=G2_F32, stream=0):
     """Quantise W ([K, N], or [N, K] if transposed) to 4 bits with a scale for each `group` rows of a column."""
-    check(lib.g2k_q4_pack(_addr(W), dtype, int(transposed), _addr(packed), N, K, group, stream))
+    check(lib.g2k_q4_pack(_sized(W, 2 if dtype else 4), dtype, int(transposed), _addr(packed), N, K, group, stream))
 
 
 def q4_unpack(packed, W, N, K, group, stream=0):
     """The values of a packed matrix, fp32 [K, N]."""
-    check(lib.g2k_q4_unpack(_addr(packed), _addr(W), N, K, group, stream))
+    check(lib.g2k_q4_unpack(_addr(packed), _sized(W, 4), N, K, group, stream))
 
 
 def matvec_q4(x, packed, y, M, N, K, group, bias=None, residual=None, gelu=False, ln_gamma=None, ln_beta=None,
               dtype=G2_F32, stream=0):
     """y [M, N] = x' [M, K] times a packed [K, N] matrix; M up to 16 rows; x, residual and y of `dtype`."""
-    check(lib.g2k_matvec_q4(_addr(x), _addr(packed), _addr(bias), _addr(residual), _addr(y), dtype, M, N, K, group,
-                            int(gelu), _addr(ln_gamma), _addr(ln_beta), stream))
+    e = 2 if dtype else 4
+    check(lib.g2k_matvec_q4(_sized(x, e), _addr(packed), _sized(bias, 4), _sized(residual, e), _sized(y, e), dtype, M, N, K,
+                            group, int(gelu), _sized(ln_gamma, 4), _sized(ln_beta, 4), stream))
 
 
 def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
@@ -437,15 +447,17 @@ def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
 def kv8_append(cache, k, v, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0, dtype=G2_F32,
                status=None, stream=0):
     """Write K and V rows of new tokens into the pages of their sequences (g2k_kv8_append)."""
-    check(lib.g2k_kv8_append(C.byref(cache), _addr(k), _addr(v), dtype, row_stride, n_rows, n_seq, _addr(q_start),
-                             _addr(pos), max_q, _addr(table), table_stride, _addr(status), stream))
+    e = 2 if dtype else 4
+    check(lib.g2k_kv8_append(C.byref(cache), _sized(k, e), _sized(v, e), dtype, row_stride, n_rows, n_seq, _sized(q_start, 4),
+                             _sized(pos, 4), max_q, _sized(table, 4), table_stride, _sized(status, 4), stream))
 
 
 def kv8_gather(cache, k_out, v_out, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0,
                dtype=G2_F32, status=None, stream=0):
     """Read rows of the cache back as values (g2k_kv8_gather)."""
-    check(lib.g2k_kv8_gather(C.byref(cache), _addr(k_out), _addr(v_out), dtype, row_stride, n_rows, n_seq, _addr(q_start),
-                             _addr(pos), max_q, _addr(table), table_stride, _addr(status), stream))
+    e = 2 if dtype else 4
+    check(lib.g2k_kv8_gather(C.byref(cache), _sized(k_out, e), _sized(v_out, e), dtype, row_stride, n_rows, n_seq,
+                             _sized(q_start, 4), _sized(pos, 4), max_q, _sized(table, 4), table_stride, _sized(status, 4), stream))
 
 
 def kv8_attention_workspace(cache, n_head: int, n_seq: int, max_q: int = 1) -> int:
@@ -455,23 +467,26 @@ def kv8_attention_workspace(cache, n_head: int, n_seq: int, max_q: int = 1) -> i
 def kv8_attention(cache, q, out, n_head, n_rows, n_seq, table, table_stride, seq_len, workspace, workspace_bytes,
                   q_start=None, max_q=1, scale=None, q_stride=0, out_stride=0, dtype=G2_F32, status=None, stream=0):
     """Softmax attention of query rows over the cache (g2k_kv8_attention); scale defaults to head_dim ** -0.5."""
-    check(lib.g2k_kv8_attention(C.byref(cache), _addr(q), q_stride, _addr(out), out_stride, dtype, n_head,
-                                cache.head_dim ** -0.5 if scale is None else scale, n_rows, n_seq, _addr(q_start),
-                                _addr(seq_len), max_q, _addr(table), table_stride, _addr(workspace), workspace_bytes,
-                                _addr(status), stream))
+    e = 2 if dtype else 4
+    check(lib.g2k_kv8_attention(C.byref(cache), _sized(q, e), q_stride, _sized(out, e), out_stride, dtype, n_head,
+                                cache.head_dim ** -0.5 if scale is None else scale, n_rows, n_seq, _sized(q_start, 4),
+                                _sized(seq_len, 4), max_q, _sized(table, 4), table_stride, _addr(workspace), workspace_bytes,
+                                _sized(status, 4), stream))
 
 
 def logit_rules(ctx=None, ctx_start=None, n_prompt=None, rep_penalty=None, presence=None, frequency=None, bias_ids=None,
                 bias=None, bias_start=None, mask=None, mask_stride=0) -> LogitRules:
     """Rules on rows of logits over the caller's device tensors (g2_logit_rules), which it keeps alive."""
-    r = LogitRules(_addr(ctx), _addr(ctx_start), _addr(n_prompt), 0 if ctx is None else ctx.numel(), _addr(rep_penalty),
-                   _addr(presence), _addr(frequency), _addr(bias_ids), _addr(bias), _addr(bias_start),
-                   0 if bias is None else bias.numel(), _addr(mask), mask_stride)
-    r.tensors = (ctx, ctx_start, n_prompt, rep_penalty, presence, frequency, bias_ids, bias, bias_start, mask)
+    arrays = (ctx, ctx_start, n_prompt, rep_penalty, presence, frequency, bias_ids, bias, bias_start, mask)
+    if bias is not None and (bias_ids is None or bias_ids.numel() != bias.numel()):
+        raise G2Error(-1, "bias_ids and bias are not of one length")
+    p = [_sized(t, 4) for t in arrays]
+    r = LogitRules(*p[:3], 0 if ctx is None else ctx.numel(), *p[3:9], 0 if bias is None else bias.numel(), p[9], mask_stride)
+    r.tensors = arrays
     return r
 
 
 def process_logits(logits, out, rows, vocab_size, rules, ld=0, ld_out=0, stream=0):
     """Apply `rules` to rows of logits (out may be logits); a row stride of 0 means vocab_size."""
-    check(lib.g2k_process_logits(_addr(logits), ld or vocab_size, _addr(out), ld_out or vocab_size, rows, vocab_size,
+    check(lib.g2k_process_logits(_sized(logits, 4), ld or vocab_size, _sized(out, 4), ld_out or vocab_size, rows, vocab_size,
                                  C.byref(rules), stream))

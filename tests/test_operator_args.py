@@ -165,3 +165,21 @@ def test_host_addresses_reach_no_kernel():
     for f in CALLS.values():
         assert code(lambda: f(cache(), {})) == want
     assert code(lambda: g2.process_logits(A, A, 1, 100, g2.LogitRules(ctx=A, n_ctx=3))) == want
+
+
+def test_tensors_of_another_type():
+    """A tensor whose elements are not of the stated size is refused: it would be read past its end."""
+    torch = pytest.importorskip("torch")
+    f, h, i64 = torch.zeros(4096), torch.zeros(4096, dtype=torch.half), torch.zeros(4096, dtype=torch.int64)
+    assert code(g2.q4_pack, h, A, 16, 64, 32, {}) == ARG
+    assert code(g2.q4_pack, f, A, 16, 64, 32, dict(dtype=g2.G2_F16)) == ARG
+    assert code(g2.q4_unpack, A, h, 16, 64, 32) == ARG
+    for bad in (dict(x=h), dict(y=h), dict(residual=h), dict(bias=h), dict(ln_gamma=h, ln_beta=h), dict(x=f, dtype=1)):
+        k = dict(bad)
+        assert code(g2.matvec_q4, k.pop("x", A), A, k.pop("y", A), 1, 16, 64, 32, k) == ARG, bad
+    for name, f8 in CALLS.items():
+        for bad in (dict(a=h), dict(b=h), dict(a=f, dtype=1), dict(table=i64), dict(per=i64), dict(status=i64), dict(q_start=i64, max_q=2)):
+            assert code(lambda: f8(cache(), dict(bad))) == ARG, (name, bad)
+    for bad in (dict(ctx=i64), dict(mask=i64), dict(rep_penalty=h), dict(bias=f, bias_ids=i64), dict(bias=f), dict(bias=f, bias_ids=f[:5])):
+        assert code(lambda: g2.logit_rules(**bad)) == ARG, bad
+    assert code(g2.process_logits, h, h, 1, 64, g2.logit_rules(), {}) == ARG
