@@ -698,16 +698,19 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
 template <typename T, bool VEC>
 int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
-    // matrices of fewer pairs than SMs (and few rows) are better spread one by one.
-    const bool one = sh.tiles / 2 < q4_sms();
+    // matrices of fewer pairs than SMs are better spread one by one.
+    const int sms = q4_sms();
+    const bool one = sh.tiles / 2 < sms;
+    // Rows in groups of 2, 4 or 8: the fewest that one CTA per SM still holds, since staging x is most of a
+    // narrow matrix's time (16 rows of 3974 x 83: 27 us in groups of 8, 7.4 in groups of 2), else as few groups as can be.
+    const auto fits = [&](int rows) { return sh.tiles * ((a.M + rows - 1) / rows) <= sms; };
     if constexpr (sizeof(T) == 2)
-        if (!a.gamma && a.M > 2 && a.M <= 8) return one ? launch_q4<T, VEC, 1, 1, 1>(a, sh, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, st);
-    if (a.M <= 2) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
-    if (a.M <= 4) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
-    if constexpr (sizeof(T) == 2)
-        if (!a.gamma && a.M > 8) return launch_q4<T, VEC, 2, 2, 1>(a, sh, st);
-    // eight rows at a time: sixteen would leave room for half as much of x at once (16 rows of 8192 x 28672:
-    // 112 us instead of 162) and spill registers
+        if (!a.gamma && a.M > 2 && !(a.M > 8 && fits(2)))
+            return a.M > 8 ? launch_q4<T, VEC, 2, 2, 1>(a, sh, st) : one ? launch_q4<T, VEC, 1, 1, 1>(a, sh, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, st);
+    if (a.M <= 2 || fits(2)) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
+    if (a.M <= 4 || fits(4)) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
+    // sixteen rows at once would leave room for half as much of x and spill registers (16 rows of
+    // 8192 x 28672: 108 us in groups of eight, 162 together)
     return launch_q4<T, VEC, 2, 2, 2>(a, sh, st);
 }
 
