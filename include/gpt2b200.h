@@ -254,10 +254,12 @@ int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *s
  * y[m][n] = sum_k x'[m][k] * W[k][n] (+bias[n]) (then GELU) (+residual[m][n]),
  * x' = LayerNorm(x; ln_gamma, ln_beta, eps 1e-5) when ln_gamma is not NULL.
  * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
- * ln_gamma and ln_beta are fp32.  Sums are fp32; with G2_F32 the operands
- * carry 22 bits of each x', with G2_F16 too after a LayerNorm, else x exactly.
- * residual may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls on
- * different streams may overlap. */
+ * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32;
+ * an x' is carried to 2^-30 of its row's largest or to 2^-22 of itself,
+ * whichever serves the shape, an fp16 x of three rows or more exactly.  A
+ * non-finite x' makes its row's outputs non-finite, and no other's.  residual
+ * may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls on different
+ * streams may overlap. */
 #define G2_Q4_MAX_ROWS 16
 #define G2_Q4_MAX_K 32768
 int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const void *residual, void *y, int dtype,
@@ -282,7 +284,10 @@ int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const vo
  * A sequence with a count outside [0, max_q], rows outside [0, n_rows), or a
  * position or length outside its table row is skipped, and so is a page whose
  * id is outside [0, n_pages); *status (may be NULL) then becomes G2_ERR_RANGE.
- * It is never cleared here. */
+ * It is never cleared here.
+ *
+ * Codes of rows in use are finite and scales positive or NaN; what other rows and
+ * pages hold does not matter.  Attention counts scales of V below 2^-64 as 2^-64. */
 #define G2_KV_I8 0      /* int8 codes in -127..127 */
 #define G2_KV_E4M3 1    /* fp8 e4m3 codes, finite, up to 448 */
 typedef struct g2_kv8 {

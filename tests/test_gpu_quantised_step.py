@@ -113,7 +113,7 @@ class Model:
         return self.wte[tokens.long()] + self.wpe[self.pos.long()]
 
 
-def checker(m):
+def comparer(m):
     def see(name, *a):
         torch.cuda.synchronize()
         assert int(m.status) == 0
@@ -152,7 +152,7 @@ def run(m, steps, graph=False, check=False):
     m.len.fill_(1)
     m.made.zero_()
     token = torch.tensor([11, 300, 777], device="cuda")
-    see = checker(m) if check else None
+    see = comparer(m) if check else None
     exec_ = None
     if graph:
         exec_ = torch.cuda.CUDAGraph()
