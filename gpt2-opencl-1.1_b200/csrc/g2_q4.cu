@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     for (int k = first + kHeld * step; k < kn; k += step) larger(value(k));
                     if (wpr > 1 && r0) __syncthreads();           // the last rows' peaks have been read
                     peak = row_largest(peak, peaks, w0, wpr);
-                    // 2^e <= the largest < 2^(e + 1); INT: 29 bits below it, and the codes are 16 times theirs
-                    const int e = max(INT ? -96 : -126, min(126, (int)(peak >> 23) - 127)), bits_down = INT ? 29 : 0;
+                    // 2^e <= the largest < 2^(e + 1) (fp16 parts: up to 4 times 2^e); INT: 29 bits below it, and the codes are 16 times theirs
+                    const int e = max(INT ? -96 : -126, min(INT ? 127 : 126, (int)(peak >> 23) - 127)), bits_down = INT ? 29 : 0;
                     const float down = __uint_as_float((unsigned)(127 + bits_down - e) << 23);
                     if (live && first == 0)
                         up_s[m] = INT && peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u)

@@ -174,6 +174,21 @@ def test_scale_of_x(g2, size):
     assert (y[3] == 0).all()
 
 
+@pytest.mark.parametrize("M", [1, 3, 5])
+def test_largest_x(g2, M):
+    """Values in fp32's last power of two, 2^127 and above."""
+    K, N = 200, 96
+    x = torch.randn(M, K, device="cuda", generator=gen(18)) * 1e38
+    x[:, 3], x[:, 100], x[:, 150] = 3.4e38, -3.2e38, 2.0 ** 127
+    x = x.clamp(-3.4e38, 3.4e38)
+    W = torch.randn(K, N, device="cuda", generator=gen(19)) * 1e-4
+    y = torch.empty(M, N, device="cuda")
+    g2.matvec_q4(x, pack(g2, W, 64), y, M, N, K, 64)
+    want = x.double() @ quantise(W, 64)
+    S = x.double().abs() @ quantise(W, 64).abs()
+    assert ((y.double() - want).abs() <= (K / 16 + 16) * 2 ** -22 * S).all()
+
+
 def test_non_finite_rows_stay_apart(g2):
     """A NaN or infinity in one row reaches that row's outputs and no other's."""
     x = torch.randn(3, 256, device="cuda", generator=gen(11))
