@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             const int d = lane * 4;
             const unsigned peak = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
             // a power of two below the largest (2^e <= it < 2^(e + 1)), so that no type's range matters
-            const int e = max(INT ? -96 : -126, min(126, (int)(peak >> 23) - 127));
+            const int e = max(INT ? -96 : -126, min(INT ? 127 : 126, (int)(peak >> 23) - 127));   // fp16 parts may reach 4
             const float down = __uint_as_float((unsigned)(127 + (INT ? 29 : 0) - e) << 23);
             const float up = __uint_as_float((unsigned)(127 + e) << 23) * (INT ? 0x1p-29f : 1.0f);
             if (lane == 0) qfac_s[grp][c] = (peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : up) * a.scale_log2e;

@@ -439,6 +439,28 @@ def test_attention_large_q(g2):
     check_attention(g2, cache, [1], [100], table, q_size=3e5, scale=1e-6)
 
 
+def attend(g2, cache, q, lens, table, scale):
+    """One query row a sequence, fp32."""
+    n, Hq, _ = q.shape
+    out = torch.empty_like(q)
+    ws = torch.zeros(g2.kv8_attention_workspace(cache.h, Hq, n, 1), dtype=torch.uint8, device="cuda")
+    g2.kv8_attention(cache.h, q, out, Hq, n, n, table, table.shape[1], ints(lens), ws, ws.numel(), scale=scale)
+    return out
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_attention_largest_q(g2, fmt):
+    """Queries in fp32's last power of two, 2^127 and above."""
+    n, table = tables(1, 4)
+    cache = Cache(g2, n, 2, 32, 64, fmt)
+    cache.fill(table, [100])
+    q = (torch.randn(1, 2, 64, device="cuda", generator=gen(8)) * 1e38).clamp(-3.4e38, 3.4e38)
+    q[:, :, 5], q[:, :, 40] = 3.4e38, -(2.0 ** 127)
+    out = attend(g2, cache, q, [100], table, 2e-38)
+    want, tol, _ = model_attention(cache, q, [1], [100], table, 2e-38)
+    assert ((out.double() - want).abs() <= tol + 2 ** -24 * want.abs()).all()
+
+
 def test_attention_non_finite_scale(g2):
     """A NaN page shows in the rows and heads that see it, and in no other."""
     lens = [100, 100]
