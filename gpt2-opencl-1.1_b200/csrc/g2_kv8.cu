@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(256)
 constexpr int kAttnWarps = 8;
 constexpr int kMaxWorkers = 4096;   // counters at the start of the workspace
 constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
-constexpr float kNoMax = -1e30f;    // reference of a column that has seen no key
+constexpr float kNoMax = -3.402823466e38f;    // reference of a column that has seen no key: no finite score is below it
 
 template <int D, int NT>
 struct AttnRing {

@@ -461,6 +461,26 @@ def test_attention_largest_q(g2, fmt):
     assert ((out.double() - want).abs() <= tol + 2 ** -24 * want.abs()).all()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens", [[100, 33], [9000, 1]])
+def test_attention_far_below_zero(g2, fmt, lens):
+    """Scores near fp32's least, all of a row the same: its result is the mean of the values."""
+    n, table = tables(2, -(-max(lens) // 32))
+    cache = Cache(g2, n, 2, 32, 64, fmt)
+    cache.fill(table, lens, spread=0.0)
+    one = torch.ones(1, device="cuda")
+    cache.k.copy_(one.to(torch.int8) if fmt == "i8" else one.to(torch.float8_e4m3fn).view(torch.int8))
+    cache.ks.fill_(1e28)
+    q = torch.full((2, 2, 64), -1e8, device="cuda")      # 64 of them by 1e28: -6.4e37, in powers of two -9.2e37
+    out = attend(g2, cache, q, lens, table, 1.0)
+    for s, m in enumerate(lens):
+        pages = table[s, :-(-m // 32)].long()
+        v = (values(cache.v[pages], fmt) * cache.vs[pages].double()[:, :, None, None]).transpose(0, 1).reshape(2, -1, 64)[:, :m]
+        # the scores lose log2 of the V scales, so equal weights need equal scales
+        assert (cache.vs[pages] == cache.vs[pages][0, 0]).all()
+        assert ((out[s].double() - v.mean(1)).abs() <= (m / 16 + 16) * 2 ** -22 * v.abs().mean(1)).all()
+
+
 def test_attention_non_finite_scale(g2):
     """A NaN page shows in the rows and heads that see it, and in no other."""
     lens = [100, 100]
