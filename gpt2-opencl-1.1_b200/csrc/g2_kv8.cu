@@ -133,7 +133,7 @@ __device__ __forceinline__ unsigned recode_word(unsigned w, const unsigned char 
 
 // Codes of four values at a scale whose reciprocal is `inv`.  x * inv is within 2^-22 of the quotient,
 // which decides its code unless it lies that near a border; then (and for e4m3 quotients below the
-// normal range) the exact quotient does.  A division for every value took 48 instructions instead of 15.
+// normal range) the exact quotient does: a division takes several times the product's instructions.
 template <int FMT>
 __device__ __forceinline__ unsigned encode4(const float4 &x, float scale, float inv) {
     const float v[4] = {x.x, x.y, x.z, x.w};
@@ -174,8 +174,9 @@ __device__ __forceinline__ unsigned encode4(const float4 &x, float scale, float 
 //
 // Several rows a sequence: one CTA takes the block's next tiles, as many as give a
 // thread kAppendVecs 4-element loads, all in flight together: a tile by itself
-// waits for its sequence's numbers, its page and its rows in turn (71 -> 26 us for
-// 8 prompts of up to 1000 tokens of 25 heads, reading the rows back included).
+// waits for its sequence's numbers, its page and its rows in turn (8 prompts of up
+// to 1000 tokens of 25 heads, appended and read back: 68 us a tile at a time, 39
+// with this, the encoding by a reciprocal and the gather below).
 constexpr int kAppendThreads = 256, kAppendVecs = 8;
 
 template <typename T, int FMT, int D, int VPT>
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     const bool by_run = all.y <= (unsigned)a.workers &&
                         all.z / (16 * WPR) <= (unsigned)((float)all.x * a.unit / (16.0f * WPR * a.workers)) + kSplitSteps;
     const unsigned total = by_run ? all.y : all.x;
-    const int unit_keys = by_run ? 1 << 30 : a.unit, ahead = by_run ? 0 : a.ahead;
+    const int unit_keys = by_run ? 0x7fffffff : a.unit, ahead = by_run ? 0 : a.ahead;
     const unsigned mine = by_run ? my_runs : my_units;
     unsigned sum = mine;
 #pragma unroll
@@ -1110,8 +1111,8 @@ int check_cache(const char *who, const g2_kv8 *c) {
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
         return arg_error(G2_ERR_ARG, who, "page_size must be 16, 32, 64 or 128");
     if (c->head_dim != 64 && c->head_dim != 128) return arg_error(G2_ERR_ARG, who, "head_dim must be 64 or 128");
-    if (c->n_pages < 1 || c->n_kv_head < 1 || c->n_kv_head > 65535)
-        return arg_error(G2_ERR_RANGE, who, "need n_pages >= 1 and 1 <= n_kv_head <= 65535");
+    if (c->n_pages < 1 || c->n_kv_head < 1 || c->n_kv_head > 32767)   // append's grid has a row for each head's K and V
+        return arg_error(G2_ERR_RANGE, who, "need n_pages >= 1 and 1 <= n_kv_head <= 32767");
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
         return arg_error(G2_ERR_ARG, who, "codes must be 16-byte aligned, scales 4-byte");
     return G2_OK;

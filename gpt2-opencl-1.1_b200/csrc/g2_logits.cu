@@ -290,8 +290,8 @@ extern "C" int g2k_process_logits(const float *logits, long long ld, float *out,
                                   const g2_logit_rules *rules, void *stream) {
     const char *who = "g2k_process_logits";
     if (!logits || !out) return arg_error(G2_ERR_ARG, who, "null argument");
-    if (rows < 0 || rows > 65535 || vocab_size < 1)
-        return arg_error(G2_ERR_RANGE, who, "need 0 <= rows <= 65535 and vocab_size >= 1");
+    if (rows < 0 || rows > 65535 || vocab_size < 1 || vocab_size > 1 << 30)
+        return arg_error(G2_ERR_RANGE, who, "need 0 <= rows <= 65535 and 1 <= vocab_size <= 2^30");
     if (rows > 1 && (ld < vocab_size || ld_out < vocab_size))
         return arg_error(G2_ERR_RANGE, who, "ld and ld_out must be at least vocab_size");
     if (out == logits && ld != ld_out && rows > 1) return arg_error(G2_ERR_ARG, who, "in place, ld and ld_out are the same");

@@ -255,8 +255,9 @@ int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *s
  * x' = LayerNorm(x; ln_gamma, ln_beta, eps 1e-5) when ln_gamma is not NULL.
  * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
  * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32;
- * an x' is carried to 2^-30 of its row's largest or to 2^-22 of itself,
- * whichever serves the shape, an fp16 x of three rows or more exactly.  A
+ * an x' is carried to 2^-30 of its row's largest (of 2^-96 where that is less)
+ * or to 2^-22 of itself, whichever serves the shape, an fp16 x of three rows or
+ * more mostly exactly.  Weights are below 2^76: sums past that may overflow.  A
  * non-finite x' makes its row's outputs non-finite, and no other's.  residual
  * may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls on different
  * streams may overlap. */
@@ -293,7 +294,7 @@ int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const vo
 typedef struct g2_kv8 {
     void *k, *v;                /* 16-byte aligned codes */
     float *k_scale, *v_scale;
-    int n_pages, n_kv_head;
+    int n_pages, n_kv_head;     /* up to 32767 heads */
     int page_size;              /* 16, 32, 64 or 128 tokens */
     int head_dim;               /* 64 or 128 */
     int format;                 /* G2_KV_I8 or G2_KV_E4M3 */
@@ -362,9 +363,10 @@ typedef struct g2_logit_rules {
     int mask_stride;            /* words */
 } g2_logit_rules;
 
-/* Apply the rules (arrays in device memory) to rows 0..rows-1 of logits
- * [rows][ld] over columns 0..vocab_size-1; the result goes to out [rows][ld_out],
- * whose other columns are left as they were.  out may be logits (same ld). */
+/* Apply the rules (arrays in device memory) to rows 0..rows-1 (at most 65535)
+ * of logits [rows][ld] over columns 0..vocab_size-1 (at most 2^30); the result
+ * goes to out [rows][ld_out], whose other columns are left as they were.  out
+ * may be logits (same ld). */
 int g2k_process_logits(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab_size,
                        const g2_logit_rules *rules, void *stream);
 

@@ -138,6 +138,14 @@ def test_logit_rules_arguments():
     assert g2.lib.g2_process_logits(None, 0, None) == ARG
 
 
+def test_sizes_past_a_launch():
+    """More heads than a grid has rows; a vocabulary whose padded length passes 32 bits."""
+    for f in CALLS.values():
+        assert code(lambda: f(cache(n_kv_head=32768), dict(heads=32768) if f is CALLS["attention"] else {})) == RANGE
+    for V in (2 ** 31 - 1, 2 ** 31 - 4, 2 ** 30 + 1):
+        assert code(lambda: g2.process_logits(A, A, 1, V, g2.LogitRules())) == RANGE
+
+
 def no_device_memory():
     """What host memory gives: it is no memory of the device, or there is no device to ask."""
     try:
