@@ -144,11 +144,11 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 //   NP = 4  int8: x as a 30-bit fixed-point number below a power of two over the
 //           row's largest, one column for each of its bytes.  Codes times bytes are
 //           summed exactly in int32, and unpacking eight codes costs three
-//           instructions.  Up to 4 rows (2 of fp16).
-//   NP = 2  fp16: the rounding of x (after a power of two has brought the row's
-//           largest below 2) and 2^11 times the rest, 22 bits in all.  Eight codes
-//           cost nine instructions.  More than 4 rows, eight at a time.
-//   NP = 1  fp16 x as it is.  More than 2 rows.
+//           instructions.  Up to 8 rows at a time (two fp16 columns a row would cost nine:
+//           8 rows of 1600 x 4800 with LayerNorm 10.0 us, bytes 9.8; of 6400 x 1600 18.7
+//           and 16.8).
+//   NP = 1  fp16 x as it is, where eight codes cost nine instructions but a row only
+//           one column.  More than 2 rows.
 // A group's sum is scaled once, in fp32.
 //
 // The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
@@ -160,7 +160,6 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 constexpr int kQ4Warps = 16, kQ4Threads = 32 * kQ4Warps;
 constexpr int kMaxTiles = 32;              // tiles of a CTA summed at a time
 constexpr int kQ4Smem = 220 * 1024;
-constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
 
 // One stage: a chunk of each of TP feature tiles.
 template <int NT, int TP>
@@ -175,6 +174,7 @@ struct Q4Args {
     const void *residual;
     void *y;
     int M, gelu;
+    int ln;                                // where LayerNorm's weights of a slice are staged (bytes; 0: nowhere)
     int copy;                              // fp16 rows of x can be copied 16 bytes at a time
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
@@ -278,8 +278,8 @@ __host__ __device__ __forceinline__ int x_stride(int slice) {
 template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
     constexpr int S = Q4Ring<NT, TP>::kStages, CB = 512 + 32 * PC;
-    constexpr bool INT = NP == 4;
-    constexpr int kHeld = INT ? 4 : 8;             // groups of four x that a thread reads once
+    constexpr bool INT = NP == 4, EARLY = INT && NT < 4;
+    constexpr int kHeld = NT < 4 ? 4 : 8;                     // groups of four x that a thread reads once
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[kQ4Warps], squares[kQ4Warps], up_s[G2_Q4_MAX_ROWS];
     __shared__ unsigned peaks[kQ4Warps];
@@ -322,6 +322,12 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     const int m = i / per_row, k = i % per_row * 8, left = K - c0 * kChunk - k;
                     cp_async16(smem_addr(xs + m * stride + 2 * k),
                                reinterpret_cast<const __half *>(x_rows) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
+                }
+            }
+            if (VEC && a.ln && stage_x) {
+                for (int i = tid; i < nc * (kChunk / 2); i += kQ4Threads) {
+                    const int second = i >= nc * (kChunk / 4), k = (i - second * nc * (kChunk / 4)) * 4, at = c0 * kChunk + k;
+                    cp_async16(smem_addr(smem + a.ln) + 16 * i, (second ? a.beta : a.gamma) + (at < K ? at : 0), at < K ? 16 : 0);
                 }
             }
             cp_commit();
@@ -369,17 +375,25 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                         continue;
                     }
                     // groups past the slice are skipped by whole warps; few rows have registers for LayerNorm's weights too
-                    float4 held[kHeld], ga[INT ? kHeld : 1], be[INT ? kHeld : 1];
+                    float4 held[kHeld], ga[EARLY ? kHeld : 1], be[EARLY ? kHeld : 1];
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i)
                         if (i * step < kn) {
                             const int k = min(k0 + first + i * step, K);
                             held[i] = load_4<VEC>(row, k, K);
-                            if (INT && a.gamma) {
-                                ga[INT ? i : 0] = load_4<VEC>(a.gamma, k, K);
-                                be[INT ? i : 0] = load_4<VEC>(a.beta, k, K);
+                            if (EARLY && a.gamma) {
+                                ga[EARLY ? i : 0] = load_4<VEC>(a.gamma, k, K);
+                                be[EARLY ? i : 0] = load_4<VEC>(a.beta, k, K);
                             }
                         }
+                    if (VEC && a.ln && r0 == 0) {
+                        cp_wait<S - 1>();
+                        __syncthreads();
+                    }
+                    auto weight = [&](const float *p, int second, int k) -> float4 {   // p[k0 + k ...], 0 past the slice
+                        if (!VEC || !a.ln) return load_4<VEC>(p, min(k0 + k, K), K);
+                        return k < kn ? *reinterpret_cast<const float4 *>(smem + a.ln + 4 * (second * kn + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    };
                     float mu = 0.0f, rstd = 1.0f;
                     if (a.gamma) {
                         if (c0 == 0 && tile == tile0) {
@@ -429,7 +443,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     };
                     auto value = [&](int k) -> float4 {           // x'[m][k .. k + 3], 0 past K
                         const float4 v = load_4<VEC>(row, k0 + k, K);
-                        return a.gamma ? norm(v, load_4<VEC>(a.gamma, k0 + k, K), load_4<VEC>(a.beta, k0 + k, K)) : v;
+                        return a.gamma ? norm(v, weight(a.gamma, 0, k), weight(a.beta, 1, k)) : v;
                     };
                     unsigned peak = 0;                            // as integers: NaN above infinity above finite
                     auto larger = [&](const float4 &v) {
@@ -439,47 +453,34 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i)
                         if (i * step < kn) {
-                            const int k = min(k0 + first + i * step, K);      // past K: 0 * 0 + 0
+                            const int k = first + i * step;               // past K: 0 * 0 + 0
                             if (a.gamma)
-                                held[i] = INT ? norm(held[i], ga[INT ? i : 0], be[INT ? i : 0])
-                                              : norm(held[i], load_4<VEC>(a.gamma, k, K), load_4<VEC>(a.beta, k, K));
+                                held[i] = EARLY ? norm(held[i], ga[EARLY ? i : 0], be[EARLY ? i : 0])
+                                                : norm(held[i], weight(a.gamma, 0, k), weight(a.beta, 1, k));
                             larger(held[i]);
                         }
 #pragma unroll 4
                     for (int k = first + kHeld * step; k < kn; k += step) larger(value(k));
                     if (wpr > 1 && r0) __syncthreads();           // the last rows' peaks have been read
                     peak = row_largest(peak, peaks, w0, wpr);
-                    // 2^e <= the largest < 2^(e + 1) (fp16 parts: up to 4 times 2^e); INT: 29 bits below it, and the codes are 16 times theirs
-                    const int e = max(INT ? -96 : -126, min(INT ? 127 : 126, (int)(peak >> 23) - 127)), bits_down = INT ? 29 : 0;
-                    const float down = __uint_as_float((unsigned)(127 + bits_down - e) << 23);
+                    // 2^e <= the largest < 2^(e + 1): 29 bits below it, and the codes are 16 times theirs
+                    const int e = max(-96, min(127, (int)(peak >> 23) - 127));
+                    const float down = __uint_as_float((unsigned)(127 + 29 - e) << 23);
                     if (live && first == 0)
-                        up_s[m] = INT && peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
-                                                             : __uint_as_float((unsigned)(127 + e) << 23) * (INT ? 0x1p-33f : 1.0f);
+                        up_s[m] = peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(127 + e) << 23) * 0x1p-33f;
                     auto put = [&](const float4 &v, int k) {
                         const float x0 = v.x * down, x1 = v.y * down, x2 = v.z * down, x3 = v.w * down;
-                        if (INT) {
-                            // signed bytes: adding 128 to each of the lower three carries into the next
-                            auto digits = [](float x) { return ((unsigned)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u; };
-                            const unsigned q0 = digits(x0), q1 = digits(x1), q2 = digits(x2), q3 = digits(x3);
-                            const unsigned l01 = __byte_perm(q0, q2, 0x5140), l23 = __byte_perm(q1, q3, 0x5140);   // bytes 0 and 1 of both
-                            const unsigned h01 = __byte_perm(q0, q2, 0x7362), h23 = __byte_perm(q1, q3, 0x7362);   // bytes 2 and 3
-                            // rows k, k + 2, k + 1, k + 3, the most significant bytes first
-                            unsigned char *o = xs + 4 * m * stride + (k & ~63) + ((k >> 3) & 3) * 16 + ((k >> 5) & 1) * 8 + (k & 7);
-                            *reinterpret_cast<unsigned *>(o) = __byte_perm(h01, h23, 0x7632);
-                            *reinterpret_cast<unsigned *>(o + stride) = __byte_perm(h01, h23, 0x5410);
-                            *reinterpret_cast<unsigned *>(o + 2 * stride) = __byte_perm(l01, l23, 0x7632);
-                            *reinterpret_cast<unsigned *>(o + 3 * stride) = __byte_perm(l01, l23, 0x5410);
-                            return;
-                        }
-                        const __half2 a0 = __floats2half2_rn(x0, x1), a1 = __floats2half2_rn(x2, x3);
-                        const float2 b0 = __half22float2(a0), b1 = __half22float2(a1);
-                        uint2 hi, lo;
-                        hi.x = bits(a0);
-                        hi.y = bits(a1);
-                        lo.x = bits(__floats2half2_rn((x0 - b0.x) * kLoScale, (x1 - b0.y) * kLoScale));
-                        lo.y = bits(__floats2half2_rn((x2 - b1.x) * kLoScale, (x3 - b1.y) * kLoScale));
-                        *reinterpret_cast<uint2 *>(xs + 2 * m * stride + 2 * k) = hi;
-                        *reinterpret_cast<uint2 *>(xs + (2 * m + 1) * stride + 2 * k) = lo;
+                        // signed bytes: adding 128 to each of the lower three carries into the next
+                        auto digits = [](float x) { return ((unsigned)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u; };
+                        const unsigned q0 = digits(x0), q1 = digits(x1), q2 = digits(x2), q3 = digits(x3);
+                        const unsigned l01 = __byte_perm(q0, q2, 0x5140), l23 = __byte_perm(q1, q3, 0x5140);   // bytes 0 and 1 of both
+                        const unsigned h01 = __byte_perm(q0, q2, 0x7362), h23 = __byte_perm(q1, q3, 0x7362);   // bytes 2 and 3
+                        // rows k, k + 2, k + 1, k + 3, the most significant bytes first
+                        unsigned char *o = xs + 4 * m * stride + (k & ~63) + ((k >> 3) & 3) * 16 + ((k >> 5) & 1) * 8 + (k & 7);
+                        *reinterpret_cast<unsigned *>(o) = __byte_perm(h01, h23, 0x7632);
+                        *reinterpret_cast<unsigned *>(o + stride) = __byte_perm(h01, h23, 0x5410);
+                        *reinterpret_cast<unsigned *>(o + 2 * stride) = __byte_perm(l01, l23, 0x7632);
+                        *reinterpret_cast<unsigned *>(o + 3 * stride) = __byte_perm(l01, l23, 0x5410);
                     };
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i)
@@ -591,12 +592,6 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                                     o[m * 16 * TP + x * 16] = fmaf(v[0], 65536.0f, lo);
                                     o[m * 16 * TP + x * 16 + 8] = fmaf(v[1], 65536.0f, hi);
                                 }
-                            } else if (NP == 2) {
-                                const int m = n * 4 + t;
-                                if (m < M) {
-                                    o[m * 16 * TP + x * 16] = fmaf(v[1], kLoUnscale, v[0]);
-                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[3 % kTot], kLoUnscale, v[2 % kTot]);
-                                }
                             } else {
 #pragma unroll
                                 for (int i = 0; i < kTot; ++i) {
@@ -683,7 +678,13 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
         while (bytes((sh.chunks + slices - 1) / slices) > kQ4Smem) ++slices;   // ends: one chunk fits
         a.slice = (sh.chunks + slices - 1) / slices;
     }
-    const size_t smem = bytes(a.slice);
+    size_t smem = bytes(a.slice);
+    // More rows have no registers for LayerNorm's weights: beside x, where there is room (8 rows of 1600 x 6400: 10.1 -> 9.3 us)
+    a.ln = 0;
+    if (VEC && NT == 4 && a.gamma && smem + a.slice * kChunk * 8 <= kQ4Smem) {
+        a.ln = (int)smem;
+        smem += a.slice * kChunk * 8;
+    }
     // the most that any call uses, so that calls from several host threads do not undo each other's
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4Smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
@@ -709,9 +710,9 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
             return a.M > 8 ? launch_q4<T, VEC, 2, 2, 1>(a, sh, st) : one ? launch_q4<T, VEC, 1, 1, 1>(a, sh, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, st);
     if (a.M <= 2 || fits(2)) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
     if (a.M <= 4 || fits(4)) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
-    // sixteen rows at once would leave room for half as much of x and spill registers (16 rows of
-    // 8192 x 28672: 108 us in groups of eight, 162 together)
-    return launch_q4<T, VEC, 2, 2, 2>(a, sh, st);
+    // Groups of eight: sixteen rows at once would leave room for half as much of x.  Two groups side by side
+    // fill the SMs with pairs of tiles as well (16 rows of 1600 x 1600: 6.4 us, tile by tile 10.8).
+    return one && a.M <= 8 ? launch_q4<T, VEC, 4, 1, 4>(a, sh, st) : launch_q4<T, VEC, 4, 2, 4>(a, sh, st);
 }
 
 bool bad_shape(int N, int K, int group) {

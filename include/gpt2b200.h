@@ -256,11 +256,10 @@ int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *s
  * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
  * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32;
  * an x' is carried to 2^-30 of its row's largest (of 2^-96 where that is less)
- * or to 2^-22 of itself, whichever serves the shape; an fp16 x of three rows or
- * more exactly where the matrix is not narrow.  Weights are below 2^76: sums past that may overflow.  A
- * non-finite x' makes its row's outputs non-finite, and no other's.  residual
- * may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls on different
- * streams may overlap. */
+ * or, an fp16 x in some shapes, as it is.  Weights are below 2^76: sums past
+ * that may overflow.  A non-finite x' makes its row's outputs non-finite, and no
+ * other's.  residual may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls
+ * on different streams may overlap. */
 #define G2_Q4_MAX_ROWS 16
 #define G2_Q4_MAX_K 32768
 int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const void *residual, void *y, int dtype,
