@@ -174,11 +174,13 @@ struct Q4Args {
     const void *residual;
     void *y;
     int M, gelu;
-    int ln;                                // where LayerNorm's weights of a slice are staged (bytes; 0: nowhere)
     int copy;                              // fp16 rows of x can be copied 16 bytes at a time
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
     int share, extra;                      // tiles of a CTA, CTAs that have one more
+    // where LayerNorm's weights of a slice are staged (bytes; 0: nowhere).  Last: ahead of `copy` it changed the
+    // compiler's allocation of the 16-row fp16 kernel (8192 x 28672: 66 us, here 46.5)
+    int ln;
 };
 
 // p[k .. k + 3] as fp32, 0 past K; VEC: in one load (K a multiple of 4, p aligned to it)
@@ -278,7 +280,7 @@ __host__ __device__ __forceinline__ int x_stride(int slice) {
 template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
     constexpr int S = Q4Ring<NT, TP>::kStages, CB = 512 + 32 * PC;
-    constexpr bool INT = NP == 4, EARLY = INT && NT < 4;
+    constexpr bool INT = NP == 4, EARLY = INT && NT < 4, STAGE_LN = VEC && NT == 4;
     constexpr int kHeld = NT < 4 ? 4 : 8;                     // groups of four x that a thread reads once
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[kQ4Warps], squares[kQ4Warps], up_s[G2_Q4_MAX_ROWS];
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                                reinterpret_cast<const __half *>(x_rows) + (size_t)m * K + (left > 0 ? c0 * kChunk + k : 0), left > 0 ? 16 : 0);
                 }
             }
-            if (VEC && a.ln && stage_x) {
+            if (STAGE_LN && a.ln && stage_x) {
                 for (int i = tid; i < nc * (kChunk / 2); i += kQ4Threads) {
                     const int second = i >= nc * (kChunk / 4), k = (i - second * nc * (kChunk / 4)) * 4, at = c0 * kChunk + k;
                     cp_async16(smem_addr(smem + a.ln) + 16 * i, (second ? a.beta : a.gamma) + (at < K ? at : 0), at < K ? 16 : 0);
@@ -386,12 +388,12 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                                 be[EARLY ? i : 0] = load_4<VEC>(a.beta, k, K);
                             }
                         }
-                    if (VEC && a.ln && r0 == 0) {
+                    if (STAGE_LN && a.ln && r0 == 0) {
                         cp_wait<S - 1>();
                         __syncthreads();
                     }
                     auto weight = [&](const float *p, int second, int k) -> float4 {   // p[k0 + k ...], 0 past the slice
-                        if (!VEC || !a.ln) return load_4<VEC>(p, min(k0 + k, K), K);
+                        if (!STAGE_LN || !a.ln) return load_4<VEC>(p, min(k0 + k, K), K);
                         return k < kn ? *reinterpret_cast<const float4 *>(smem + a.ln + 4 * (second * kn + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     };
                     float mu = 0.0f, rstd = 1.0f;
