@@ -1548,6 +1548,7 @@ extern "C" int g2_sample_device(g2_engine *e, int slot, const int *context_ids, 
     CKL();
     CK(cudaMemcpyAsync(e->h_small, e->argmax_out, sizeof(int), cudaMemcpyDeviceToHost, e->st));
     if ((rc = sync_and_check(e))) return rc;
+    if (e->h_small[0] < 0) return set_err(G2_ERR_STATE, "g2_sample_device: every token of slot %d is removed", slot);
     *out_token = e->h_small[0];
     return G2_OK;
 }

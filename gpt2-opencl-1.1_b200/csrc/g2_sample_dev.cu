@@ -17,6 +17,11 @@
 //   6. the first index whose running sum reaches u * sum (main.c:1933-1938),
 //      u supplied by the caller (the reference draws rand() / (RAND_MAX + 1)).
 //      Each thread owns a contiguous block; block sums are scanned in order.
+// Where the slot's logits hold removed tokens (G2_MASKED and below: rules were
+// applied), none of them is drawn: the reference's picks of index 0 at u = 0 and
+// of index V - 1 where rounding leaves the sum short become the first and the
+// last index with a weight, a removed logit keeps its value under any
+// temperature, and -1 says that nothing is left.
 #include <cfloat>
 
 #include "g2_device.cuh"
@@ -27,6 +32,7 @@ namespace g2 {
 namespace {
 
 constexpr int kThreads = 1024;
+constexpr float kRemoved = -1e29f;   // logits at or below it are removed (main.c:1925)
 
 __device__ __forceinline__ unsigned float_key(float f) {
     const unsigned b = __float_as_uint(f);
@@ -47,7 +53,7 @@ struct SampleArgs {
     int top_k;
     float rep_penalty;
     double u;             // uniform draw in [0, 1)
-    int *out;             // [0] token
+    int *out;             // [0] token, -1: every token is removed
 };
 
 __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
@@ -60,8 +66,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int V = a.V;
     float *w = a.work;
-    for (int i = t; i < V; i += kThreads) w[i] = a.logits[i];
-    __syncthreads();
+    bool removed = false;
+    for (int i = t; i < V; i += kThreads) {
+        const float l = a.logits[i];
+        w[i] = l;
+        removed |= l <= kRemoved;
+    }
+    const bool ruled = __syncthreads_or(removed);
     if (t == 0 && a.forbid_eos && G2_EOS < V) w[G2_EOS] = -1e30f;
     __syncthreads();
     if (a.rep_penalty > 1.0f) {
@@ -108,13 +119,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
                     bv = fred[q];
                     bi = ired[q];
                 }
-            a.out[0] = bi == INT_MAX ? 0 : bi;
+            a.out[0] = bi == INT_MAX ? 0 : ruled && bv <= kRemoved ? -1 : bi;
         }
         return;
     }
 
     const float inv_t = 1.0f / a.temperature;
-    for (int i = t; i < V; i += kThreads) w[i] *= inv_t;
+    for (int i = t; i < V; i += kThreads) w[i] = w[i] <= kRemoved ? G2_MASKED : w[i] * inv_t;
     int k = a.top_k;
     if (k <= 0 || k > V) k = V;
     if (k > G2_MAX_TOPK) k = G2_MAX_TOPK;
@@ -150,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
         }
         const float thresh = key_float(sel[0]);
         for (int i = t; i < V; i += kThreads)
-            if (w[i] < thresh) w[i] = -1e30f;
+            if (w[i] < thresh) w[i] = G2_MASKED;
         __syncthreads();
     }
     // maximum
@@ -167,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     for (int i = lo; i < hi; ++i) {
         const float l = w[i];
         float e = 0.0f;
-        if (l > -1e29f) e = expf(l - mx);
+        if (l > kRemoved) e = expf(l - mx);
         w[i] = e;
         s += e;
     }
@@ -182,25 +193,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
             acc += v;
         }
         ired[0] = INT_MAX;
+        ired[1] = ruled ? -1 : V - 1;
         total_s = acc;
     }
     __syncthreads();
     const double total = total_s;
     const double r = a.u * total;
     double acc = dsum[t];
-    int found = INT_MAX;
+    int found = INT_MAX, last = -1;
     for (int i = lo; i < hi; ++i) {
         acc += w[i];
-        if (acc >= r) {
+        if (acc >= r && (!ruled || w[i] > 0.0f)) {
             found = i;
             break;
         }
+        if (w[i] > 0.0f) last = i;
     }
-    for (int o = 16; o; o >>= 1) found = min(found, __shfl_xor_sync(0xffffffffu, found, o));
+    found = __reduce_min_sync(0xffffffffu, found);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) {
+        atomicMin(&ired[0], found);
+        if (ruled) atomicMax(&ired[1], last);
+    }
     __syncthreads();
-    if (lane == 0) atomicMin(&ired[0], found);
-    __syncthreads();
-    if (t == 0) a.out[0] = ired[0] == INT_MAX ? V - 1 : ired[0];
+    if (t == 0) a.out[0] = ired[0] == INT_MAX ? ired[1] : ired[0];
 }
 
 // The k (<= G2_MAX_TOPK) largest of logits[0..V), in the order of the reference's

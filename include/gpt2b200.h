@@ -113,7 +113,9 @@ int g2_topk(g2_engine *e, int slot, int k, float *values, int *ids);
 
 /* sample_next_token (main.c:1872-1939) on host logits[0..vocab_size): EOS mask,
  * repetition penalty over the unique context ids, then greedy (temperature
- * <= 0, first max) or temperature + top-k (<= G2_MAX_TOPK) + C rand() draw. */
+ * <= 0, first max) or temperature + top-k (<= G2_MAX_TOPK) + C rand() draw.
+ * Tokens removed by rules (logits of G2_MASKED and below, down from -1e29) are
+ * never picked; G2_ERR_STATE where nothing else is left. */
 int g2_sample(const float *logits, int vocab_size, const int *context_ids, int n_context,
               int forbid_eos, float temperature, int top_k, float rep_penalty, int *out_token);
 
@@ -124,7 +126,9 @@ int g2_sample(const float *logits, int vocab_size, const int *context_ids, int n
  * threshold (k-th largest; k clamped to G2_MAX_TOPK) and the inverse-CDF draw
  * at u01 * sum.  The caller supplies the uniform draw u01 in [0, 1) -- the
  * reference uses rand() / (RAND_MAX + 1.0).  Only the token comes back to the
- * host (4 bytes instead of the vocab_size logits). */
+ * host (4 bytes instead of the vocab_size logits).  Removed tokens as in
+ * g2_sample: a slot without any keeps the reference's picks, index 0 at u01 = 0
+ * and the last index where rounding leaves the sum short. */
 int g2_sample_device(g2_engine *e, int slot, const int *context_ids, int n_context, int forbid_eos,
                      float temperature, int top_k, float rep_penalty, double u01, int *out_token);
 
@@ -343,8 +347,9 @@ int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q_stride, vo
  *     after the first n_prompt[r] ids of the context (n_prompt NULL: 0);
  *  3. l += bias of the row's (bias_ids, bias) pairs; of pairs with the same id
  *     the last one counts;
- *  4. a token whose bit is 0 in the row's grammar mask becomes G2_MASKED, the
- *     value that the samplers treat as removed: bit v % 32 of word
+ *  4. a token whose bit is 0 in the row's grammar mask becomes G2_MASKED, which
+ *     the samplers never pick (g2_argmax and g2_topk give it with its value where
+ *     nothing larger is left): bit v % 32 of word
  *     mask[r * mask_stride + v / 32] (mask_stride 0: one mask for every row).
  * Row r's context is ctx[ctx_start[r] .. ctx_start[r+1]), its pairs are
  * bias_ids / bias[bias_start[r] .. bias_start[r+1]); ids outside the vocabulary
