@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "g2_args.h"
 #include "g2_device.cuh"
@@ -140,16 +141,24 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 // ---- the product ----------------------------------------------------------------
 // One CTA of 16 warps per SM takes an equal share of the tiles.  Its x is staged
 // in shared memory once, as columns of the tensor cores' B operand (features on m,
-// rows of x on n).  A few rows leave columns idle, so each takes several:
-//   NP = 4  int8: x as a 30-bit fixed-point number below a power of two over the
-//           row's largest, one column for each of its bytes.  Codes times bytes are
-//           summed exactly in int32, and unpacking eight codes costs three
-//           instructions.  Up to 8 rows at a time (two fp16 columns a row would cost nine:
-//           8 rows of 1600 x 4800 with LayerNorm 10.0 us, bytes 9.8; of 6400 x 1600 18.7
-//           and 16.8).
-//   NP = 1  fp16 x as it is, where eight codes cost nine instructions but a row only
-//           one column.  More than 2 rows.
-// A group's sum is scaled once, in fp32.
+// rows of x on n), in a form that keeps every x' to its own 24 bits: a column whose
+// codes are 0 at a row's large values must not inherit their step.
+//   NP = 8, 4, 2  int8: x as a fixed-point number below a power of two over the
+//           row's largest, one column for each of its bytes, NP bytes in an n tile.
+//           Codes times bytes are summed exactly in int32, and unpacking eight codes
+//           costs three instructions.  Up to four rows have eight bytes (61 bits, so
+//           that an x' 2^37 below the largest still has its own 24); three or four of
+//           fp16 six (46 bits, more than fp16 spans).  Four bytes took 6.9 us for 4 rows
+//           of 1600 x 6400 with LayerNorm, where eight take 7.9, and 14.7 and 18.1 for
+//           1600 x 50257, but left 10 bits of a value 2^20 below the largest.  Leaving the
+//           lower bytes out where no x' needs them, by a second loop or a second pass, cost
+//           every call 0.6 us or more, or calls with one tiny value 3 us.
+//   NP = 3  three bf16 parts: the upper 8 bits of 2^-16 x (which keeps sums of its
+//           largest values finite), of the rest and of what that leaves, cut off, not
+//           rounded, so that they add up to x.  A part has 8 rows in an n tile;
+//           each part has its own sums over 32 or 64 rows of W, joined smallest first.
+//           Eight codes cost eleven instructions.
+//   NP = 1  fp16 x as it is, nine instructions for eight codes.
 //
 // The CTA's (tile, chunk) units are cut into 16 equal ranges, one per warp, so
 // that each warp streams one contiguous piece of the packed matrix whatever the
@@ -175,11 +184,11 @@ struct Q4Args {
     void *y;
     int M, gelu;
     int copy;                              // fp16 rows of x can be copied 16 bytes at a time
+    int rows;                              // rows of x of a CTA
     int slice;                             // chunks of x staged at a time
     int most;                              // tiles (of TP feature tiles) summed at a time
     int share, extra;                      // tiles of a CTA, CTAs that have one more
-    // where LayerNorm's weights of a slice are staged (bytes; 0: nowhere).  Last: ahead of `copy` it changed the
-    // compiler's allocation of the 16-row fp16 kernel (8192 x 28672: 66 us, here 46.5)
+    // where LayerNorm's weights of a slice are staged (bytes; 0: nowhere)
     int ln;
 };
 
@@ -229,6 +238,18 @@ __device__ __forceinline__ void mma16832(int (&c)[4], const unsigned (&w)[4], un
                  : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma16816_bf16(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
+}
+// The same onto zeros.
+__device__ __forceinline__ void mma16816_bf16_first(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // Two codes as two fp16 of 1024 + (16 times, for upper nibbles) code + 8: flipping a
 // two's complement nibble's sign bit adds 8, and 0x6400 | n is 1024 + n.
 __device__ __forceinline__ __half2 nibbles(unsigned w, unsigned mask, unsigned flip) {
@@ -245,6 +266,21 @@ __device__ __forceinline__ void codes_to_half(unsigned w, unsigned (&f)[4]) {
     w >>= 8;
     f[2] = bits(__hfma2(nibbles(w, 0x00f000f0u, 0x64806480u), sixteenth, up));
     f[3] = bits(__hsub2(nibbles(w, 0x000f000fu, 0x64086408u), low));
+}
+
+// As bf16 pairs: 0x4300 | n is 128 + n.
+__device__ __forceinline__ void codes_to_bf16(unsigned w, unsigned (&f)[4]) {
+    const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)0x4308));   // 136
+    auto pair = [&](unsigned v) {
+        unsigned r;
+        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(r) : "r"(v), "r"(0x000f000fu), "r"(0x43084308u));   // (v & mask) ^ flip
+        const __nv_bfloat162 p = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&r), low);
+        return *reinterpret_cast<const unsigned *>(&p);
+    };
+    f[0] = pair(w >> 4);
+    f[1] = pair(w);
+    f[2] = pair(w >> 12);
+    f[3] = pair(w >> 8);
 }
 
 // Sum of v over the `n` warps of a row, a power of two that begins at warp `w0`: every lane gets it.
@@ -273,32 +309,38 @@ __device__ __forceinline__ unsigned row_largest(unsigned v, unsigned *scratch, i
 // Bytes of a staged column: 64 past a multiple of 128, so that eight columns' reads meet no bank twice.
 template <int NP>
 __host__ __device__ __forceinline__ int x_stride(int slice) {
-    return NP == 4 ? (slice * kChunk + 127) / 128 * 128 + 64 : slice * kChunk * 2 + 64;
+    return NP == 8 || NP == 4 || NP == 2 ? (slice * kChunk + 127) / 128 * 128 + 64 : slice * kChunk * 2 + 64;
 }
+// Rows of x that the columns hold, and columns for them.
+template <int NT, int NP>
+constexpr int kRowsHeld = NP == 8 || NP == 4 || NP == 2 ? 8 / NP : 8 * NT;
+template <int NT, int NP>
+constexpr int kColumns = NP == 3 ? 24 * NT : 8 * NT;
 
-// NT n tiles of 8 columns, TP feature tiles that share an operand of x, NP columns a row, PC scale groups a chunk.
+// NT n tiles of 8 columns (of each of three parts where NP is 3), TP feature tiles that share an operand of x, the form
+// NP of x (above), PC scale groups a chunk.
 template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Shape sh) {
     constexpr int S = Q4Ring<NT, TP>::kStages, CB = 512 + 32 * PC;
-    constexpr bool INT = NP == 4, EARLY = INT && NT < 4, STAGE_LN = VEC && NT == 4;
-    constexpr int kHeld = NT < 4 ? 4 : 8;                     // groups of four x that a thread reads once
+    constexpr bool INT = NP == 8 || NP == 4 || NP == 2, BF = NP == 3, STAGE_LN = VEC && BF;
+    constexpr int kHeld = INT ? 4 : 8;                        // groups of four x that a thread reads once
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sums[kQ4Warps], squares[kQ4Warps], up_s[G2_Q4_MAX_ROWS];
     __shared__ unsigned peaks[kQ4Warps];
     __shared__ float2 row_stats[G2_Q4_MAX_ROWS];
     __shared__ unsigned char range_s[kMaxTiles][2];
+    constexpr int kPairs = INT ? NT * NP / 2 : 1;                 // pairs of bytes of an x
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch();
-    constexpr int kMost = 8 * NT / NP;                            // rows of x that the columns hold; others are other CTAs'
-    const int row0 = blockIdx.y * kMost, M = min(kMost, a.M - row0), K = sh.K;
+    const int row0 = blockIdx.y * a.rows, M = min(a.rows, a.M - row0), K = sh.K;   // other rows are other CTAs'
     const T *x_rows = static_cast<const T *>(a.x) + (size_t)row0 * K;
     const T *residual = a.residual ? static_cast<const T *>(a.residual) + (size_t)row0 * sh.N : nullptr;
     T *y = static_cast<T *>(a.y) + (size_t)row0 * sh.N;
     const int stride = x_stride<NP>(a.slice);                     // bytes of a column
     unsigned char *ring = smem + (size_t)warp * S * TP * CB;      // [stage][TP] chunks
-    unsigned char *xs = smem + (size_t)kQ4Warps * S * TP * CB;    // [8 NT][stride]
-    float *pieces = reinterpret_cast<float *>(xs + (size_t)8 * NT * stride);          // [tiles + warps][M][16 TP]
+    unsigned char *xs = smem + (size_t)kQ4Warps * S * TP * CB;    // [columns][stride]
+    float *pieces = reinterpret_cast<float *>(xs + (size_t)kColumns<NT, NP> * stride);   // [tiles + warps][M][16 TP]
     float *total = pieces + (size_t)(a.most + kQ4Warps) * M * 16 * TP;                // [M][tiles][16 TP], only with slices
     const unsigned ring_addr = smem_addr(ring);
     const int b = blockIdx.x;                                     // tiles of TP feature tiles: a.share, or one more
@@ -306,7 +348,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     // warps of a row of x in the passes over it
     int wpr = kQ4Warps;
     while (wpr * M > kQ4Warps && wpr > 1) wpr >>= 1;
-    const int rows_at_once = kQ4Warps / wpr, w0 = warp / wpr * wpr;
+    const int w0 = warp / wpr * wpr;
     const int first = ((warp - w0) * 32 + lane) * 4, step = wpr * 128;
 
     for (int tile = tile0; tile < tile1; tile += a.most) {
@@ -362,33 +404,31 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
             // ---- x of this slice, once
             if (stage_x && !(NP == 1 && a.copy)) {
                 const int k0 = c0 * kChunk, kn = nc * kChunk;
-                for (int r0 = 0; r0 < M; r0 += rows_at_once) {    // columns past M rows keep what they hold
-                    const int m = r0 + warp / wpr;
-                    const bool live = m < M;
-                    const T *row = x_rows + (size_t)(live ? m : 0) * K;
-                    if (NP == 1) {
-                        for (int k = live ? first : kn; k < kn; k += step) {
-                            const float4 v = load_4<VEC>(row, k0 + k, K);
-                            uint2 o;
-                            o.x = bits(__floats2half2_rn(v.x, v.y));
-                            o.y = bits(__floats2half2_rn(v.z, v.w));
-                            *reinterpret_cast<uint2 *>(xs + m * stride + 2 * k) = o;
-                        }
-                        continue;
+                const int m = warp / wpr;                         // wpr M <= 16: every row has its warps; columns past M rows keep what they hold
+                const bool live = m < M;
+                const T *row = x_rows + (size_t)(live ? m : 0) * K;
+                if constexpr (NP == 1) {
+                    for (int k = live ? first : kn; k < kn; k += step) {
+                        const float4 v = load_4<VEC>(row, k0 + k, K);
+                        uint2 o;
+                        o.x = bits(__floats2half2_rn(v.x, v.y));
+                        o.y = bits(__floats2half2_rn(v.z, v.w));
+                        *reinterpret_cast<uint2 *>(xs + m * stride + 2 * k) = o;
                     }
+                } else {
                     // groups past the slice are skipped by whole warps; few rows have registers for LayerNorm's weights too
-                    float4 held[kHeld], ga[EARLY ? kHeld : 1], be[EARLY ? kHeld : 1];
+                    float4 held[kHeld], ga[INT ? kHeld : 1], be[INT ? kHeld : 1];
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i)
                         if (i * step < kn) {
                             const int k = min(k0 + first + i * step, K);
                             held[i] = load_4<VEC>(row, k, K);
-                            if (EARLY && a.gamma) {
-                                ga[EARLY ? i : 0] = load_4<VEC>(a.gamma, k, K);
-                                be[EARLY ? i : 0] = load_4<VEC>(a.beta, k, K);
+                            if (INT && a.gamma) {
+                                ga[INT ? i : 0] = load_4<VEC>(a.gamma, k, K);
+                                be[INT ? i : 0] = load_4<VEC>(a.beta, k, K);
                             }
                         }
-                    if (STAGE_LN && a.ln && r0 == 0) {
+                    if (STAGE_LN && a.ln) {
                         cp_wait<S - 1>();
                         __syncthreads();
                     }
@@ -447,48 +487,86 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                         const float4 v = load_4<VEC>(row, k0 + k, K);
                         return a.gamma ? norm(v, weight(a.gamma, 0, k), weight(a.beta, 1, k)) : v;
                     };
-                    unsigned peak = 0;                            // as integers: NaN above infinity above finite
-                    auto larger = [&](const float4 &v) {
-                        auto mag = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
-                        peak = max(max(peak, max(mag(v.x), mag(v.y))), max(mag(v.z), mag(v.w)));
+                    auto normed = [&](int i) -> float4 {          // held[i] after LayerNorm; past K: 0 * 0 + 0
+                        if (!a.gamma) return held[i];
+                        const int k = first + i * step;
+                        return INT ? norm(held[i], ga[INT ? i : 0], be[INT ? i : 0]) : norm(held[i], weight(a.gamma, 0, k), weight(a.beta, 1, k));
                     };
+                    if constexpr (BF) {
+                        auto put = [&](const float4 &v, int k) {
+                            float r[4] = {v.x * 0x1p-16f, v.y * 0x1p-16f, v.z * 0x1p-16f, v.w * 0x1p-16f};
+                            unsigned char *o = xs + m * stride + 2 * k;
 #pragma unroll
-                    for (int i = 0; i < kHeld; ++i)
-                        if (i * step < kn) {
-                            const int k = first + i * step;               // past K: 0 * 0 + 0
-                            if (a.gamma)
-                                held[i] = EARLY ? norm(held[i], ga[EARLY ? i : 0], be[EARLY ? i : 0])
-                                                : norm(held[i], weight(a.gamma, 0, k), weight(a.beta, 1, k));
-                            larger(held[i]);
-                        }
-#pragma unroll 4
-                    for (int k = first + kHeld * step; k < kn; k += step) larger(value(k));
-                    if (wpr > 1 && r0) __syncthreads();           // the last rows' peaks have been read
-                    peak = row_largest(peak, peaks, w0, wpr);
-                    // 2^e <= the largest < 2^(e + 1): 29 bits below it, and the codes are 16 times theirs
-                    const int e = max(-96, min(127, (int)(peak >> 23) - 127));
-                    const float down = __uint_as_float((unsigned)(127 + 29 - e) << 23);
-                    if (live && first == 0)
-                        up_s[m] = peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(127 + e) << 23) * 0x1p-33f;
-                    auto put = [&](const float4 &v, int k) {
-                        const float x0 = v.x * down, x1 = v.y * down, x2 = v.z * down, x3 = v.w * down;
-                        // signed bytes: adding 128 to each of the lower three carries into the next
-                        auto digits = [](float x) { return ((unsigned)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u; };
-                        const unsigned q0 = digits(x0), q1 = digits(x1), q2 = digits(x2), q3 = digits(x3);
-                        const unsigned l01 = __byte_perm(q0, q2, 0x5140), l23 = __byte_perm(q1, q3, 0x5140);   // bytes 0 and 1 of both
-                        const unsigned h01 = __byte_perm(q0, q2, 0x7362), h23 = __byte_perm(q1, q3, 0x7362);   // bytes 2 and 3
-                        // rows k, k + 2, k + 1, k + 3, the most significant bytes first
-                        unsigned char *o = xs + 4 * m * stride + (k & ~63) + ((k >> 3) & 3) * 16 + ((k >> 5) & 1) * 8 + (k & 7);
-                        *reinterpret_cast<unsigned *>(o) = __byte_perm(h01, h23, 0x7632);
-                        *reinterpret_cast<unsigned *>(o + stride) = __byte_perm(h01, h23, 0x5410);
-                        *reinterpret_cast<unsigned *>(o + 2 * stride) = __byte_perm(l01, l23, 0x7632);
-                        *reinterpret_cast<unsigned *>(o + 3 * stride) = __byte_perm(l01, l23, 0x5410);
-                    };
+                            for (int p = 0; p < 3; ++p, o += 8 * NT * stride) {
+                                const uint2 w = make_uint2(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x7632),
+                                                           __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x7632));
+                                *reinterpret_cast<uint2 *>(o) = w;
 #pragma unroll
-                    for (int i = 0; i < kHeld; ++i)
-                        if (i * step < kn && live && first + i * step < kn) put(held[i], first + i * step);
+                                for (int j = 0; j < 4; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
+                            }
+                        };
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i)
+                            if (i * step < kn) {
+                                const float4 v = normed(i);
+                                if (live && first + i * step < kn) put(v, first + i * step);
+                            }
 #pragma unroll 4
-                    for (int k = live ? first + kHeld * step : kn; k < kn; k += step) put(value(k), k);
+                        for (int k = live ? first + kHeld * step : kn; k < kn; k += step) put(value(k), k);
+                    } else {
+                        // as integers: NaN above infinity above finite
+                        unsigned peak = 0;
+                        auto measure = [&](const float4 &v) {
+                            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) peak = max(peak, __float_as_uint(x[j]) & 0x7fffffffu);
+                        };
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i)
+                            if (i * step < kn) {
+                                held[i] = normed(i);
+                                measure(held[i]);
+                            }
+#pragma unroll 4
+                        for (int k = first + kHeld * step; k < kn; k += step) measure(value(k));
+                        peak = row_largest(peak, peaks, w0, wpr);
+                        // 2^e <= the largest < 2^(e + 1): 29 bits below it are the upper four bytes' unit, and the codes are 16 times theirs
+                        const int e = max(-96, min(127, (int)(peak >> 23) - 127));
+                        const float down = __uint_as_float((unsigned)(127 + 29 - e) << 23);
+                        if (live && first == 0)
+                            up_s[m] = peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(127 + e) << 23) * 0x1p-33f;
+                        auto put = [&](const float4 &v, int k) {
+                            // rows k, k + 2, k + 1, k + 3 of a column, the most significant bytes first
+                            unsigned char *o = xs + m * NP * stride + (k & ~63) + ((k >> 3) & 3) * 16 + ((k >> 5) & 1) * 8 + (k & 7);
+                            auto column = [&](int b) { return reinterpret_cast<unsigned *>(o + (b / NP * 8 + b % NP) * stride); };
+                            float x[4] = {v.x * down, v.y * down, v.z * down, v.w * down};
+#pragma unroll
+                            for (int half = 0; half < (kPairs + 1) / 2; ++half) {
+                                const bool two = kPairs == 3 && half == 1;   // two bytes, not four
+                                unsigned q[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const int n = __float2int_rn(x[j]);
+                                    x[j] = (x[j] - (float)n) * (kPairs == 3 ? 0x1p15f : 0x1p31f);   // both exact: n has at most the bits of x
+                                    // signed bytes: adding 128 to each of the lower ones carries into the next
+                                    q[j] = two ? ((unsigned)n + 0x0080u) ^ 0x0080u : ((unsigned)n + 0x00808080u) ^ 0x00808080u;
+                                }
+                                const unsigned l01 = __byte_perm(q[0], q[2], 0x5140), l23 = __byte_perm(q[1], q[3], 0x5140);   // bytes 0 and 1 of both
+                                const unsigned h01 = __byte_perm(q[0], q[2], 0x7362), h23 = __byte_perm(q[1], q[3], 0x7362);   // bytes 2 and 3
+                                if (!two) {
+                                    *column(4 * half) = __byte_perm(h01, h23, 0x7632);
+                                    *column(4 * half + 1) = __byte_perm(h01, h23, 0x5410);
+                                }
+                                *column(4 * half + (two ? 0 : 2)) = __byte_perm(l01, l23, 0x7632);
+                                *column(4 * half + (two ? 1 : 3)) = __byte_perm(l01, l23, 0x5410);
+                            }
+                        };
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i)
+                            if (i * step < kn && live && first + i * step < kn) put(held[i], first + i * step);
+#pragma unroll 4
+                        for (int k = live ? first + kHeld * step : kn; k < kn; k += step) put(value(k), k);
+                    }
                 }
             }
             if (tid < R) {                                        // the warps that have units of each tile
@@ -516,20 +594,57 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                 cp_wait<S - 2>();
                 __syncwarp();
                 issue();
-                uint4 xv[NT][INT ? 1 : 2];
+                if constexpr (BF) {
+                    constexpr bool BOTH = PC == 1;                // sums over 64 rows, or over a group of 32
+                    uint4 w[TP];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int x = 0; x < TP; ++x) w[x] = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
+                    float acc[TP][3][NT][4];
 #pragma unroll
-                    for (int half = 0; half < (INT ? 1 : 2); ++half)
-                        xv[n][half] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride + half * 64);
+                    for (int half = 0; half < 2; ++half) {
+                        uint4 xv[3][NT];
 #pragma unroll
-                for (int x = 0; x < TP; ++x) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
-                    const unsigned words[4] = {w.x, w.y, w.z, w.w};
-                    unsigned sc[PC];
+                        for (int p = 0; p < 3; ++p)
 #pragma unroll
-                    for (int i = 0; i < PC; ++i) sc[i] = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + i * 32 + g * 4);
-                    if constexpr (INT) {
+                            for (int n = 0; n < NT; ++n)
+                                xv[p][n] = *reinterpret_cast<const uint4 *>(xk + (p * NT + n) * 8 * stride + half * 64);
+#pragma unroll
+                        for (int x = 0; x < TP; ++x) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                unsigned f[4];
+                                codes_to_bf16(half ? (i ? w[x].w : w[x].z) : (i ? w[x].y : w[x].x), f);
+#pragma unroll
+                                for (int p = 0; p < 3; ++p)
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) {
+                                        const unsigned b0 = i ? xv[p][n].z : xv[p][n].x, b1 = i ? xv[p][n].w : xv[p][n].y;
+                                        if (i == 0 && (half == 0 || !BOTH)) mma16816_bf16_first(acc[x][p][n], f, b0, b1);
+                                        else mma16816_bf16(acc[x][p][n], f, b0, b1);
+                                    }
+                            }
+                            if (half == 1 || !BOTH) {             // the group's sum, scaled
+                                const unsigned s = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + (PC == 2 ? half * 32 : 0) + g * 4);
+                                const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        tot[x][n][j] = fmaf((acc[x][2][n][j] + acc[x][1][n][j]) + acc[x][0][n][j], j < 2 ? lo : hi, tot[x][n][j]);
+                            }
+                        }
+                    }
+                } else if constexpr (INT) {
+                    uint4 xv[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) xv[n] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride);
+#pragma unroll
+                    for (int x = 0; x < TP; ++x) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
+                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
+                        unsigned sc[PC];
+#pragma unroll
+                        for (int i = 0; i < PC; ++i) sc[i] = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + i * 32 + g * 4);
                         int acc[NT][4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
@@ -539,8 +654,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                             const unsigned u0 = words[2 * i], u1 = words[2 * i + 1];
                             const unsigned f[4] = {u0 & 0xf0f0f0f0u, (u0 << 4) & 0xf0f0f0f0u, u1 & 0xf0f0f0f0u, (u1 << 4) & 0xf0f0f0f0u};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma16832(acc[n], f, i ? xv[n][0].z : xv[n][0].x, i ? xv[n][0].w : xv[n][0].y);
-                            if (i == 1 || PC == 2) {              // the group's sums of two neighbouring bytes, below 2^29
+                            for (int n = 0; n < NT; ++n) mma16832(acc[n], f, i ? xv[n].z : xv[n].x, i ? xv[n].w : xv[n].y);
+                            if (i == 1 || PC == 2) {          // the group's sums of two neighbouring bytes, below 2^29
                                 const unsigned s = sc[PC == 2 ? i : 0];
                                 const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
 #pragma unroll
@@ -550,7 +665,21 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                                 }
                             }
                         }
-                    } else {
+                    }
+                } else {
+                    uint4 xv[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            xv[n][half] = *reinterpret_cast<const uint4 *>(xk + n * 8 * stride + half * 64);
+#pragma unroll
+                    for (int x = 0; x < TP; ++x) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(slot + x * CB + lane * 16);
+                        const unsigned words[4] = {w.x, w.y, w.z, w.w};
+                        unsigned sc[PC];
+#pragma unroll
+                        for (int i = 0; i < PC; ++i) sc[i] = *reinterpret_cast<const unsigned *>(slot + x * CB + 512 + i * 32 + g * 4);
                         float acc[NT][4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -561,7 +690,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                             codes_to_half(words[i], f);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                const uint4 &v = xv[n][INT ? 0 : i >> 1];
+                                const uint4 &v = xv[n][i >> 1];
                                 mma16816(acc[n], f, (i & 1) ? v.z : v.x, (i & 1) ? v.w : v.y);
                             }
                             if (i == 3 || (PC == 2 && i == 1)) {  // the group's sum, scaled
@@ -587,12 +716,22 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
 #pragma unroll
                         for (int x = 0; x < TP; ++x) {
                             float (&v)[kTot] = tot[x][n];
-                            if (INT) {                            // columns 2t, 2t + 1: the upper or the lower half of row t / 2
-                                const float lo = __shfl_down_sync(0xffffffffu, v[0], 1), hi = __shfl_down_sync(0xffffffffu, v[1], 1);
-                                const int m = n * 2 + (t >> 1);
-                                if (m < M && !(t & 1)) {
-                                    o[m * 16 * TP + x * 16] = fmaf(v[0], 65536.0f, lo);
-                                    o[m * 16 * TP + x * 16 + 8] = fmaf(v[1], 65536.0f, hi);
+                            if constexpr (INT) {                  // thread t has two bytes of each tile, the upper ones first
+                                if (n > 0) break;
+                                constexpr int kThreads = NP / 2;  // threads of a row
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    auto pair = [&](int j) -> float {   // of the row that begins with this thread
+                                        if (j >= kPairs) return 0.0f;
+                                        const float w = tot[x][j / kThreads][i];
+                                        return j % kThreads ? __shfl_down_sync(0xffffffffu, w, j % kThreads) : w;
+                                    };
+                                    float all = pair(1);
+                                    if (kPairs > 2) all = fmaf(pair(2), 0x1p-15f, all);
+                                    if (kPairs > 3) all = fmaf(pair(3), 0x1p-31f, all);
+                                    all = fmaf(pair(0), 65536.0f, all);
+                                    const int m = t / kThreads;
+                                    if (m < M && t % kThreads == 0) o[m * 16 * TP + x * 16 + 8 * i] = all;
                                 }
                             } else {
 #pragma unroll
@@ -601,9 +740,13 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                                     if (m < M) o[m * 16 * TP + x * 16 + (i >> 1) * 8] = v[i];
                                 }
                             }
-#pragma unroll
-                            for (int i = 0; i < kTot; ++i) v[i] = 0.0f;
                         }
+#pragma unroll
+                    for (int x = 0; x < TP; ++x)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < kTot; ++i) tot[x][n][i] = 0.0f;
                     c = nc;
                     xk -= nc * kStep;
                     ++r;
@@ -614,7 +757,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
 
             // ---- sums over the warps of each tile, in order; after the last slice bias, GELU, residual
             // (four rows, a tile) at a time: 32 features of one item, or 16 of two, a warp
-            constexpr int kPer = 2 / TP, kRows = NP == 4 ? 1 : 4;
+            constexpr int kPer = 2 / TP, kRows = INT ? 1 : 4;
             const int f = lane % (16 * TP), row_groups = (M + kRows - 1) / kRows;
             int mg = 0, rr = warp * kPer + lane / (16 * TP);
             for (;; rr += kQ4Warps * kPer) {
@@ -639,7 +782,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
                     const int m = m0 + j;
                     if (m >= M) break;
                     float *so_far = total + (m * R + rr) * 16 * TP + f;
-                    if (NP > 1) v[j] *= up_s[m];
+                    if (INT) v[j] *= up_s[m];
+                    if (BF) v[j] *= 65536.0f;
                     if (c0 > 0) v[j] += *so_far;
                     if (!last) *so_far = v[j];
                     if (there) {
@@ -670,9 +814,9 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     a.extra = ntiles % grid;
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
     // x in equal slices that fit beside the ring and the sums
-    const size_t ring = (size_t)kQ4Warps * Q4Ring<NT, TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)std::min(a.M, 8 * NT / NP) * 16 * TP * 4;
+    const size_t ring = (size_t)kQ4Warps * Q4Ring<NT, TP>::kStages * TP * sh.chunk_bytes, tile = (size_t)std::min(a.M, a.rows) * 16 * TP * 4;
     size_t sums = (a.most + kQ4Warps) * tile;
-    auto bytes = [&](int slice) { return ring + (size_t)8 * NT * x_stride<NP>(slice) + sums; };
+    auto bytes = [&](int slice) { return ring + (size_t)kColumns<NT, NP> * x_stride<NP>(slice) + sums; };
     a.slice = sh.chunks;
     if (bytes(a.slice) > kQ4Smem) {
         sums += a.most * tile;
@@ -681,20 +825,22 @@ int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
         a.slice = (sh.chunks + slices - 1) / slices;
     }
     size_t smem = bytes(a.slice);
-    // More rows have no registers for LayerNorm's weights: beside x, where there is room (8 rows of 1600 x 6400: 10.1 -> 9.3 us)
+    // More rows have no registers for LayerNorm's weights: beside x, where there is room (8 rows of 1600 x 6400: 10.1 us without)
     a.ln = 0;
-    if (VEC && NT == 4 && a.gamma && smem + a.slice * kChunk * 8 <= kQ4Smem) {
+    if (VEC && NP == 3 && a.gamma && smem + a.slice * kChunk * 8 <= kQ4Smem) {
         a.ln = (int)smem;
         smem += a.slice * kChunk * 8;
     }
     // the most that any call uses, so that calls from several host threads do not undo each other's
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQ4Smem) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_matvec_q4", cudaGetErrorString(cudaGetLastError()));
-    return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid, (a.M + 8 * NT / NP - 1) / (8 * NT / NP)), dim3(kQ4Threads), smem, st, a, sh));
+    return launch_status("g2k_matvec_q4", launch_pdl(kernel, dim3(grid, (a.M + a.rows - 1) / a.rows), dim3(kQ4Threads), smem, st, a, sh));
 }
 
+// `rows` rows of x to a CTA
 template <typename T, bool VEC, int NT, int TP, int NP>
-int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
+int launch_q4(Q4Args a, const Q4Shape &sh, int rows, cudaStream_t st) {
+    a.rows = std::min(rows, kRowsHeld<NT, NP>);
     return sh.per_chunk == 2 ? launch_q4<T, VEC, NT, TP, NP, 2>(a, sh, st) : launch_q4<T, VEC, NT, TP, NP, 1>(a, sh, st);
 }
 
@@ -709,12 +855,15 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     const auto fits = [&](int rows) { return sh.tiles * ((a.M + rows - 1) / rows) <= sms; };
     if constexpr (sizeof(T) == 2)
         if (!a.gamma && a.M > 2 && !(a.M > 8 && fits(2)))
-            return a.M > 8 ? launch_q4<T, VEC, 2, 2, 1>(a, sh, st) : one ? launch_q4<T, VEC, 1, 1, 1>(a, sh, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, st);
-    if (a.M <= 2 || fits(2)) return one ? launch_q4<T, VEC, 1, 1, 4>(a, sh, st) : launch_q4<T, VEC, 1, 2, 4>(a, sh, st);
-    if (a.M <= 4 || fits(4)) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, st);
+            return a.M > 8 ? launch_q4<T, VEC, 2, 2, 1>(a, sh, 16, st)
+                 : one     ? launch_q4<T, VEC, 1, 1, 1>(a, sh, 8, st) : launch_q4<T, VEC, 1, 2, 1>(a, sh, 8, st);
+    constexpr int kFour = sizeof(T) == 4 ? 4 : 3;   // n tiles of four rows' bytes
+    if (a.M == 1) return one ? launch_q4<T, VEC, 1, 1, 8>(a, sh, 1, st) : launch_q4<T, VEC, 1, 2, 8>(a, sh, 1, st);
+    if (a.M == 2 || fits(2)) return one ? launch_q4<T, VEC, 2, 1, 4>(a, sh, 2, st) : launch_q4<T, VEC, 2, 2, 4>(a, sh, 2, st);
+    if (a.M <= 4 || fits(4)) return one ? launch_q4<T, VEC, kFour, 1, 2>(a, sh, 4, st) : launch_q4<T, VEC, kFour, 2, 2>(a, sh, 4, st);
     // Groups of eight: sixteen rows at once would leave room for half as much of x.  Two groups side by side
     // fill the SMs with pairs of tiles as well (16 rows of 1600 x 1600: 6.4 us, tile by tile 10.8).
-    return one && a.M <= 8 ? launch_q4<T, VEC, 4, 1, 4>(a, sh, st) : launch_q4<T, VEC, 4, 2, 4>(a, sh, st);
+    return one && a.M <= 8 ? launch_q4<T, VEC, 1, 1, 3>(a, sh, 8, st) : launch_q4<T, VEC, 1, 2, 3>(a, sh, 8, st);
 }
 
 bool bad_shape(int N, int K, int group) {
@@ -789,7 +938,7 @@ extern "C" int g2k_matvec_q4(const void *x, const void *packed, const float *bia
     const Q4Shape sh(N, K, group);
     const bool vec = K % 4 == 0 && aligned(x, 4 * es) && aligned(ln_gamma, 16) && aligned(ln_beta, 16);
     const Q4Args a{x, static_cast<const unsigned char *>(packed), bias, ln_gamma, ln_beta, residual, y, M, apply_gelu,
-                   dtype == G2_F16 && K % 8 == 0 && !ln_gamma && aligned(x, 16), 0, 0, 0, 0};
+                   dtype == G2_F16 && K % 8 == 0 && !ln_gamma && aligned(x, 16), 0, 0, 0, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == G2_F32) return vec ? launch_q4<float, true>(a, sh, st) : launch_q4<float, false>(a, sh, st);
     return vec ? launch_q4<__half, true>(a, sh, st) : launch_q4<__half, false>(a, sh, st);

@@ -258,9 +258,11 @@ int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *s
  * y[m][n] = sum_k x'[m][k] * W[k][n] (+bias[n]) (then GELU) (+residual[m][n]),
  * x' = LayerNorm(x; ln_gamma, ln_beta, eps 1e-5) when ln_gamma is not NULL.
  * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
- * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32;
- * an x' is carried to 2^-30 of its row's largest (of 2^-96 where that is less)
- * or, an fp16 x in some shapes, as it is.  Weights are below 2^76: sums past
+ * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32; an
+ * x' is carried exactly but for what lies below 2^-60 of its row's largest (2^-44
+ * for three or four fp16 rows with LayerNorm) or below 2^-117, so a column whose
+ * codes are 0 at a row's large values keeps its accuracy.  A row's last bits may
+ * differ with the number of rows and N.  Weights are below 2^76: sums past
  * that may overflow.  A non-finite x' makes its row's outputs non-finite, and no
  * other's.  residual may alias y.  K <= G2_Q4_MAX_K.  Needs no workspace; calls
  * on different streams may overlap. */
