@@ -1151,7 +1151,7 @@ cudaError_t launch_append(const g2_kv8 &c, const void *k, const void *v, long lo
         return c.head_dim == 64 ? launch_pdl(kv8_append_token_kernel<T, FMT, 64>, grid, dim3(256), 0, st, c, kt, vt, stride, pos, r)
                                 : launch_pdl(kv8_append_token_kernel<T, FMT, 128>, grid, dim3(256), 0, st, c, kt, vt, stride, pos, r);
     }
-    const int per = (c.page_size + r.max_q - 2) / c.page_size + 1;   // blocks that max_q rows can touch
+    const int per = (int)(((long long)c.page_size + r.max_q - 2) / c.page_size) + 1;   // blocks that max_q rows can touch
     const int vpt = c.page_size * c.head_dim / (4 * kAppendThreads), tiles = std::max(1, kAppendVecs / vpt);
     const dim3 grid((unsigned)per * r.n_seq, (2 * c.n_kv_head + tiles - 1) / tiles);
     auto launch = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kAppendThreads), 0, st, c, kt, vt, stride, pos, r, per); };
@@ -1174,10 +1174,13 @@ cudaError_t launch_append(const g2_kv8 &c, const void *k, const void *v, long lo
 
 template <typename T, int FMT>
 cudaError_t launch_gather(const g2_kv8 &c, void *k, void *v, long long stride, const int *pos, const Rows8 &r, cudaStream_t st) {
-    const int per = (r.max_q + kGatherRows - 2) / kGatherRows + 1;   // chunks that max_q rows can touch
+    const int per = (int)(((long long)r.max_q + kGatherRows - 2) / kGatherRows) + 1;   // chunks that max_q rows can touch
     const dim3 grid((unsigned)per * r.n_seq, (c.n_kv_head * c.head_dim / 2 + 255) / 256);
     return launch_pdl(kv8_gather_kernel<T, FMT>, grid, dim3(256), 0, st, c, static_cast<T *>(k), static_cast<T *>(v), stride, pos, r, per);
 }
+
+// A sequence has no more rows than there are: a larger bound only makes larger grids.
+int bound_rows(int max_q, int n_rows) { return std::min(max_q, std::max(n_rows, 1)); }
 
 // dtype and format to template arguments
 #define G2_KV8_DISPATCH(fn, ...)                                                                                       \
@@ -1196,9 +1199,10 @@ extern "C" int g2k_kv8_append(const g2_kv8 *cache, const void *k, const void *v,
     const char *who = "g2k_kv8_append";
     int rc;
     if ((rc = check_cache(who, cache))) return rc;
-    const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
+    Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, cache->n_kv_head, k, v, dtype, &row_stride, nullptr, r, pos))) return rc;
-    if (((long long)max_q / cache->page_size + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many blocks");
+    r.max_q = bound_rows(max_q, n_rows);
+    if (((long long)r.max_q / cache->page_size + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many blocks");
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k, v, q_start, pos, table, status})))
         return rc;
@@ -1211,9 +1215,10 @@ extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int
     const char *who = "g2k_kv8_gather";
     int rc;
     if ((rc = check_cache(who, cache))) return rc;
-    const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
+    Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, cache->n_kv_head, k_out, v_out, dtype, &row_stride, nullptr, r, pos))) return rc;
-    if (((long long)max_q / kGatherRows + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
+    r.max_q = bound_rows(max_q, n_rows);
+    if (((long long)r.max_q / kGatherRows + 3) * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
     if (n_rows == 0 || n_seq == 0) return G2_OK;
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, k_out, v_out, q_start, pos, table, status})))
         return rc;
@@ -1236,13 +1241,14 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if (n_head < 1 || n_head % cache->n_kv_head || n_head > 65535)
         return arg_error(G2_ERR_RANGE, who, "n_head must be a multiple of n_kv_head, at most 65535");
     if (!(scale > 0.0f) || !std::isfinite(scale)) return arg_error(G2_ERR_ARG, who, "scale must be positive");
-    const Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
+    Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, n_head, q, out, dtype, &q_stride, &out_stride, r, seq_len))) return rc;
-    if ((long long)max_q * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
+    r.max_q = bound_rows(max_q, n_rows);
+    if ((long long)r.max_q * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
     {   // the kernel counts units in 32 bits
-        const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, 1);
+        const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, 1);
         const double units = ((double)table_stride * cache->page_size / p.unit + 1 + p.ahead) * n_seq * cache->n_kv_head *
-                             ((double)max_q * (n_head / cache->n_kv_head) / (4 * p.nt) + 1);
+                             ((double)r.max_q * (n_head / cache->n_kv_head) / (4 * p.nt) + 1);
         if (units > 2147483647.0) return arg_error(G2_ERR_RANGE, who, "too much work for one call");
     }
     if (!workspace || !aligned(workspace, 256)) return arg_error(G2_ERR_ARG, who, "workspace not 256-byte aligned");
@@ -1253,7 +1259,7 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
                                       workspace, status})))
         return rc;
     const int sms = attn_sms();
-    const AttnPlan p = attn_plan(*cache, n_head, n_seq, max_q, sms);
+    const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, sms);   // needs no more workspace than max_q's plan
     const AttnArgs a{*cache, q, out, q_stride, out_stride, dtype == G2_F16, n_head / cache->n_kv_head,
                      scale * 1.4426950408889634f, seq_len, r, p.unit, p.ahead, p.workers, static_cast<unsigned *>(workspace),
                      static_cast<float *>(workspace) + kMaxWorkers};

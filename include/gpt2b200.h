@@ -281,7 +281,8 @@ int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const vo
  * All arrays below are in device memory unless said otherwise.
  *
  * Rows: with q_start NULL sequence s has the one row s (n_rows == n_seq, max_q
- * 1); else rows q_start[s] .. q_start[s+1]-1, at most max_q of them.  Rows that
+ * 1); else rows q_start[s] .. q_start[s+1]-1, at most max_q of them (any bound
+ * that holds: one above n_rows costs no more than n_rows).  Rows that
  * no sequence has are left as they were.  Row i of head h is at element
  * i * stride + h * head_dim; a stride of 0 means heads * head_dim, others let
  * rows be parts of wider ones (the thirds of a c_attn row).  Base pointers and

@@ -1,0 +1,50 @@
+"""The 8-bit cache's calls at the limits of their arguments: bounds on the rows of
+a sequence that no sequence reaches (GPU), and refusals (CPU)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import gpt2b200 as g2  # noqa: E402
+from test_operator_args import CALLS, cache, code, no_device_memory  # noqa: E402
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [5, 64, 2 ** 31 - 1])
+@pytest.mark.parametrize("page", [16, 128])
+def test_any_bound_on_the_rows(most, page):
+    """max_q may be far above every count; counts above it are still refused."""
+    H, D, counts, pos = 2, 64, [5, 0, 3], [7, 1, 30]
+    k, v = (torch.zeros(9, H, page, D, dtype=torch.int8, device="cuda") for _ in "kv")
+    ks, vs = (torch.ones(9, H, device="cuda") for _ in "kv")
+    c = g2.kv8_cache(k, v, ks, vs)
+    table = ints([[0, 1, 2], [3, 4, 5], [6, 7, 8]])
+    x = torch.randn(8, 3, H, D, device="cuda", generator=gen(1))
+    starts, st = ints([0, 5, 5, 8]), torch.zeros(1, dtype=torch.int32, device="cuda")
+    kw = dict(q_start=starts, max_q=most, status=st)
+    g2.kv8_append(c, x[:, 1], x[:, 2], 8, 3, table, 3, ints(pos), row_stride=3 * H * D, **kw)
+    back = torch.zeros(8, 2, H, D, device="cuda")
+    g2.kv8_gather(c, back[:, 0], back[:, 1], 8, 3, table, 3, ints(pos), row_stride=2 * H * D, **kw)
+    # a page with rows that stay keeps its scale of 1: half a step is at most half of that
+    assert int(st) == 0 and ((back - x[:, 1:]).abs() <= 0.5 * 1.001).all()
+    k5, v5, ks5, vs5, exact = torch.zeros_like(k), torch.zeros_like(v), torch.ones_like(ks), torch.ones_like(vs), dict(kw, max_q=5)
+    g2.kv8_append(g2.kv8_cache(k5, v5, ks5, vs5), x[:, 1], x[:, 2], 8, 3, table, 3, ints(pos), row_stride=3 * H * D, **exact)
+    assert all(torch.equal(a, b) for a, b in ((k, k5), (v, v5), (ks, ks5), (vs, vs5)))
+    lens, out = ints([12, 1, 33]), torch.full((8, H, D), 7.0, device="cuda")
+    ws = torch.zeros(g2.kv8_attention_workspace(c, H, 3, most), dtype=torch.uint8, device="cuda")
+    g2.kv8_attention(c, x[:, 0], out, H, 8, 3, table, 3, lens, ws, ws.numel(), q_stride=3 * H * D, **kw)
+    want = torch.full_like(out, 7.0)
+    ws5 = torch.zeros(g2.kv8_attention_workspace(c, H, 3, 5), dtype=torch.uint8, device="cuda")
+    g2.kv8_attention(c, x[:, 0], want, H, 8, 3, table, 3, lens, ws5, ws5.numel(), q_stride=3 * H * D, **exact)
+    assert int(st) == 0 and (out - want).norm() <= 2 ** -19 * want.norm() and not (out == 7).any()
+    if most == 5:
+        g2.kv8_append(c, x[:, 1], x[:, 2], 8, 3, table, 3, ints(pos), row_stride=3 * H * D, **dict(kw, max_q=4))
+        assert int(st) == -6
