@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     // A run in p pieces takes units / p steps and then a merge of p: at most kPieces workers a run (one run of
     // 40000 keys over all 296 workers: 25.2 us, 32 pieces: 13.2).
     constexpr unsigned kPieces = 32;
-    const unsigned W = min(min((unsigned)a.workers, total), all.y * kPieces);
+    const unsigned W = min(min((unsigned)a.workers, total), min(all.y, (unsigned)kMaxWorkers) * kPieces);
     const unsigned worker = blockIdx.x * GROUPS + grp;
     if (worker >= W) return;   // whole groups leave; later barriers are the groups' own
     const unsigned share = total / W, extra = total - share * W;   // the first `extra` workers have one unit more

@@ -48,3 +48,20 @@ def test_any_bound_on_the_rows(most, page):
     if most == 5:
         g2.kv8_append(c, x[:, 1], x[:, 2], 8, 3, table, 3, ints(pos), row_stride=3 * H * D, **dict(kw, max_q=4))
         assert int(st) == -6
+
+
+@pytest.mark.gpu
+def test_2_27_runs():
+    """So many (sequence, head) runs that 32 of each pass 32 bits: every output is written."""
+    S, H, D = 2 ** 22, 32, 64
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    k, v = (torch.randint(-127, 128, (1, H, 16, D), device="cuda", generator=gen(i)).to(torch.int8) for i in range(2))
+    ks, vs = (torch.full((1, H), 2.0 ** -6, device="cuda") for _ in "kv")
+    c = g2.kv8_cache(k, v, ks, vs)
+    q, out = torch.zeros(S, H, D, dtype=torch.half, device="cuda"), torch.full((S, H, D), 9.0, dtype=torch.half, device="cuda")
+    table, lens = torch.zeros(S, 1, dtype=torch.int32, device="cuda"), torch.ones(S, dtype=torch.int32, device="cuda")
+    ws = torch.zeros(g2.kv8_attention_workspace(c, H, S, 1), dtype=torch.uint8, device="cuda")
+    g2.kv8_attention(c, q, out, H, S, S, table, 1, lens, ws, ws.numel(), dtype=g2.G2_F16)
+    want = (v[0, :, 0].float() * 2.0 ** -6).half()          # one key: its value, exact in fp16
+    assert all(torch.equal(part, want.expand_as(part)) for part in out.split(2 ** 18))
