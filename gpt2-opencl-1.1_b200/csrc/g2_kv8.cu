@@ -1104,6 +1104,9 @@ int launch_attn(const AttnArgs &a, const AttnPlan &p, int sms, cudaStream_t st) 
     return p.nt == 1 ? launch_attn<FMT, 128, 1>(a, p.wpr, sms, st) : launch_attn<FMT, 128, 2>(a, p.wpr, sms, st);
 }
 
+// Positions of a table row: the attention counts up to a unit of keys past the last in 32 bits.
+constexpr long long kMaxPositions = 0x7fffff00LL;
+
 // ---- argument checks ----------------------------------------------------------------
 int check_cache(const char *who, const g2_kv8 *c) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return arg_error(G2_ERR_ARG, who, "null cache or cache array");
@@ -1127,8 +1130,8 @@ int check_rows(const char *who, const g2_kv8 *c, int heads, const void *a, const
         return arg_error(G2_ERR_RANGE, who, "need n_rows >= 0, n_seq >= 0, max_q >= 1 and table_stride >= 1");
     if (!r.q_start && (r.max_q != 1 || r.n_rows != r.n_seq))
         return arg_error(G2_ERR_RANGE, who, "without q_start n_rows is n_seq and max_q is 1");
-    if ((long long)r.table_stride * c->page_size > 0x7fffffffLL)
-        return arg_error(G2_ERR_RANGE, who, "a table row holds more than 2^31 - 1 positions");
+    if ((long long)r.table_stride * c->page_size > kMaxPositions)
+        return arg_error(G2_ERR_RANGE, who, "a table row holds more than 2^31 - 256 positions");
     const int es = dtype == G2_F32 ? 4 : 2;
     for (long long *s : {sa, sb}) {
         if (!s) continue;

@@ -278,6 +278,7 @@ int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const vo
  * head h of page p is at ((p * n_kv_head + h) * page_size + t) * head_dim + j;
  * its scale at p * n_kv_head + h.  The caller owns the memory and which pages
  * a sequence has: `table` [n_seq][table_stride] (device) lists them in order.
+ * A table row holds up to 2^31 - 256 positions.
  * All arrays below are in device memory unless said otherwise.
  *
  * Rows: with q_start NULL sequence s has the one row s (n_rows == n_seq, max_q

@@ -50,6 +50,16 @@ def test_any_bound_on_the_rows(most, page):
         assert int(st) == -6
 
 
+@pytest.mark.parametrize("name", CALLS)
+def test_longest_table(name):
+    """Positions near 2^31, where a tile past the last one no longer fits 32 bits, are refused."""
+    f = CALLS[name]
+    for page in (16, 128):
+        for last in (2 ** 31 - 128, 2 ** 31 - 256 + page):
+            assert code(lambda: f(cache(page_size=page), dict(table_stride=last // page))) == -6
+        assert code(lambda: f(cache(page_size=page, n_kv_head=1), dict(table_stride=(2 ** 31 - 256) // page, n_rows=1, n_seq=1))) == no_device_memory()
+
+
 @pytest.mark.gpu
 def test_2_27_runs():
     """So many (sequence, head) runs that 32 of each pass 32 bits: every output is written."""
