@@ -25,7 +25,7 @@ struct Rows8 {   // which rows a call is about (see gpt2b200.h)
 };
 
 struct Span {
-    int first, n;   // rows of the sequence; n = 0: none, or out of range
+    int first, n;   // rows of the sequence; n = -1: out of range
 };
 
 __device__ __forceinline__ void bad(const Rows8 &r) {
@@ -40,7 +40,7 @@ __device__ __forceinline__ Span seq_rows(const Rows8 &r, int s) {
         const long long n = (long long)next - p.first;
         if (n < 0 || n > r.max_q || p.first < 0 || p.first + n > r.n_rows) {
             bad(r);
-            return Span{0, 0};
+            return Span{0, -1};
         }
         p.n = (int)n;
     }
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kAppendThreads)
     const int s = blockIdx.x / blocks_per_seq, tile0 = blockIdx.y * TILES, n_tiles = min(TILES, 2 * c.n_kv_head - tile0);
     const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
-    if (sp.n == 0) return;
+    if (sp.n <= 0) return;
     if (p0 < 0 || (long long)p0 + sp.n > (long long)r.table_stride * P) {
         bad(r);
         return;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(256) kv8_append_token_kernel(g2_kv8 c, const T
     if (tile >= 2 * c.n_kv_head) return;
     const int p = pos[s];
     const Span sp = seq_rows(r, s);
-    if (sp.n == 0) return;
+    if (sp.n <= 0) return;
     if (p < 0 || p >= (long long)r.table_stride * P) {
         bad(r);
         return;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256)
     const int P = c.page_size, D = c.head_dim, per_row = c.n_kv_head * D / 4;
     const int p0 = pos[s];
     const Span sp = seq_rows(r, s);
-    if (sp.n == 0) return;
+    if (sp.n <= 0) return;
     if (p0 < 0 || (long long)p0 + sp.n > (long long)r.table_stride * P) {
         bad(r);
         return;
@@ -522,7 +522,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, int s) {
     const Span sp = seq_rows(a.r, s);
     w.first = sp.first;
     w.n = sp.n;
-    if (!sp.n) return w;
+    if (sp.n <= 0) return w;
     if (w.len < 0 || w.len > (long long)a.r.table_stride * a.c.page_size) {
         bad(a.r);
         w.n = 0;
@@ -558,9 +558,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     // ---- the units before every `per` sequences
     const int per = (n_seq + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
     unsigned my_units = 0, my_runs = 0, longest = 0;
+    bool skipped = false;
     for (int s = tid * per; s < min(n_seq, (tid + 1) * per); ++s) {
         const SeqWork w = seq_work<COLS>(a, s);
         if (per == 1) cached[tid] = w;
+        skipped |= w.n < 0;
         my_units += w.total;
         my_runs += w.runs;
         if (w.runs) longest = max(longest, (unsigned)w.len);
@@ -570,7 +572,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
                                    __reduce_max_sync(0xffffffffu, longest), 0);
         if (lane == 0) warp_sum[warp] = x;
     }
-    __syncthreads();
+    if (__syncthreads_or(skipped)) {
+        // The host allowed for n_rows rows; where a count was below 0, others may overlap and be more.
+        __shared__ unsigned long long units;
+        if (tid == 0) units = 0;
+        __syncthreads();
+        for (int s = tid; s < n_seq; s += kAttnWarps * 32) atomicAdd(&units, (unsigned long long)seq_work<COLS>(a, s).total);
+        __syncthreads();
+        if (units > 0x7fffffffULL) {
+            bad(a.r);
+            return;
+        }
+    }
     uint4 before = make_uint4(0, 0, 0, 0), all = before;
 #pragma unroll
     for (int i = 0; i < kAttnWarps; ++i) {
@@ -1248,10 +1261,12 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if ((rc = check_rows(who, cache, n_head, q, out, dtype, &q_stride, &out_stride, r, seq_len))) return rc;
     r.max_q = bound_rows(max_q, n_rows);
     if ((long long)r.max_q * n_seq > 0x7fffffffLL) return arg_error(G2_ERR_RANGE, who, "too many rows");
-    {   // the kernel counts units in 32 bits
+    {   // the kernel counts units in 32 bits: those of the longest sequences, for each group of query columns (the last
+        // of a sequence may be part full)
         const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, 1);
-        const double units = ((double)table_stride * cache->page_size / p.unit + 1 + p.ahead) * n_seq * cache->n_kv_head *
-                             ((double)r.max_q * (n_head / cache->n_kv_head) / (4 * p.nt) + 1);
+        const double columns = (double)std::min((long long)r.max_q * n_seq, (long long)n_rows) * (n_head / cache->n_kv_head);
+        const double units = ((double)table_stride * cache->page_size / p.unit + 1 + p.ahead) * cache->n_kv_head *
+                             (columns / (4 * p.nt) + std::min(n_seq, n_rows));
         if (units > 2147483647.0) return arg_error(G2_ERR_RANGE, who, "too much work for one call");
     }
     if (!workspace || !aligned(workspace, 256)) return arg_error(G2_ERR_ARG, who, "workspace not 256-byte aligned");

@@ -292,6 +292,8 @@ int g2k_matvec_q4(const void *x, const void *packed, const float *bias, const vo
  * A sequence with a count outside [0, max_q], rows outside [0, n_rows), or a
  * position or length outside its table row is skipped, and so is a page whose
  * id is outside [0, n_pages); *status (may be NULL) then becomes G2_ERR_RANGE.
+ * (Attention skips them all where the others' rows overlap and add up to more
+ * work than a call can count.)
  * It is never cleared here.
  *
  * Codes of rows in use are finite and scales positive or NaN; what other rows and

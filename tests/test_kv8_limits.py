@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import gpt2b200 as g2  # noqa: E402
-from test_operator_args import CALLS, cache, code, no_device_memory  # noqa: E402
+from test_operator_args import A as CALLS_A, CALLS, cache, code, no_device_memory  # noqa: E402
 
 
 def gen(seed):
@@ -60,6 +60,16 @@ def test_longest_table(name):
         assert code(lambda: f(cache(page_size=page, n_kv_head=1), dict(table_stride=(2 ** 31 - 256) // page, n_rows=1, n_seq=1))) == no_device_memory()
 
 
+def test_work_goes_by_the_rows_there_are():
+    """One long prompt among many sequences with long tables: max_q times n_seq is far above the rows."""
+    f = CALLS["attention"]
+    call = dict(heads=32, n_seq=256, n_rows=2048 + 255, max_q=2048, q_start=CALLS_A, table_stride=8192)
+    assert code(lambda: f(cache(n_kv_head=8), dict(call))) == no_device_memory()
+    # as many rows as max_q allows is too much for the kernel's 32-bit counts
+    assert code(lambda: f(cache(n_kv_head=8), dict(call, n_rows=2048 * 256, max_q=2048))) == -6
+    assert code(lambda: f(cache(n_kv_head=8), dict(call, n_seq=2 ** 22, n_rows=2 ** 22))) == -6
+
+
 @pytest.mark.gpu
 def test_2_27_runs():
     """So many (sequence, head) runs that 32 of each pass 32 bits: every output is written."""
@@ -75,3 +85,21 @@ def test_2_27_runs():
     g2.kv8_attention(c, q, out, H, S, S, table, 1, lens, ws, ws.numel(), dtype=g2.G2_F16)
     want = (v[0, :, 0].float() * 2.0 ** -6).half()          # one key: its value, exact in fp16
     assert all(torch.equal(part, want.expand_as(part)) for part in out.split(2 ** 18))
+
+
+@pytest.mark.gpu
+def test_overlapping_rows_past_a_calls_work():
+    """q_start that runs back and forth: half of the sequences have all the rows, together too much to count."""
+    S, R, H, page, blocks = 4096, 64, 32, 128, 8192
+    k = torch.ones(1, H, page, 64, dtype=torch.int8, device="cuda")
+    c = g2.kv8_cache(k, k.clone(), torch.ones(1, H, device="cuda"), torch.ones(1, H, device="cuda"))
+    q, out = torch.ones(R, H, 64, device="cuda"), torch.full((R, H, 64), 7.0, device="cuda")
+    table, st = torch.zeros(S, blocks, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    back_and_forth = ints([0, R] * (S // 2) + [0])
+    ws = torch.zeros(g2.kv8_attention_workspace(c, H, S, R), dtype=torch.uint8, device="cuda")
+    kw = dict(q_start=back_and_forth, max_q=R, status=st)
+    g2.kv8_attention(c, q, out, H, R, S, table, blocks, torch.full((S,), page * blocks, dtype=torch.int32, device="cuda"), ws, ws.numel(), **kw)
+    assert int(st) == -6 and (out == 7).all() and not ws[:4096 * 4].any()
+    st.zero_()   # few enough: the sequences with rows are computed
+    g2.kv8_attention(c, q, out, H, R, S, table, blocks, torch.full((S,), 70, dtype=torch.int32, device="cuda"), ws, ws.numel(), **kw)
+    assert int(st) == -6 and (out == 1).all()
