@@ -785,8 +785,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
         unsigned qf[NT][KS][2];
         float qfac[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {   // columns past the last hold anything: they are not written
-            qfac[n] = n * 4 + t < cols ? qfac_s[grp][n * 4 + t] : 0.0f;
+        for (int n = 0; n < NT; ++n) {   // columns past the last hold anything: as NaN they never raise a reference
+            qfac[n] = n * 4 + t < cols ? qfac_s[grp][n * 4 + t] : __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 qf[n][k][0] = qs[((n * KS + k) * 2) * 32 + lane];
