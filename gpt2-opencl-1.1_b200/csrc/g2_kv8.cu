@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(256)
     unsigned w[kGatherRows];
 #pragma unroll
     for (int j = 0; j < kGatherRows; ++j)
-        if (j >= j0 && j < j1) w[j] = __ldg(src + j * (D / 4));
+        if (j >= j0 && j < j1) w[j] = src[j * (D / 4)];   // plain loads: the kernel before may write codes until the wait
 #pragma unroll
     for (int j = 0; j < kGatherRows; ++j)
         if (j >= j0 && j < j1) {

@@ -53,3 +53,36 @@ def test_bits_after_other_kernels(g2, fmt, D):
         got.append(attend(g2, c, q, n * P, table))
     assert got[0].isfinite().all()
     assert all(torch.equal(got[0], g) for g in got[1:])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_read_back_right_after_writing(g2, fmt):
+    """append, gather and attention one after the other, each started while the one before runs, on the same pages."""
+    H, P, D, S, n = 16, 32, 64, 6, 90
+    f = g2.G2_KV_E4M3 if fmt == "e4m3" else g2.G2_KV_I8
+    k, v = (torch.zeros(S * 3, H, P, D, dtype=torch.int8, device="cuda") for _ in "kv")
+    ks, vs = (torch.ones(S * 3, H, device="cuda") for _ in "kv")
+    c = g2.kv8_cache(k, v, ks, vs, f)
+    table = torch.arange(S * 3, dtype=torch.int32, device="cuda").view(S, 3)
+    pos, starts = torch.zeros(S, dtype=torch.int32, device="cuda"), torch.arange(0, S * n + 1, n, dtype=torch.int32, device="cuda")
+    x = torch.randn(8, 2, S * n, H, D, device="cuda", generator=gen(4))
+    back, outs = torch.zeros_like(x), torch.zeros(8, S, H, D, device="cuda")
+    ws = torch.zeros(g2.kv8_attention_workspace(c, H, S, 1), dtype=torch.uint8, device="cuda")
+    kw, lens = dict(q_start=starts, max_q=n), torch.full((S,), n, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+
+    def step(i, wait):
+        for call in (lambda: g2.kv8_append(c, x[i, 0], x[i, 1], S * n, S, table, 3, pos, **kw),
+                     lambda: g2.kv8_gather(c, back[i, 0], back[i, 1], S * n, S, table, 3, pos, **kw),
+                     lambda: g2.kv8_attention(c, x[i, 0, :S], outs[i], H, S, S, table, 3, lens, ws, ws.numel())):
+            call()
+            if wait:
+                torch.cuda.synchronize()
+    for i in range(8):
+        step(i, False)
+    torch.cuda.synchronize()
+    got = back.clone(), outs.clone()
+    for i in range(8):
+        step(i, True)
+    assert torch.equal(got[0], back) and torch.equal(got[1], outs)
+    assert ((back - x).abs() <= x.abs().max() / 14).all()       # half a step of e4m3 at its largest is 1 / 28 of it
