@@ -405,11 +405,13 @@ __global__ void __launch_bounds__(256)
 //   scores   keys on m, query columns on n;
 //   outputs  dimensions on m, query columns on n, keys on k.
 // Eight columns are more than a few queries fill, so each query takes several.
-// int8 keys meet the four bytes of a fixed-point q (30 bits below a power of two
-// over its largest) in m16n8k32 products, exactly and without any conversion of
+// int8 keys meet the six bytes of a fixed-point q (46 bits below a power of two
+// over its largest: keys whose codes are 0 at a query's large values must not
+// inherit their step) in m16n8k32 products, exactly and without any conversion of
 // the keys.  e4m3 keys, and the values of both formats, become fp16 exactly and
 // meet two fp16 columns, the rounding of q or of a weight and 2^11 times the rest
-// (22 bits).  All columns of a query lie in the same threads, so neither product
+// (22 bits of its own; q is scaled to 2^14 at its largest, so that this holds 2^28
+// below it).  All columns of a query lie in the same threads, so neither product
 // needs a shuffle; `movmatrix` turns the weights into the second one's operand.
 // Operand orders are permuted (dimensions of the scores' k, of the outputs' m) so
 // that every thread reads 8 or 16 consecutive bytes; the ring's slots are swizzled
@@ -427,7 +429,9 @@ struct AttnRing {
     static constexpr int kBlocks = D * NT >= 256 ? 1 : 2;   // CTAs per SM; wide column groups need the registers of two
     static constexpr int kStages = (D == 64 ? 6 : 3) * (kBlocks == 1 ? 2 : 1);
     static constexpr int kTileBytes = 32 * D;               // 16 keys' K and V codes
-    static constexpr int kSmem = kAttnWarps * kStages * (kTileBytes + 8);
+    static constexpr int kLowBytes = 8 * D * NT;            // the last two of six bytes of a run's queries
+    template <int FMT, int WPR>
+    static constexpr int kSmem = kAttnWarps * kStages * (kTileBytes + 8) + (FMT == G2_KV_I8 ? kAttnWarps / WPR * kLowBytes : 0);
 };
 
 struct AttnArgs {
@@ -647,6 +651,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
     unsigned char *slots = ring + warp * S * TILE;
     float *meta = reinterpret_cast<float *>(ring + kAttnWarps * S * TILE) + warp * S * 2;   // K and V scale; -1: no page
     float *merge = reinterpret_cast<float *>(ring + grp * WPR * S * TILE);                  // [WPR][PART]
+    uint4 *low = reinterpret_cast<uint4 *>(ring + kAttnWarps * S * (TILE + 8) + grp * AttnRing<D, NT>::kLowBytes);   // [NT][lane][KS / 4]
     const unsigned slots_addr = smem_addr(slots), meta_addr = smem_addr(meta) + lane * 4;   // lanes 0 and 1 bring the scales
     const unsigned char *k_lane = static_cast<const unsigned char *>(a.c.k) + lane * 16, *v_lane = static_cast<const unsigned char *>(a.c.v) + lane * 16;
     const float *scale_lane = lane ? a.c.v_scale : a.c.k_scale;
@@ -750,17 +755,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             const int d = lane * 4;
             const unsigned peak = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
             // a power of two below the largest (2^e <= it < 2^(e + 1)), so that no type's range matters
-            const int e = max(INT ? -96 : -126, min(INT ? 127 : 126, (int)(peak >> 23) - 127));   // fp16 parts may reach 4
-            const float down = __uint_as_float((unsigned)(127 + (INT ? 29 : 0) - e) << 23);
-            const float up = __uint_as_float((unsigned)(127 + e) << 23) * (INT ? 0x1p-29f : 1.0f);
+            const int e = max(INT ? -96 : -112, (int)(peak >> 23) - 127);
+            const float down = __uint_as_float((unsigned)(127 + (INT ? 29 : 14) - min(e, 127)) << 23);
+            const float up = __uint_as_float((unsigned)(127 + min(e, 127)) << 23) * (INT ? 0x1p-29f : 0x1p-14f);
             if (lane == 0) qfac_s[grp][c] = (peak >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : up) * a.scale_log2e;
             const int k = (d >> 6) * 4 + ((d >> 2) & 3);   // thread (d & 63) >> 4 of a quad has these four dimensions
             unsigned *at = qs + ((c >> 2) * KS * 2) * 32 + (c & 3) * 8 + ((d & 63) >> 4);
             if (d < D) {
                 if (INT) {
-                    // signed bytes: adding 128 to each of the lower three carries into the next
-                    auto digits = [&](float v) { return ((unsigned)__float2int_rn(v * down) + 0x00808080u) ^ 0x00808080u; };
-                    const unsigned y0 = digits(x.x), y1 = digits(x.y), y2 = digits(x.z), y3 = digits(x.w);
+                    // signed bytes: adding 128 to each of the lower ones carries into the next
+                    unsigned z[4];   // 2^15 times what the upper four bytes leave (exact: they have at most the bits of v)
+                    auto digits = [&](float v, int i) {
+                        const int n = __float2int_rn(v * down);
+                        z[i] = ((unsigned)__float2int_rn((v * down - (float)n) * 0x1p15f) + 0x0080u) ^ 0x0080u;
+                        return ((unsigned)n + 0x00808080u) ^ 0x00808080u;
+                    };
+                    const unsigned y0 = digits(x.x, 0), y1 = digits(x.y, 1), y2 = digits(x.z, 2), y3 = digits(x.w, 3);
+                    const unsigned z01 = __byte_perm(z[0], z[1], 0x5140), z23 = __byte_perm(z[2], z[3], 0x5140);
+                    unsigned *lo = reinterpret_cast<unsigned *>(low) + ((c >> 2) * 32 + (c & 3) * 8 + ((d & 63) >> 4)) * KS + k;
+                    lo[0] = __byte_perm(z01, z23, 0x7632);
+                    lo[4 * KS] = __byte_perm(z01, z23, 0x5410);
                     const unsigned a01 = __byte_perm(y0, y1, 0x7362), a23 = __byte_perm(y2, y3, 0x7362);   // bytes 2 and 3
                     const unsigned b01 = __byte_perm(y0, y1, 0x5140), b23 = __byte_perm(y2, y3, 0x5140);   // bytes 0 and 1
                     at += ((k >> 1) * 2 + (k & 1)) * 32;
@@ -817,11 +831,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
             // ---- scores
             float sc[NT][2];   // of keys g and g + 8
             if constexpr (INT) {
-                int s[NT][2][4];
+                int s[NT][3][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0;
+                    for (int i = 0; i < 3; ++i) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0;
 #pragma unroll
                 for (int b = 0; b < D / 64; ++b) {
                     const int c = D == 64 ? t : (b * 4 + t) ^ ((g & 1) << 2);
@@ -829,17 +843,22 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
                     const uint4 r1 = *reinterpret_cast<const uint4 *>(slot + (g + 8) * D + c * 16);
                     const unsigned f0[4] = {r0.x, r1.x, r0.y, r1.y}, f1[4] = {r0.z, r1.z, r0.w, r1.w};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             mma16832(s[n][i], f0, qf[n][i * (KS / 2) + b * 2][0], qf[n][i * (KS / 2) + b * 2][1]);
                             mma16832(s[n][i], f1, qf[n][i * (KS / 2) + b * 2 + 1][0], qf[n][i * (KS / 2) + b * 2 + 1][1]);
                         }
+                        const uint4 lo = low[(n * 32 + lane) * (KS / 4) + b];
+                        mma16832(s[n][2], f0, lo.x, lo.y);
+                        mma16832(s[n][2], f1, lo.z, lo.w);
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    sc[n][0] = fmaf((float)(s[n][0][0] * 256 + s[n][0][1]), 65536.0f, (float)(s[n][1][0] * 256 + s[n][1][1]));
-                    sc[n][1] = fmaf((float)(s[n][0][2] * 256 + s[n][0][3]), 65536.0f, (float)(s[n][1][2] * 256 + s[n][1][3]));
+                    auto pair = [&](int i, int j) { return (float)(s[n][i][2 * j] * 256 + s[n][i][2 * j + 1]); };
+                    sc[n][0] = fmaf(pair(0, 0), 65536.0f, fmaf(pair(2, 0), 0x1p-15f, pair(1, 0)));
+                    sc[n][1] = fmaf(pair(0, 1), 65536.0f, fmaf(pair(2, 1), 0x1p-15f, pair(1, 1)));
                 }
             } else {
                 float s[NT][4];
@@ -1097,11 +1116,11 @@ int attn_sms() {
 template <int FMT, int D, int NT, int WPR>
 int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
     auto kernel = kv8_attention_kernel<FMT, D, NT, WPR>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (AttnRing<D, NT>::kSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (AttnRing<D, NT>::template kSmem<FMT, WPR>)) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_kv8_attention", cudaGetErrorString(cudaGetLastError()));
     const int per_cta = kAttnWarps / WPR;
     return launch_status("g2k_kv8_attention", launch_pdl(kernel, dim3((a.workers + per_cta - 1) / per_cta), dim3(kAttnWarps * 32),
-                                                         (AttnRing<D, NT>::kSmem), st, a));
+                                                         (AttnRing<D, NT>::template kSmem<FMT, WPR>), st, a));
 }
 
 template <int FMT, int D, int NT>

@@ -332,7 +332,9 @@ int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int dtype, lon
  * n rows in sequence s and seq_len[s] tokens in its cache (the new ones
  * included), row j attends to positions 0 .. seq_len[s] - n + j; a row with no
  * position gives zeros.  Query head h reads K/V head h / (n_head / n_kv_head).
- * q and out are of `dtype`; sums are fp32, and so is the accuracy of G2_F32.
+ * q and out are of `dtype`; sums are fp32.  A q is carried exactly but for what
+ * lies below 2^-44 of its row's largest (over e4m3 keys to 22 bits of its own, or
+ * to 2^-50 of the largest), a weight to 21 bits of its own.
  * scale multiplies q . k (1 / sqrt(head_dim)).  Keys of a skipped page count
  * as absent.  `workspace` holds g2k_kv8_attention_workspace() bytes,
  * 256-byte aligned, zero-filled before its first use; each call leaves it ready
