@@ -410,16 +410,17 @@ __global__ void __launch_bounds__(256)
 // inherit their step) in m16n8k32 products, exactly and without any conversion of
 // the keys.  e4m3 keys, and the values of both formats, become fp16 exactly and
 // meet two fp16 columns, the rounding of q or of a weight and 2^11 times the rest
-// (22 bits of its own; q is scaled to 2^14 at its largest, so that this holds 2^28
-// below it).  All columns of a query lie in the same threads, so neither product
+// (22 bits of its own; q is scaled to 2^14 and weights to 2^7 at their largest, so
+// that this holds 2^28 and 2^21 below it).  All columns of a query lie in the same threads, so neither product
 // needs a shuffle; `movmatrix` turns the weights into the second one's operand.
 // Operand orders are permuted (dimensions of the scores' k, of the outputs' m) so
 // that every thread reads 8 or 16 consecutive bytes; the ring's slots are swizzled
 // so that those reads have no bank conflicts.
 //
-// The running reference m is raised only when a score exceeds it by 2^8: one
-// vote a tile in place of a maximum over the warp.
+// The running reference m is raised, to 2^-7 of the largest weight, only when a
+// score exceeds it by 2^15: one vote a tile in place of a maximum over the warp.
 constexpr int kAttnWarps = 8;
+constexpr float kLead = 7.0f, kLag = 15.0f;   // powers of two of the reference's largest weight and of weights until it is raised
 constexpr int kMaxWorkers = 4096;   // counters at the start of the workspace
 constexpr float kLoScale = 2048.0f, kLoUnscale = 1.0f / 2048.0f;
 constexpr float kNoMax = -3.402823466e38f;    // reference of a column that has seen no key: no finite score is below it
@@ -902,12 +903,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, (AttnRing<D, NT>::kBlocks)) k
                     if (key0 + g >= lim[n]) w[n][0] = -INFINITY;
                     if (key0 + g + 8 >= lim[n]) w[n][1] = -INFINITY;
                 }
-                raise |= fmaxf(w[n][0], w[n][1]) > mref[n] + 8.0f;
+                raise |= fmaxf(w[n][0], w[n][1]) > mref[n] + kLag;
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float m = fmaxf(fmaxf(w[n][0], w[n][1]), mref[n]);
+                    float m = fmaxf(fmaxf(w[n][0], w[n][1]) - kLead, mref[n]);
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));

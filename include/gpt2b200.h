@@ -334,7 +334,8 @@ int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int dtype, lon
  * position gives zeros.  Query head h reads K/V head h / (n_head / n_kv_head).
  * q and out are of `dtype`; sums are fp32.  A q is carried exactly but for what
  * lies below 2^-44 of its row's largest (over e4m3 keys to 22 bits of its own, or
- * to 2^-50 of the largest), a weight to 21 bits of its own.
+ * to 2^-50 of the largest), a weight times its V scale to 21 bits of its own or
+ * to 2^-42 of the row's largest.  V scales that a row sees lie within 2^126.
  * scale multiplies q . k (1 / sqrt(head_dim)).  Keys of a skipped page count
  * as absent.  `workspace` holds g2k_kv8_attention_workspace() bytes,
  * 256-byte aligned, zero-filled before its first use; each call leaves it ready

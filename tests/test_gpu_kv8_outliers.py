@@ -87,3 +87,20 @@ def test_fp16_queries_of_all_sizes(g2, fmt):
     q[..., 5] = 60000.0
     s = torch.full((7, H), 0.5, device="cuda")
     check(g2, fmt, k, v, s, s, q.half(), n, 1.0)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("gap", [15.0, 17.3, 18.3, 19.7, 20.1])
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_weights_beside_a_large_one(g2, fmt, gap, D):
+    """The first key takes nearly all of the weight and has a value of 0: what is left are weights e^-gap of it."""
+    H, P, n = 2, 64, 16
+    k = torch.zeros(4, H, P, D, dtype=torch.int8, device="cuda")
+    one = codes(torch.ones(1, device="cuda"), fmt)
+    k[0, :, 0, 0] = one
+    v = codes(70 + 20 * torch.rand(4, H, P, D, device="cuda", generator=gen(4)), fmt)
+    v[0, :, 0] = 0
+    q = torch.zeros(1, H, D, device="cuda")
+    q[..., 0] = gap
+    s = torch.ones(4, H, device="cuda")
+    check(g2, fmt, k, v, s, s, q, n, 1.0)
