@@ -405,6 +405,20 @@ def _sized(t, size):
     return t.data_ptr()
 
 
+_names = {}   # torch dtypes' names
+
+
+def _real(t, dtype):
+    """_addr of a tensor of fp32, or fp16 where `dtype` is G2_F16."""
+    if t is None or t.__class__ is int:
+        return t
+    d = t.dtype
+    name = _names.get(d) or _names.setdefault(d, str(d))
+    if name != ("torch.float16" if dtype else "torch.float32"):
+        raise G2Error(-1, f"a tensor is of {name}, not torch.{'float16' if dtype else 'float32'}")
+    return t.data_ptr()
+
+
 def q4_bytes(N: int, K: int, group: int) -> int:
     """Bytes of a [K, N] weight matrix packed in 4 bits (0 for a bad shape or group)."""
     return lib.g2k_q4_bytes(N, K, group)
@@ -412,20 +426,19 @@ def q4_bytes(N: int, K: int, group: int) -> int:
 
 def q4_pack(W, packed, N, K, group, transposed=False, dtype=G2_F32, stream=0):
     """Quantise W ([K, N], or [N, K] if transposed) to 4 bits with a scale for each `group` rows of a column."""
-    check(lib.g2k_q4_pack(_sized(W, 2 if dtype else 4), dtype, int(transposed), _addr(packed), N, K, group, stream))
+    check(lib.g2k_q4_pack(_real(W, dtype), dtype, int(transposed), _addr(packed), N, K, group, stream))
 
 
 def q4_unpack(packed, W, N, K, group, stream=0):
     """The values of a packed matrix, fp32 [K, N]."""
-    check(lib.g2k_q4_unpack(_addr(packed), _sized(W, 4), N, K, group, stream))
+    check(lib.g2k_q4_unpack(_addr(packed), _real(W, G2_F32), N, K, group, stream))
 
 
 def matvec_q4(x, packed, y, M, N, K, group, bias=None, residual=None, gelu=False, ln_gamma=None, ln_beta=None,
               dtype=G2_F32, stream=0):
     """y [M, N] = x' [M, K] times a packed [K, N] matrix; M up to 16 rows; x, residual and y of `dtype`."""
-    e = 2 if dtype else 4
-    check(lib.g2k_matvec_q4(_sized(x, e), _addr(packed), _sized(bias, 4), _sized(residual, e), _sized(y, e), dtype, M, N, K,
-                            group, int(gelu), _sized(ln_gamma, 4), _sized(ln_beta, 4), stream))
+    check(lib.g2k_matvec_q4(_real(x, dtype), _addr(packed), _real(bias, G2_F32), _real(residual, dtype), _real(y, dtype), dtype, M,
+                            N, K, group, int(gelu), _real(ln_gamma, G2_F32), _real(ln_beta, G2_F32), stream))
 
 
 def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
@@ -434,12 +447,11 @@ def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
     shape = tuple(k.shape)
     if len(shape) != 4 or tuple(v.shape) != shape or k.element_size() != 1 or v.element_size() != 1:
         raise G2Error(-1, "k and v are one-byte tensors [n_pages, n_kv_head, page_size, head_dim]")
-    if tuple(k_scale.shape) != shape[:2] or tuple(v_scale.shape) != shape[:2] or k_scale.element_size() != 4 \
-            or v_scale.element_size() != 4:
+    if tuple(k_scale.shape) != shape[:2] or tuple(v_scale.shape) != shape[:2]:
         raise G2Error(-1, "the scales are fp32 tensors [n_pages, n_kv_head]")
     if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
         raise G2Error(-1, "the cache's tensors are not contiguous")
-    c = KV8(_addr(k), _addr(v), _addr(k_scale), _addr(v_scale), *shape, fmt)
+    c = KV8(_addr(k), _addr(v), _real(k_scale, G2_F32), _real(v_scale, G2_F32), *shape, fmt)
     c.tensors = (k, v, k_scale, v_scale)
     return c
 
@@ -447,16 +459,14 @@ def kv8_cache(k, v, k_scale, v_scale, fmt=G2_KV_I8) -> KV8:
 def kv8_append(cache, k, v, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0, dtype=G2_F32,
                status=None, stream=0):
     """Write K and V rows of new tokens into the pages of their sequences (g2k_kv8_append)."""
-    e = 2 if dtype else 4
-    check(lib.g2k_kv8_append(C.byref(cache), _sized(k, e), _sized(v, e), dtype, row_stride, n_rows, n_seq, _sized(q_start, 4),
+    check(lib.g2k_kv8_append(C.byref(cache), _real(k, dtype), _real(v, dtype), dtype, row_stride, n_rows, n_seq, _sized(q_start, 4),
                              _sized(pos, 4), max_q, _sized(table, 4), table_stride, _sized(status, 4), stream))
 
 
 def kv8_gather(cache, k_out, v_out, n_rows, n_seq, table, table_stride, pos, q_start=None, max_q=1, row_stride=0,
                dtype=G2_F32, status=None, stream=0):
     """Read rows of the cache back as values (g2k_kv8_gather)."""
-    e = 2 if dtype else 4
-    check(lib.g2k_kv8_gather(C.byref(cache), _sized(k_out, e), _sized(v_out, e), dtype, row_stride, n_rows, n_seq,
+    check(lib.g2k_kv8_gather(C.byref(cache), _real(k_out, dtype), _real(v_out, dtype), dtype, row_stride, n_rows, n_seq,
                              _sized(q_start, 4), _sized(pos, 4), max_q, _sized(table, 4), table_stride, _sized(status, 4), stream))
 
 
@@ -467,8 +477,7 @@ def kv8_attention_workspace(cache, n_head: int, n_seq: int, max_q: int = 1) -> i
 def kv8_attention(cache, q, out, n_head, n_rows, n_seq, table, table_stride, seq_len, workspace, workspace_bytes,
                   q_start=None, max_q=1, scale=None, q_stride=0, out_stride=0, dtype=G2_F32, status=None, stream=0):
     """Softmax attention of query rows over the cache (g2k_kv8_attention); scale defaults to head_dim ** -0.5."""
-    e = 2 if dtype else 4
-    check(lib.g2k_kv8_attention(C.byref(cache), _sized(q, e), q_stride, _sized(out, e), out_stride, dtype, n_head,
+    check(lib.g2k_kv8_attention(C.byref(cache), _real(q, dtype), q_stride, _real(out, dtype), out_stride, dtype, n_head,
                                 cache.head_dim ** -0.5 if scale is None else scale, n_rows, n_seq, _sized(q_start, 4),
                                 _sized(seq_len, 4), max_q, _sized(table, 4), table_stride, _addr(workspace), workspace_bytes,
                                 _sized(status, 4), stream))
@@ -480,13 +489,14 @@ def logit_rules(ctx=None, ctx_start=None, n_prompt=None, rep_penalty=None, prese
     arrays = (ctx, ctx_start, n_prompt, rep_penalty, presence, frequency, bias_ids, bias, bias_start, mask)
     if bias is not None and (bias_ids is None or bias_ids.numel() != bias.numel()):
         raise G2Error(-1, "bias_ids and bias are not of one length")
-    p = [_sized(t, 4) for t in arrays]
-    r = LogitRules(*p[:3], 0 if ctx is None else ctx.numel(), *p[3:9], 0 if bias is None else bias.numel(), p[9], mask_stride)
+    r = LogitRules(_sized(ctx, 4), _sized(ctx_start, 4), _sized(n_prompt, 4), 0 if ctx is None else ctx.numel(),
+                   _real(rep_penalty, G2_F32), _real(presence, G2_F32), _real(frequency, G2_F32), _sized(bias_ids, 4),
+                   _real(bias, G2_F32), _sized(bias_start, 4), 0 if bias is None else bias.numel(), _sized(mask, 4), mask_stride)
     r.tensors = arrays
     return r
 
 
 def process_logits(logits, out, rows, vocab_size, rules, ld=0, ld_out=0, stream=0):
     """Apply `rules` to rows of logits (out may be logits); a row stride of 0 means vocab_size."""
-    check(lib.g2k_process_logits(_sized(logits, 4), ld or vocab_size, _sized(out, 4), ld_out or vocab_size, rows, vocab_size,
+    check(lib.g2k_process_logits(_real(logits, G2_F32), ld or vocab_size, _real(out, G2_F32), ld_out or vocab_size, rows, vocab_size,
                                  C.byref(rules), stream))
