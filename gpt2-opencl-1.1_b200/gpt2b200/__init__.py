@@ -391,6 +391,7 @@ def attention(q, K, V, out, n_head, max_seq, T_kv, workspace, workspace_bytes, s
 
 
 # ---- 4-bit weights, the 8-bit paged cache, rules on logits: kernels on device pointers ----
+# Tensors are contiguous but for the row strides that a call takes; only their element types are checked.
 def _addr(t):
     """The address of a tensor, or an int (a device address); the library refuses other memory than the current device's."""
     return t if t is None or t.__class__ is int else t.data_ptr()
@@ -405,17 +406,18 @@ def _sized(t, size):
     return t.data_ptr()
 
 
-_names = {}   # torch dtypes' names
+_real_types = [None, None]   # torch.float32, torch.float16, once a tensor has been seen
 
 
 def _real(t, dtype):
     """_addr of a tensor of fp32, or fp16 where `dtype` is G2_F16."""
     if t is None or t.__class__ is int:
         return t
-    d = t.dtype
-    name = _names.get(d) or _names.setdefault(d, str(d))
-    if name != ("torch.float16" if dtype else "torch.float32"):
-        raise G2Error(-1, f"a tensor is of {name}, not torch.{'float16' if dtype else 'float32'}")
+    if t.dtype is not _real_types[1 if dtype else 0]:
+        import torch
+        _real_types[:] = torch.float32, torch.float16
+        if t.dtype is not _real_types[1 if dtype else 0]:
+            raise G2Error(-1, f"a tensor is of {t.dtype}, not {_real_types[1 if dtype else 0]}")
     return t.data_ptr()
 
 
@@ -489,6 +491,8 @@ def logit_rules(ctx=None, ctx_start=None, n_prompt=None, rep_penalty=None, prese
     arrays = (ctx, ctx_start, n_prompt, rep_penalty, presence, frequency, bias_ids, bias, bias_start, mask)
     if bias is not None and (bias_ids is None or bias_ids.numel() != bias.numel()):
         raise G2Error(-1, "bias_ids and bias are not of one length")
+    if not all(t is None or t.__class__ is int or t.is_contiguous() for t in arrays):
+        raise G2Error(-1, "an array of the rules is not contiguous")
     r = LogitRules(_sized(ctx, 4), _sized(ctx_start, 4), _sized(n_prompt, 4), 0 if ctx is None else ctx.numel(),
                    _real(rep_penalty, G2_F32), _real(presence, G2_F32), _real(frequency, G2_F32), _sized(bias_ids, 4),
                    _real(bias, G2_F32), _sized(bias_start, 4), 0 if bias is None else bias.numel(), _sized(mask, 4), mask_stride)

@@ -36,3 +36,10 @@ def test_cache_scales_and_rules():
             g2.logit_rules(**bad)
     with pytest.raises(g2.G2Error, match="torch"):
         g2.process_logits(I, I, 1, 64, g2.logit_rules())
+
+
+def test_rules_are_contiguous():
+    """The rules' lengths are those of the tensors, so every other element would be read as the next one."""
+    for bad in (dict(ctx=I[::2]), dict(mask=I[::2]), dict(bias=torch.zeros(64)[::2], bias_ids=I[:32]), dict(rep_penalty=torch.zeros(64)[::2])):
+        with pytest.raises(g2.G2Error, match="contiguous"):
+            g2.logit_rules(**bad)
