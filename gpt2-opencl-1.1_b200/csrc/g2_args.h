@@ -1,4 +1,4 @@
-// g2_args.h -- argument checks of the single-kernel entry points that take many
+// g2_args.h -- host side of the single-kernel entry points that take many
 // device pointers (g2k_matvec_q4, g2k_kv8_*, g2k_process_logits).
 #pragma once
 #include <cuda_runtime.h>
@@ -48,5 +48,15 @@ inline int launch_status(const char *who, cudaError_t r) {
     return r == cudaSuccess ? G2_OK : arg_error(G2_ERR_CUDA, who, cudaGetErrorString(r));
 }
 inline int launch_status(const char *who) { return launch_status(who, cudaGetLastError()); }
+
+// SMs of the current device (a B200's where there is none to ask).
+inline int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    return n > 0 ? n : 148;
+}
 
 }  // namespace g2

@@ -11,6 +11,7 @@
 
 #include "g2_args.h"
 #include "g2_device.cuh"
+#include "g2_mma.cuh"
 
 namespace g2 {
 
@@ -450,27 +451,8 @@ struct AttnArgs {
     float *parts;            // [workers][2][columns * (D + 2)]
 };
 
-__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(unsigned dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async4(unsigned dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16832(int (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
     unsigned r;
@@ -493,14 +475,7 @@ __device__ __forceinline__ float log2_fast(float x) {
     return y;
 }
 
-// v = hi + lo / 2048 as a pair of fp16 (hi in the low half)
-__device__ __forceinline__ unsigned split_half(float v) {
-    const __half h = __float2half_rn(v);
-    const __half2 p = __halves2half2(h, __float2half_rn((v - __half2float(h)) * kLoScale));
-    return *reinterpret_cast<const unsigned *>(&p);
-}
-
-// The same of two, sharing the conversions.
+// v = hi + lo / 2048 of two, each a pair of fp16 (hi in the low half).
 __device__ __forceinline__ void split_half2(float v0, float v1, unsigned &s0, unsigned &s1) {
     const __half2 h = __floats2half2_rn(v0, v1);
     const float2 f = __half22float2(h);
@@ -1105,17 +1080,8 @@ AttnPlan attn_plan(const g2_kv8 &c, int n_head, int n_seq, int max_q, int sms) {
     return p;
 }
 
-int attn_sms() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-        cudaGetLastError();
-        n = 0;
-    }
-    return n > 0 ? n : 148;
-}
-
 template <int FMT, int D, int NT, int WPR>
-int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
+int launch_attn(const AttnArgs &a, cudaStream_t st) {
     auto kernel = kv8_attention_kernel<FMT, D, NT, WPR>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (AttnRing<D, NT>::template kSmem<FMT, WPR>)) != cudaSuccess)
         return arg_error(G2_ERR_CUDA, "g2k_kv8_attention", cudaGetErrorString(cudaGetLastError()));
@@ -1125,16 +1091,16 @@ int launch_attn(const AttnArgs &a, int sms, cudaStream_t st) {
 }
 
 template <int FMT, int D, int NT>
-int launch_attn(const AttnArgs &a, int wpr, int sms, cudaStream_t st) {
-    return wpr == 2 ? launch_attn<FMT, D, NT, 2>(a, sms, st) : launch_attn<FMT, D, NT, 8>(a, sms, st);
+int launch_attn(const AttnArgs &a, int wpr, cudaStream_t st) {
+    return wpr == 2 ? launch_attn<FMT, D, NT, 2>(a, st) : launch_attn<FMT, D, NT, 8>(a, st);
 }
 
 template <int FMT>
-int launch_attn(const AttnArgs &a, const AttnPlan &p, int sms, cudaStream_t st) {
+int launch_attn(const AttnArgs &a, const AttnPlan &p, cudaStream_t st) {
     if (a.c.head_dim == 64)
-        return p.nt == 1 ? launch_attn<FMT, 64, 1>(a, p.wpr, sms, st)
-             : p.nt == 2 ? launch_attn<FMT, 64, 2>(a, p.wpr, sms, st) : launch_attn<FMT, 64, 4>(a, p.wpr, sms, st);
-    return p.nt == 1 ? launch_attn<FMT, 128, 1>(a, p.wpr, sms, st) : launch_attn<FMT, 128, 2>(a, p.wpr, sms, st);
+        return p.nt == 1 ? launch_attn<FMT, 64, 1>(a, p.wpr, st)
+             : p.nt == 2 ? launch_attn<FMT, 64, 2>(a, p.wpr, st) : launch_attn<FMT, 64, 4>(a, p.wpr, st);
+    return p.nt == 1 ? launch_attn<FMT, 128, 1>(a, p.wpr, st) : launch_attn<FMT, 128, 2>(a, p.wpr, st);
 }
 
 // Positions of a table row: the attention counts up to a unit of keys past the last in 32 bits.
@@ -1264,7 +1230,7 @@ extern "C" int g2k_kv8_gather(const g2_kv8 *cache, void *k_out, void *v_out, int
 // [counters | partial results], each 256-byte aligned; the counters' place does not depend on the call's sizes
 extern "C" size_t g2k_kv8_attention_workspace(const g2_kv8 *cache, int n_head, int n_seq, int max_q) {
     if (!cache || n_head < 1 || n_seq < 0 || max_q < 1 || cache->n_kv_head < 1 || n_head % cache->n_kv_head) return 0;
-    return kMaxWorkers * 4 + attn_plan(*cache, n_head, n_seq, max_q, attn_sms()).part_floats * 4;
+    return kMaxWorkers * 4 + attn_plan(*cache, n_head, n_seq, max_q, sm_count()).part_floats * 4;
 }
 
 extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q_stride, void *out, long long out_stride,
@@ -1296,11 +1262,10 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if ((rc = check_device_ptrs(who, {cache->k, cache->v, cache->k_scale, cache->v_scale, q, out, q_start, seq_len, table,
                                       workspace, status})))
         return rc;
-    const int sms = attn_sms();
-    const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, sms);   // needs no more workspace than max_q's plan
+    const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, sm_count());   // needs no more workspace than max_q's plan
     const AttnArgs a{*cache, q, out, q_stride, out_stride, dtype == G2_F16, n_head / cache->n_kv_head,
                      scale * 1.4426950408889634f, seq_len, r, p.unit, p.ahead, p.workers, static_cast<unsigned *>(workspace),
                      static_cast<float *>(workspace) + kMaxWorkers};
-    return cache->format == G2_KV_I8 ? launch_attn<G2_KV_I8>(a, p, sms, (cudaStream_t)stream)
-                                     : launch_attn<G2_KV_E4M3>(a, p, sms, (cudaStream_t)stream);
+    return cache->format == G2_KV_I8 ? launch_attn<G2_KV_I8>(a, p, (cudaStream_t)stream)
+                                     : launch_attn<G2_KV_E4M3>(a, p, (cudaStream_t)stream);
 }

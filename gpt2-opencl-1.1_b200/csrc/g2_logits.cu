@@ -265,9 +265,7 @@ int check_rules(const char *who, const g2_logit_rules *r, int rows, int vocab, b
 
 cudaError_t launch_rules(const float *logits, long long ld, float *out, long long ld_out, int rows, int vocab,
                          const g2_logit_rules &rules, cudaStream_t st) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = sm_count();
     const int columns = vocab + 3;   // 3: a row that begins past a multiple of 16 bytes
     // equal slices, about eight for each SM over all rows (four: 27.7 us for 256 rows of 50257, eight: 25.6, sixteen: 30.6)
     const int fewest = (columns + kMaxSlice - 1) / kMaxSlice, most = (columns + kMinSlice - 1) / kMinSlice;

@@ -25,6 +25,7 @@
 
 #include "g2_args.h"
 #include "g2_device.cuh"
+#include "g2_mma.cuh"
 
 namespace g2 {
 
@@ -214,28 +215,6 @@ __device__ __forceinline__ float4 load_4(const T *p, int k, int K) {
         if (k + 3 < K) v.w = tof(p[k + 3]);
     }
     return v;
-}
-
-__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(unsigned dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma16832(int (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void mma16816_bf16(float (&c)[4], const unsigned (&w)[4], unsigned b0, unsigned b1) {
@@ -799,17 +778,10 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_matvec_kernel(Q4Args a, Q4Sh
     }
 }
 
-int q4_sms() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
-    return n;
-}
-
 template <typename T, bool VEC, int NT, int TP, int NP, int PC>
 int launch_q4(Q4Args a, const Q4Shape &sh, cudaStream_t st) {
     auto kernel = q4_matvec_kernel<T, VEC, NT, TP, NP, PC>;
-    const int ntiles = sh.tiles / TP, grid = std::min(q4_sms(), ntiles);
+    const int ntiles = sh.tiles / TP, grid = std::min(sm_count(), ntiles);
     a.share = ntiles / grid;
     a.extra = ntiles % grid;
     a.most = std::min((ntiles + grid - 1) / grid, kMaxTiles / TP);
@@ -848,7 +820,7 @@ template <typename T, bool VEC>
 int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     // Two feature tiles share each operand of x, which halves its reads and the loop's own instructions;
     // matrices of fewer pairs than SMs are better spread one by one.
-    const int sms = q4_sms();
+    const int sms = sm_count();
     const bool one = sh.tiles / 2 < sms;
     // Rows in groups of 2, 4 or 8: the fewest that one CTA per SM still holds, since staging x is most of a
     // narrow matrix's time (16 rows of 3974 x 83: 27 us in groups of 8, 7.4 in groups of 2), else as few groups as can be.
