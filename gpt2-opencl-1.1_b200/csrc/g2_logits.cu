@@ -14,9 +14,11 @@
 //   4. The touched columns are computed and written over the copy.  A context touches
 //      about one column in a hundred; testing all of them in the copy took longer
 //      than the copy.
-// Bound by the bytes of the logits, read and written once.  Slices are as long as
-// leaves eight CTAs to an SM: every slice of a row reads the whole context, and with
-// slices of 4096 columns that took longer than the columns (256 rows of 50257: 37 us).
+// Bound by the bytes of the logits, read and written once, and by what each CTA does
+// before its copy is all on its way.  Rows are cut into about eight slices for each
+// SM, of which five run at a time (256 threads of 48 registers): every slice of a row
+// reads the whole context, and with slices of 4096 columns that took longer than the
+// columns (256 rows of 50257: 37 us).
 #include <algorithm>
 
 #include "g2_args.h"
@@ -267,7 +269,8 @@ cudaError_t launch_rules(const float *logits, long long ld, float *out, long lon
                          const g2_logit_rules &rules, cudaStream_t st) {
     const int sms = sm_count();
     const int columns = vocab + 3;   // 3: a row that begins past a multiple of 16 bytes
-    // equal slices, about eight for each SM over all rows (four: 27.7 us for 256 rows of 50257, eight: 25.6, sixteen: 30.6)
+    // equal slices, about eight for each SM over all rows, in waves of five (256 rows of 50257: four 27.7 us, one wave;
+    // eight 25.6, two waves of which the second is 73% full; sixteen 30.6)
     const int fewest = (columns + kMaxSlice - 1) / kMaxSlice, most = (columns + kMinSlice - 1) / kMinSlice;
     const int slices = std::min(std::max((8 * sms + rows - 1) / rows, fewest), most);
     const int slice = ((columns + slices - 1) / slices + 127) / 128 * 128;

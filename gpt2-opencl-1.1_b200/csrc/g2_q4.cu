@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(const unsigned char *pac
 //           row's largest, one column for each of its bytes, NP bytes in an n tile.
 //           Codes times bytes are summed exactly in int32, and unpacking eight codes
 //           costs three instructions.  Up to four rows have eight bytes (61 bits, so
-//           that an x' 2^37 below the largest still has its own 24); three or four of
-//           fp16 six (46 bits, more than fp16 spans).  Four bytes took 6.9 us for 4 rows
+//           that an x' 2^37 below the largest still has its own 24); groups of three or
+//           four fp16 rows with LayerNorm six (46 bits, more than fp16 spans).  Four bytes took 6.9 us for 4 rows
 //           of 1600 x 6400 with LayerNorm, where eight take 7.9, and 14.7 and 18.1 for
 //           1600 x 50257, but left 10 bits of a value 2^20 below the largest.  Leaving the
 //           lower bytes out where no x' needs them, by a second loop or a second pass, cost
@@ -823,7 +823,7 @@ int launch_q4(const Q4Args &a, const Q4Shape &sh, cudaStream_t st) {
     const int sms = sm_count();
     const bool one = sh.tiles / 2 < sms;
     // Rows in groups of 2, 4 or 8: the fewest that one CTA per SM still holds, since staging x is most of a
-    // narrow matrix's time (16 rows of 3974 x 83: 27 us in groups of 8, 7.4 in groups of 2), else as few groups as can be.
+    // narrow matrix's time (16 rows of 3974 x 83: 27 us in groups of 8, 5.8 in groups of 2), else as few groups as can be.
     const auto fits = [&](int rows) { return sh.tiles * ((a.M + rows - 1) / rows) <= sms; };
     if constexpr (sizeof(T) == 2)
         if (!a.gamma && a.M > 2 && !(a.M > 8 && fits(2)))

@@ -260,7 +260,7 @@ int g2k_q4_unpack(const void *packed, float *W, int N, int K, int group, void *s
  * x [M][K], y and residual [M][N] are of `dtype` (G2_F32 or G2_F16); bias,
  * ln_gamma and ln_beta are fp32.  Products are exact and sums fp32 or int32; an
  * x' is carried exactly but for what lies below 2^-60 of its row's largest (2^-44
- * for three or four fp16 rows with LayerNorm) or below 2^-117, so a column whose
+ * for more than two fp16 rows with LayerNorm) or below 2^-117, so a column whose
  * codes are 0 at a row's large values keeps its accuracy.  A row's last bits may
  * differ with the number of rows and N.  Weights are below 2^76: sums past
  * that may overflow.  A non-finite x' makes its row's outputs non-finite, and no
