@@ -1242,7 +1242,8 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
     if ((rc = check_cache(who, cache))) return rc;
     if (n_head < 1 || n_head % cache->n_kv_head || n_head > 65535)
         return arg_error(G2_ERR_RANGE, who, "n_head must be a multiple of n_kv_head, at most 65535");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return arg_error(G2_ERR_ARG, who, "scale must be positive");
+    constexpr float kLog2e = 1.4426950408889634f;
+    if (!(scale > 0.0f) || !std::isfinite(scale * kLog2e)) return arg_error(G2_ERR_ARG, who, "scale must be positive and at most 2.3e38");
     Rows8 r{n_rows, n_seq, max_q, q_start, table, table_stride, status};
     if ((rc = check_rows(who, cache, n_head, q, out, dtype, &q_stride, &out_stride, r, seq_len))) return rc;
     r.max_q = bound_rows(max_q, n_rows);
@@ -1264,7 +1265,7 @@ extern "C" int g2k_kv8_attention(const g2_kv8 *cache, const void *q, long long q
         return rc;
     const AttnPlan p = attn_plan(*cache, n_head, n_seq, r.max_q, sm_count());   // needs no more workspace than max_q's plan
     const AttnArgs a{*cache, q, out, q_stride, out_stride, dtype == G2_F16, n_head / cache->n_kv_head,
-                     scale * 1.4426950408889634f, seq_len, r, p.unit, p.ahead, p.workers, static_cast<unsigned *>(workspace),
+                     scale * kLog2e, seq_len, r, p.unit, p.ahead, p.workers, static_cast<unsigned *>(workspace),
                      static_cast<float *>(workspace) + kMaxWorkers};
     return cache->format == G2_KV_I8 ? launch_attn<G2_KV_I8>(a, p, (cudaStream_t)stream)
                                      : launch_attn<G2_KV_E4M3>(a, p, (cudaStream_t)stream);

@@ -70,6 +70,13 @@ def test_work_goes_by_the_rows_there_are():
     assert code(lambda: f(cache(n_kv_head=8), dict(call, n_seq=2 ** 22, n_rows=2 ** 22))) == -6
 
 
+def test_largest_scale():
+    """A scale that passes fp32's range in powers of two (times log2 e) would make every score infinite or NaN."""
+    f = CALLS["attention"]
+    assert code(lambda: f(cache(), dict(scale=3.0e38))) == -1
+    assert code(lambda: f(cache(), dict(scale=2.3e38))) == no_device_memory()
+
+
 @pytest.mark.gpu
 def test_2_27_runs():
     """So many (sequence, head) runs that 32 of each pass 32 bits: every output is written."""
